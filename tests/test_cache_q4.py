@@ -1,0 +1,127 @@
+"""A cache in 4 bits, without a device: the format, what its entry points refuse, what the memory plan counts."""
+import numpy as np
+import pytest
+import torch
+
+import plain_q4 as plain
+
+
+def test_a_group_keeps_its_largest_value_to_a_64th_and_the_others_to_half_a_step():
+    rng = np.random.default_rng(3)
+    x = (rng.standard_normal((50, 128)) * np.exp(rng.standard_normal((50, 1)) * 3)).astype(np.float32)
+    codes, scales = plain.quantise(x)
+    back = plain.stand_for(codes, scales).reshape(50, 4, 32)
+    groups = x.reshape(50, 4, 32).astype(np.float64)
+    largest = np.abs(groups).max(-1, keepdims=True)
+    step = np.abs(scales)[..., None]
+    # the largest value lies on code -8 but for the scale's rounding, half of 1/16 of it at most; what passes +7 steps is cut there
+    assert (np.abs(back - groups) <= np.where(np.abs(groups) == largest, largest / 32, np.maximum(step / 2, np.abs(groups) - 7 * step) + 1e-12)).all()
+    assert codes.min() == -8 and codes.max() <= 7
+
+
+def test_what_a_row_stands_for_is_a_bfloat16_exactly():
+    rng = np.random.default_rng(4)
+    values = plain.stand_for(*plain.quantise((rng.standard_normal((200, 256)) * 7).astype(np.float32)))
+    assert np.array_equal(torch.from_numpy(values).to(torch.bfloat16).double().numpy(), values)
+
+
+@pytest.mark.parametrize("keys", [True, False])
+@pytest.mark.parametrize("d", [32, 64, 96, 128, 256])
+def test_packing_and_unpacking_agree_and_use_every_nibble_once(keys, d):
+    codes = np.random.default_rng(5).integers(-8, 8, size=(3, 7, d // 32, 32))
+    packed = plain.pack(codes, keys)
+    assert packed.shape == (3, 7, d // 2)
+    assert np.array_equal(plain.unpack(packed, keys), codes)
+
+
+def _pages(ops, pages=3, page_size=16, kv_heads=2, d=64):
+    u8 = dict(dtype=torch.uint8)
+    return ops.Q4Pages(torch.zeros(pages, kv_heads, page_size, d // 2, **u8),
+                       torch.zeros(pages, kv_heads, page_size, d // 32, dtype=torch.bfloat16),
+                       torch.zeros(pages, kv_heads, page_size, d // 2, **u8),
+                       torch.zeros(pages, kv_heads, page_size, d // 32, dtype=torch.bfloat16))
+
+
+@pytest.fixture
+def entry_points(monkeypatch):
+    """The wrappers with the kernels' libraries out of reach: what they refuse, they refuse before a launch."""
+    import vipera_rs_b200  # noqa: F401
+    from vipera_rs_b200.kernels import ops
+
+    def no_launch(*_):
+        raise AssertionError("launched")
+
+    monkeypatch.setattr(ops, "_function", lambda *_: no_launch)
+    monkeypatch.setattr(ops, "_check_struct", lambda *_: None)
+    monkeypatch.setattr(ops, "_one_device", lambda *_: None)
+    return ops
+
+
+def _int(*values):
+    return torch.tensor(values, dtype=torch.int32)
+
+
+def test_step_maps_refuses_lengths_that_do_not_agree(entry_points):
+    from vipera_rs_b200.errors import InvalidArgumentError
+
+    ops = entry_points
+    table = torch.zeros(2, 4, dtype=torch.int32)
+    good = dict(page_size=16, block_table=table, page_starts=_int(0, 1, 2), pages=_int(0, 1), slots=torch.zeros(5, dtype=torch.int32))
+    starts, pos0 = _int(0, 2, 5), _int(0, 9)
+    for change in (dict(page_size=0), dict(block_table=table[:1]), dict(page_starts=None), dict(pages=None),
+                   dict(page_starts=_int(0, 1)), dict(positions=torch.zeros(4, dtype=torch.int32))):
+        with pytest.raises(InvalidArgumentError):
+            ops.step_maps(starts, pos0, **{**good, **change})
+    with pytest.raises(InvalidArgumentError):
+        ops.step_maps(_int(0, 2), pos0, **good)
+
+
+def test_rope_cache_q4_refuses_shapes_and_sizes_it_does_not_take(entry_points):
+    from vipera_rs_b200.errors import InvalidArgumentError, UnsupportedError
+
+    ops = entry_points
+    good = dict(num_heads=4, num_kv_heads=2, head_dim=64, positions=_int(0, 1, 2), cos=torch.zeros(8, 32), sin=torch.zeros(8, 32),
+                style=ops.ROPE_NEOX, slots=_int(0, 1, 2))
+    qkv, q = torch.zeros(3, 8 * 64), torch.zeros(3, 4 * 64)
+    for change in (dict(positions=_int(0)), dict(slots=_int(0)), dict(rot_dims=33), dict(rot_dims=66), dict(cos=None),
+                   dict(cos=torch.zeros(8, 16)), dict(num_kv_heads=3), dict(cos=torch.zeros(0, 32), sin=torch.zeros(0, 32))):
+        with pytest.raises(InvalidArgumentError):
+            ops.rope_cache_q4(qkv, q, _pages(ops), **{**good, **change})
+    for bad_qkv, bad_q in ((qkv[:, :-1], q), (qkv.t(), q), (qkv, q[:2]), (qkv.double(), q), (qkv, q)):   # the last: not on a device
+        with pytest.raises(InvalidArgumentError):
+            ops.rope_cache_q4(bad_qkv, bad_q, _pages(ops), **good)
+    with pytest.raises(UnsupportedError):
+        ops.rope_cache_q4(torch.zeros(3, 8 * 48), torch.zeros(3, 4 * 48), _pages(ops), **{**good, "head_dim": 48})
+    bad = _pages(ops)._replace(v_scales=torch.zeros(3, 2, 16, 4, dtype=torch.bfloat16))
+    with pytest.raises(InvalidArgumentError):
+        ops.rope_cache_q4(qkv, q, bad, **good)
+
+
+def test_expand_q4_refuses_rooms_of_another_cache(entry_points):
+    from vipera_rs_b200.errors import InvalidArgumentError
+
+    ops = entry_points
+    room = torch.zeros(3, 16, 2, 64)
+    good = dict(entry_starts=_int(0, 1), entry_pos0=_int(4), block_table=torch.zeros(1, 2, dtype=torch.int32))
+    for k, v in ((room, room[:2]), (room, room.double()), (room[:2], room[:2]), (room[:, :8], room[:, :8])):
+        with pytest.raises(InvalidArgumentError):
+            ops.expand_q4(_pages(ops), k, v, **good)
+    with pytest.raises(InvalidArgumentError):
+        ops.expand_q4(_pages(ops), room, room, **{**good, "entry_starts": _int(0)})
+
+
+def test_attention_q4_refuses_steps_that_do_not_agree(entry_points):
+    from vipera_rs_b200.errors import InvalidArgumentError
+
+    ops = entry_points
+    q = torch.zeros(3, 4 * 64, dtype=torch.bfloat16)
+    good = dict(entry_starts=_int(0, 1, 3), entry_pos0=_int(5, 0), positions=_int(5, 0, 1), token_entry=_int(0, 1, 1),
+                block_table=torch.zeros(2, 2, dtype=torch.int32), num_heads=4, num_kv_heads=2, head_dim=64, scale=0.125, max_keys=6,
+                all_single=False, any_single=True, workspace=None)
+    for change in (dict(num_heads=3), dict(entry_starts=_int(0, 3)), dict(all_single=True), dict(positions=_int(5)),
+                   dict(max_keys=0), dict(max_keys=33), dict(window=-1), dict(sink_values=torch.zeros(3)), dict(keep_first=-2),
+                   dict(block_table=torch.zeros(1, 2, dtype=torch.int32))):
+        with pytest.raises(InvalidArgumentError):
+            ops.attention_q4(q, torch.zeros_like(q), _pages(ops), **{**good, **change})
+    with pytest.raises(InvalidArgumentError):
+        ops.attention_q4(q, torch.zeros(3, 4 * 64), _pages(ops), **good)

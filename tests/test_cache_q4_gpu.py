@@ -1,0 +1,392 @@
+"""Operators of the 4-bit cache on the device against their definitions in 64 bits."""
+import numpy as np
+import pytest
+import torch
+
+import plain_q4 as plain
+
+pytestmark = pytest.mark.gpu
+DEVICE = "cuda:0"
+
+
+@pytest.fixture(scope="module")
+def ops():
+    import vipera_rs_b200  # noqa: F401
+    from vipera_rs_b200.kernels import ops
+
+    return ops
+
+
+def _workspace():
+    from vipera_rs_b200.parts.base import Workspace
+
+    return Workspace(DEVICE)
+
+
+def _int(values):
+    return torch.tensor(values, dtype=torch.int32, device=DEVICE)
+
+
+class Step:
+    """A step's description: lengths, pages in random order, block tables, and the maps of its tokens."""
+
+    def __init__(self, counts, history, page_size, seed=0, spare=3, width=None):
+        rng = np.random.default_rng(seed)
+        self.counts, self.history, self.page_size = counts, history, page_size
+        self.held = [-(-(c + h) // page_size) for c, h in zip(counts, history)]
+        self.num_pages = sum(self.held) + spare
+        order = rng.permutation(self.num_pages)
+        self.tables, at = [], 0
+        width = width or max(self.held + [1])
+        self.pages = order[:sum(self.held)]
+        for n in self.held:
+            self.tables.append([int(x) for x in order[at:at + n]] + [-1] * (width - n))
+            at += n
+        self.starts = np.concatenate([[0], np.cumsum(counts)]).astype(int)
+        self.positions = [h + i for c, h in zip(counts, history) for i in range(c)]
+        self.entry = [e for e, c in enumerate(counts) for _ in range(c)]
+        self.slots = [self.tables[e][p // page_size] * page_size + p % page_size for e, p in zip(self.entry, self.positions)]
+
+    def device(self):
+        return dict(entry_starts=_int(self.starts), entry_pos0=_int(self.history), positions=_int(self.positions),
+                    token_entry=_int(self.entry), block_table=_int(self.tables),
+                    max_keys=max(c + h for c, h in zip(self.counts, self.history)), all_single=all(c == 1 for c in self.counts),
+                    any_single=any(c == 1 for c in self.counts))
+
+
+@pytest.mark.parametrize("page_size", [1, 7, 16, 64])
+@pytest.mark.parametrize("counts, history", [
+    ([1], [0]), ([1, 1, 1], [5, 0, 100]), ([3, 1, 200], [0, 63, 17]), ([0, 2, 0, 1, 0], [0, 3, 9, 0, 0]), ([700], [1]),
+    ([1] * 70, list(range(70)))])
+def test_maps_are_those_of_the_lengths(ops, page_size, counts, history):
+    step = Step(counts, history, page_size, width=60 if page_size >= 16 else None)
+    tokens = len(step.positions)
+    table = torch.full((len(counts), len(step.tables[0])), 77, dtype=torch.int32, device=DEVICE)
+    out = {name: torch.full((tokens + 3,), 77, dtype=torch.int32, device=DEVICE) for name in ("positions", "token_entry", "slots")}
+    page_starts = _int(np.concatenate([[0], np.cumsum(step.held)]))
+    ops.step_maps(_int(step.starts), _int(history), page_size=page_size, page_starts=page_starts, pages=_int(step.pages),
+                  block_table=table, **out)
+    assert table.tolist() == step.tables
+    for name, expected in (("positions", step.positions), ("token_entry", step.entry), ("slots", step.slots)):
+        assert out[name].tolist() == expected + [77] * 3       # what lies behind the last token stays
+    again = torch.full_like(out["slots"], 77)
+    ops.step_maps(_int(step.starts), _int(history), page_size=page_size, block_table=table, slots=again)   # from the tables alone
+    assert again.tolist() == step.slots + [77] * 3
+    assert table.tolist() == step.tables
+
+
+def test_maps_where_pages_are_missing_or_tables_are_short(ops):
+    table = torch.zeros(2, 2, dtype=torch.int32, device=DEVICE)
+    slots = torch.zeros(6, dtype=torch.int32, device=DEVICE)
+    # the first holds one page of the two that its tokens need, the second three where the table has room for two
+    ops.step_maps(_int([0, 3, 6]), _int([2, 7]), page_size=4, page_starts=_int([0, 1, 4]), pages=_int([5, 1, 2, 9]), block_table=table,
+                  slots=slots)
+    assert table.tolist() == [[5, -1], [1, 2]]
+    assert slots.tolist() == [22, 23, -1, 11, 36, 37]
+    ops.step_maps(_int([0, 3, 6]), _int([2, 7]), page_size=4, block_table=table, slots=slots)
+    assert slots.tolist() == [22, 23, -1, 11, -1, -1]
+    ops.step_maps(_int([0]), _int([]), page_size=4, block_table=table[:0], slots=slots[:0])   # a step of nothing
+
+
+def _turn(x, cos, sin, rot, interleaved):
+    """The rotation in 32 bits, every product and sum rounded by itself (numpy does not fuse)."""
+    x = x.astype(np.float32).copy()
+    half = rot // 2
+    first = 2 * np.arange(half) if interleaved else np.arange(half)
+    second = first + 1 if interleaved else first + half
+    a, b = x[..., first].copy(), x[..., second].copy()
+    c, s = cos[:, None, :], sin[:, None, :]
+    x[..., first], x[..., second] = a * c - b * s, a * s + b * c
+    return x
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads, kv_heads, d, rot, style, extra", [
+    (4, 2, 64, 64, "neox", 0), (12, 2, 128, 128, "neox", 0), (5, 1, 128, 64, "neox", 4), (3, 3, 96, 96, "interleaved", 0),
+    (2, 1, 32, 6, "interleaved", 3), (2, 1, 32, 20, "neox", 0), (2, 2, 256, 256, "neox", 1), (7, 1, 64, 0, "neox", 0),
+    (4, 4, 64, 64, "none", 0)])
+def test_keys_and_values_are_the_nearest_codes(ops, dtype, heads, kv_heads, d, rot, style, extra):
+    step = Step([1, 37, 2], [40, 0, 15], 16, seed=d + rot)
+    tokens = len(step.positions)
+    rng = np.random.default_rng(d)
+    x = (rng.standard_normal((tokens, heads + 2 * kv_heads, d)) * np.exp(rng.standard_normal(d))).astype(np.float32)
+    x[3, heads, :32] = 0.0                       # a group of zeros
+    x[4, heads + kv_heads, 5] = np.nan           # groups that are not finite show as a whole
+    x[5, heads + kv_heads, 7] = -np.inf
+    x[6, heads + kv_heads, :32] *= np.float32(1e-42) / 3    # a group whose scale has no bits left
+    x[7, heads + kv_heads, :32] *= np.float32(2.0 ** 100)
+    x[8, heads + kv_heads, :32] = 3.0            # all alike
+    x[9, heads + kv_heads, :4] = [2.0, -2.0, 1.875, -1.875]
+    angles = np.arange(64)[:, None] * 10000.0 ** (-np.arange(max(rot // 2, 1)) / max(rot // 2, 1))
+    cos, sin = np.cos(angles).astype(np.float32), np.sin(angles).astype(np.float32)
+    turned = x.copy()
+    if style != "none" and rot:
+        turned[:, :heads + kv_heads] = _turn(x[:, :heads + kv_heads], cos[step.positions], sin[step.positions], rot, style == "interleaved")
+    qkv = torch.full((tokens, x[0].size + extra), 9e9, dtype=torch.float32, device=DEVICE)
+    qkv[:, :x[0].size] = torch.from_numpy(x.reshape(tokens, -1)).to(DEVICE)
+    pages = ops.Q4Pages(*plain.make_pages(step.num_pages, 16, kv_heads, d, 1, DEVICE))
+    before = [t.clone() for t in pages]
+    q_out = torch.zeros(tokens, heads * d, dtype=dtype, device=DEVICE)
+    slots = _int(step.slots)
+    slots[2] = -1                                # not written
+    slots[10] = step.num_pages * 16              # nor is a slot outside the pool
+    tables = [torch.from_numpy(t[:, :rot // 2].copy()).to(DEVICE) if rot else None for t in (cos, sin)]
+    ops.rope_cache_q4(qkv, q_out, pages, num_heads=heads, num_kv_heads=kv_heads, head_dim=d, rot_dims=rot, positions=_int(step.positions),
+                      cos=tables[0], sin=tables[1], slots=slots,
+                      style={"neox": ops.ROPE_NEOX, "interleaved": ops.ROPE_INTERLEAVED, "none": ops.ROPE_NONE}[style])
+    expected_q = torch.from_numpy(turned[:, :heads].reshape(tokens, -1)).to(dtype)
+    assert torch.equal(q_out.cpu(), expected_q)
+    written = [t for t in range(tokens) if t not in (2, 10)]
+    for which, keys in ((0, True), (1, False)):
+        codes, scales = plain.quantise(turned[written, heads + which * kv_heads:heads + (which + 1) * kv_heads])
+        tiny = np.abs(scales) < 2.0 ** -126       # 19 bits go there too, of a number that has fewer
+        expected_codes, expected_scales = before[2 * which].cpu().numpy().copy(), before[2 * which + 1].float().cpu().numpy().copy()
+        got_codes, got_scales = pages[2 * which].cpu().numpy(), pages[2 * which + 1].float().cpu().numpy()
+        at = np.asarray([step.slots[t] for t in written])
+        page, place = at // 16, at % 16
+        if tiny.any():
+            assert np.abs(got_scales[page, :, place][tiny]).max() < 2.0 ** -126
+            scales = np.where(tiny, got_scales[page, :, place], scales)
+            codes = np.where(tiny[..., None], plain.unpack(got_codes[page, :, place], keys), codes)
+        expected_codes[page, :, place] = plain.pack(codes, keys)
+        expected_scales[page, :, place] = scales
+        assert np.array_equal(got_codes, expected_codes)
+        assert np.array_equal(got_scales, expected_scales, equal_nan=True)
+
+
+def test_queries_alone_leave_the_pages(ops):
+    step = Step([3], [0], 16)
+    pages = ops.Q4Pages(*plain.make_pages(step.num_pages, 16, 1, 64, 1, DEVICE))
+    before = [t.clone() for t in pages]
+    qkv = torch.randn(3, 4 * 64, device=DEVICE)
+    q = torch.zeros(3, 2 * 64, device=DEVICE)
+    ops.rope_cache_q4(qkv, q, pages, num_heads=2, num_kv_heads=1, head_dim=64, positions=_int([0, 1, 2]), cos=None, sin=None,
+                      style=ops.ROPE_NONE, slots=None)
+    assert torch.equal(q, qkv[:, :128]) and all(torch.equal(a, b) for a, b in zip(pages, before))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("page_size, kv_heads, d, window, keep_first, skip", [
+    (16, 2, 128, 0, 0, False), (16, 1, 64, 20, 3, False), (5, 3, 96, 33, 40, True), (32, 2, 32, 1, 0, False), (16, 2, 256, 50, 17, True)])
+def test_rows_are_read_back_where_the_step_sees_them(ops, dtype, page_size, kv_heads, d, window, keep_first, skip):
+    counts, history = [1, 30, 0, 5, 1], [90, 61, 10, 0, 0]
+    step = Step(counts, history, page_size, seed=3)
+    raw = plain.make_pages(step.num_pages, page_size, kv_heads, d, 2, DEVICE)
+    raw[1][0, 0, 0, 0] = float("nan")
+    pages = ops.Q4Pages(*raw)
+    rooms = [torch.full((step.num_pages, page_size, kv_heads, d), 5.5, dtype=dtype, device=DEVICE) for _ in range(2)]
+    described = step.device()
+    ops.expand_q4(pages, *rooms, window=window, keep_first=keep_first, skip_single=skip,
+                  **{name: described[name] for name in ("entry_starts", "entry_pos0", "block_table")})
+    seen = np.zeros((step.num_pages, page_size), dtype=bool)
+    for e, (count, held) in enumerate(zip(counts, history)):
+        if count == 0 or (skip and count == 1):
+            continue
+        first = max(0, held - window + 1) if window else 0
+        for j in range(held + count):
+            if j >= first or (window and j < keep_first):
+                seen[step.tables[e][j // page_size], j % page_size] = True
+    for room, (codes, scales), keys in ((rooms[0], pages[:2], True), (rooms[1], pages[2:], False)):
+        rows = np.swapaxes(plain.rows_of(codes, scales, keys), 1, 2)
+        expected = np.where(seen[:, :, None, None], rows, 5.5)
+        assert np.array_equal(room.double().cpu().numpy(), expected, equal_nan=True)
+
+
+def _hide(step, pages, window=0, keep_first=0):
+    """NaN in every row that no token of the step sees, and tables that name no page where a window has left one behind."""
+    seen = np.zeros((step.num_pages, step.page_size), dtype=bool)
+    for e, (count, held) in enumerate(zip(step.counts, step.history)):
+        for j in range(held + count):
+            if not window or j > held - window or j < keep_first:
+                seen[step.tables[e][j // step.page_size], j % step.page_size] = True
+        for index, page in enumerate(step.tables[e]):
+            if page >= 0 and window and not any(index * step.page_size <= j < (index + 1) * step.page_size
+                                                for j in range(held + count) if j > held - window or j < keep_first):
+                step.tables[e][index] = -1
+    hidden = torch.from_numpy(~seen).to(DEVICE)[:, None, :, None]
+    for scales in (pages.k_scales, pages.v_scales):
+        scales.masked_fill_(hidden, float("nan"))
+
+
+def _attend(ops, step, dtype, heads, kv_heads, d, seed=0, window=0, keep_first=0, sink=False, sink_values=None, gate=None,
+            gate_per_head=False, workspace=None):
+    raw = plain.make_pages(step.num_pages, step.page_size, kv_heads, d, seed + 10, DEVICE)
+    k_rows, v_rows = plain.rows_of(raw[0], raw[1], True), plain.rows_of(raw[2], raw[3], False)
+    pages = ops.Q4Pages(*raw)
+    tables = [list(row) for row in step.tables]
+    _hide(step, pages, window, keep_first)
+    tokens = len(step.positions)
+    generator = torch.Generator().manual_seed(seed)
+    q = (torch.randn(tokens, heads * d, generator=generator) * 1.5).to(dtype)
+    out = torch.full((tokens + 2, heads * d), 7.0, dtype=dtype, device=DEVICE)
+    scale = d ** -0.5
+    gates = None if gate is None else torch.from_numpy(np.concatenate([np.full((tokens, 4), 9.0, dtype=np.float32), gate], 1)).to(DEVICE)
+    ops.attention_q4(q.to(DEVICE), out[:tokens], pages, num_heads=heads, num_kv_heads=kv_heads, head_dim=d, scale=scale,
+                     workspace=workspace or _workspace(), window=window, keep_first=keep_first, sink=sink,
+                     sink_values=None if sink_values is None else torch.from_numpy(sink_values).to(DEVICE),
+                     gate=gates, gate_offset=4, gate_per_head=gate_per_head, **step.device())
+    expected, spread, reach = plain.attend(q.double().numpy(), k_rows, v_rows, counts=step.counts, history=step.history, tables=tables,
+                                           page_size=step.page_size, num_heads=heads, num_kv_heads=kv_heads, d=d, scale=scale,
+                                           window=window, keep_first=keep_first, sink=sink, sink_values=sink_values, gate=gate)
+    got = out[:tokens].double().cpu().numpy().reshape(expected.shape)
+    keys = max(c + h for c, h in zip(step.counts, step.history))
+    limit = plain.allowed(expected, spread, reach, keys, d, dtype)
+    assert np.isfinite(got).all()
+    worst = (np.abs(got - expected) / limit).max()
+    assert worst <= 1.0, worst
+    assert (out[tokens:] == 7.0).all()          # rows behind the step's last token
+
+
+@pytest.mark.parametrize("heads, kv_heads, d", [(12, 2, 128), (14, 2, 64), (4, 4, 128), (20, 1, 128), (5, 1, 64), (16, 1, 64), (40, 2, 64)])
+@pytest.mark.parametrize("history", [[0], [15, 16, 17, 0, 31], [300, 127, 128, 1, 129]])
+def test_single_tokens_over_packed_pages(ops, heads, kv_heads, d, history):
+    _attend(ops, Step([1] * len(history), history, 16, seed=heads), torch.bfloat16, heads, kv_heads, d)
+
+
+@pytest.mark.parametrize("page_size", [32, 48, 64])
+def test_single_tokens_over_pages_of_other_sizes(ops, page_size):
+    _attend(ops, Step([1, 1], [200, 47], page_size), torch.bfloat16, 6, 2, 128)
+
+
+@pytest.mark.parametrize("window, keep_first", [(1, 0), (16, 0), (100, 4), (40, 37), (1000, 5), (33, 64)])
+@pytest.mark.parametrize("sink", [False, True])
+@pytest.mark.parametrize("d", [64, 128])
+def test_windows_kept_keys_and_sinks(ops, window, keep_first, sink, d):
+    _attend(ops, Step([1, 1, 1], [300, 39, 0], 16, seed=window), torch.bfloat16, 8, 2, d, window=window, keep_first=keep_first, sink=sink)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("counts, history", [([1, 1], [70, 3]), ([20, 1, 40], [33, 64, 0])])
+@pytest.mark.parametrize("per_head", [False, True])
+@pytest.mark.parametrize("keep_first", [0, 4])
+def test_learned_sinks_and_gates(ops, dtype, counts, history, per_head, keep_first):
+    heads, d = 4, 64
+    rng = np.random.default_rng(8)
+    gate = rng.standard_normal((sum(counts), heads * (1 if per_head else d))).astype(np.float32)
+    sinks = rng.standard_normal(heads).astype(np.float32)
+    _attend(ops, Step(counts, history, 16), dtype, heads, 2, d, sink=True, sink_values=sinks, gate=gate, gate_per_head=per_head,
+            window=50 if keep_first else 0, keep_first=keep_first)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads, kv_heads, d, page_size", [(6, 2, 128, 16), (7, 1, 64, 32), (4, 2, 96, 16), (3, 3, 32, 5), (2, 1, 256, 16), (6, 2, 64, 24)])
+@pytest.mark.parametrize("counts, history, window", [([50], [0], 0), ([1, 33, 1, 2], [40, 70, 0, 15], 0), ([20, 1], [100, 64], 30)])
+def test_portions_and_mixed_steps(ops, dtype, heads, kv_heads, d, page_size, counts, history, window):
+    _attend(ops, Step(counts, history, page_size, seed=d), dtype, heads, kv_heads, d, window=window)
+
+
+def test_a_long_history_in_many_splits(ops):
+    """Thousands of keys, the longest beside a short one."""
+    _attend(ops, Step([1, 1], [9000, 5], 16), torch.bfloat16, 2, 1, 64)
+
+
+def test_values_that_are_not_finite_show_where_they_are_seen(ops):
+    """A NaN key or value makes the outputs of the tokens that see it NaN, and of no others."""
+    for which in ("k_scales", "v_scales"):
+        step = Step([1, 1, 1], [200, 40, 40], 16)
+        pages = ops.Q4Pages(*plain.make_pages(step.num_pages, 16, 1, 64, 3, DEVICE))
+        getattr(pages, which)[step.tables[1][40 // 16], 0, 40 % 16] = float("nan")     # the second's own token
+        q = torch.randn(3, 4 * 64, device=DEVICE).to(torch.bfloat16)
+        out = torch.zeros_like(q)
+        ops.attention_q4(q, out, pages, num_heads=4, num_kv_heads=1, head_dim=64, scale=0.125, workspace=_workspace(), **step.device())
+        assert out[1].isnan().all() and out[[0, 2]].isfinite().all()
+    # every key of a whole split is NaN
+    step = Step([1], [700], 16)
+    pages = ops.Q4Pages(*plain.make_pages(step.num_pages, 16, 1, 64, 3, DEVICE))
+    for index in range(8):
+        pages.k_scales[step.tables[0][index]] = float("nan")
+    q = torch.randn(1, 4 * 64, device=DEVICE).to(torch.bfloat16)
+    out = torch.zeros_like(q)
+    ops.attention_q4(q, out, pages, num_heads=4, num_kv_heads=1, head_dim=64, scale=0.125, workspace=_workspace(), **step.device())
+    assert out.isnan().all()
+
+
+def test_scores_of_zero_and_equal_keys_give_the_mean(ops):
+    """A query of zeros weighs its keys alike: scores whose maximum is exactly 0."""
+    step = Step([1], [99], 16)
+    pages = ops.Q4Pages(*plain.make_pages(step.num_pages, 16, 1, 64, 4, DEVICE))
+    q = torch.zeros(1, 2 * 64, dtype=torch.bfloat16, device=DEVICE)
+    out = torch.zeros_like(q)
+    ops.attention_q4(q, out, pages, num_heads=2, num_kv_heads=1, head_dim=64, scale=0.125, workspace=_workspace(), **step.device())
+    v = plain.rows_of(pages.v_codes, pages.v_scales, False)[:, 0]
+    seen = np.stack([v[step.tables[0][j // 16], j % 16] for j in range(100)])
+    got = out.double().cpu().numpy().reshape(2, 64)
+    # weights of 1 are exact, times a scale too: the sums in 32 bits and the output's rounding are left
+    limit = np.abs(seen).mean(0) * 2.0 ** -14 + np.abs(seen.mean(0)) * 2.0 ** -8
+    assert (np.abs(got - seen.mean(0)) <= limit).all()
+
+
+def test_a_step_as_it_is_used_eager_captured_and_on_a_stream_of_its_own(ops):
+    """Maps, write and attention in a row, step after step: captured and replayed they give the eager run's bits, and the cache's
+    rows those of the keys and values that went in."""
+    heads, kv_heads, d, page = 6, 2, 128, 16
+    counts, history = [40, 1, 9], [0, 0, 0]
+    rng = np.random.default_rng(6)
+
+    def steps():
+        held = [0, 0, 0]
+        for number in range(4):
+            now = counts if number == 0 else [1, 1, 1]
+            yield now, list(held)
+            held = [h + c for h, c in zip(held, now)]
+
+    table_pages = rng.permutation(30)
+    inputs = [rng.standard_normal((sum(c), (heads + 2 * kv_heads) * d)).astype(np.float32) for c, _ in steps()]
+    cos = torch.from_numpy(np.cos(np.arange(64)[:, None] * 0.1 ** np.arange(64)).astype(np.float32)).to(DEVICE)
+    sin = torch.from_numpy(np.sin(np.arange(64)[:, None] * 0.1 ** np.arange(64)).astype(np.float32)).to(DEVICE)
+
+    def play(captured):
+        pages = ops.Q4Pages(*[t.clone().zero_() for t in plain.make_pages(30, page, kv_heads, d, 0, DEVICE)])
+        workspace = _workspace()
+        outs = []
+        for (now, held), x in zip(steps(), inputs):
+            tokens = sum(now)
+            need = [-(-(h + c) // page) for h, c in zip(held, now)]
+            lists = [table_pages[e * 10:e * 10 + n] for e, n in enumerate(need)]
+            starts, pos0 = _int(np.concatenate([[0], np.cumsum(now)])), _int(held)
+            page_starts, page_list = _int(np.concatenate([[0], np.cumsum(need)])), _int(np.concatenate(lists))
+            table = torch.empty(3, 4, dtype=torch.int32, device=DEVICE)
+            maps = {n: torch.empty(tokens, dtype=torch.int32, device=DEVICE) for n in ("positions", "token_entry", "slots")}
+            qkv = torch.from_numpy(x).to(DEVICE)
+            q, out = (torch.zeros(tokens, heads * d, dtype=torch.bfloat16, device=DEVICE) for _ in range(2))
+
+            def one():
+                ops.step_maps(starts, pos0, page_size=page, page_starts=page_starts, pages=page_list, block_table=table, **maps)
+                ops.rope_cache_q4(qkv, q, pages, num_heads=heads, num_kv_heads=kv_heads, head_dim=d, positions=maps["positions"],
+                                  cos=cos, sin=sin, style=ops.ROPE_NEOX, slots=maps["slots"])
+                ops.attention_q4(q, out, pages, entry_starts=starts, entry_pos0=pos0, positions=maps["positions"],
+                                 token_entry=maps["token_entry"], block_table=table, num_heads=heads, num_kv_heads=kv_heads, head_dim=d,
+                                 scale=d ** -0.5, max_keys=64, all_single=tokens == 3, any_single=True, workspace=workspace)
+
+            if captured:
+                one()
+                torch.cuda.synchronize()
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graph):
+                    one()
+                out.zero_()
+                graph.replay()
+            else:
+                one()
+            torch.cuda.synchronize()
+            outs.append(out.clone())
+        return pages, outs
+
+    pages, outs = play(False)
+    again, replayed = play(True)
+    with torch.cuda.stream(torch.cuda.Stream()):
+        elsewhere, streamed = play(False)
+    for other in (replayed, streamed):
+        assert all(torch.equal(a, b) for a, b in zip(outs, other))
+    for other in (again, elsewhere):
+        assert all(torch.equal(a, b) for a, b in zip(pages, other))
+    # the last step's outputs are attention over what the pages hold
+    k_rows, v_rows = plain.rows_of(pages.k_codes, pages.k_scales, True), plain.rows_of(pages.v_codes, pages.v_scales, False)
+    held = [42, 3, 11]
+    q = _turn(inputs[3].reshape(3, -1, d)[:, :heads], cos.cpu().numpy()[held], sin.cpu().numpy()[held], d, False)
+    q = torch.from_numpy(q.reshape(3, -1)).to(torch.bfloat16).double().numpy()
+    tables = [list(table_pages[e * 10:e * 10 + 4]) for e in range(3)]
+    expected, spread, reach = plain.attend(q, k_rows, v_rows, counts=[1, 1, 1], history=held, tables=tables, page_size=page, num_heads=heads,
+                                           num_kv_heads=kv_heads, d=d, scale=d ** -0.5)
+    limit = plain.allowed(expected, spread, reach, 64, d, torch.bfloat16)
+    assert (np.abs(outs[3].double().cpu().numpy().reshape(expected.shape) - expected) <= limit).all()

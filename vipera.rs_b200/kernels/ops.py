@@ -10,7 +10,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import os
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -96,7 +96,7 @@ class KernelProfile:
         "attention": "attention", "attention_prefill": "attention", "attention_prefill_tc": "attention",
         "attention_decode": "attention", "mlstm": "recurrence", "mamba_scan": "recurrence", "gla": "recurrence",
         "lightning": "recurrence", "mamba2": "recurrence", "moe": "experts",
-        "layernorm": "norm", "causal_conv": "conv",
+        "layernorm": "norm", "causal_conv": "conv", "step_maps": "rope_kv", "expand_q4": "attention",
         "argmax": "sample", "sample": "sample", "apply_penalties": "sample", "feed_tokens": "sample",
         "logprobs": "sample",
     }
@@ -1043,6 +1043,260 @@ def attention_decode(q: torch.Tensor, out: torch.Tensor, k_pool: torch.Tensor, v
 def attention_decode_scratch_floats(num_entries: int, num_heads: int, head_dim: int, num_splits: int) -> int:
     rows = num_entries * num_heads * num_splits
     return (2 * rows + 3) // 4 * 4 + rows * head_dim
+
+
+# ----------------------------------------------------------------------------------------
+# a cache of keys and values in 4 bits
+# ----------------------------------------------------------------------------------------
+Q4_GROUP = 32   # channels that share a scale
+
+
+class Q4Pages(NamedTuple):
+    """Pages of keys and values held in 4 bits: codes uint8 [pages, kv_heads, page_size, d / 2] and scales bfloat16
+    [pages, kv_heads, page_size, d / 32], for keys and for values.  A group of 32 channels has the scale ``s = -m / 8`` in five
+    significant bits, m its value of the largest magnitude (the positive one of two), and stands for ``code * s`` with the nearest code
+    of -8 .. 7 (ties to even); a group with a value that is not finite stands for NaN.  The codes' order is in csrc/kernels/q4.cuh."""
+
+    k_codes: torch.Tensor
+    k_scales: torch.Tensor
+    v_codes: torch.Tensor
+    v_scales: torch.Tensor
+
+
+class _MapsParams(ctypes.Structure):
+    _fields_ = [("entry_starts", _c_void), ("entry_pos0", _c_void), ("page_starts", _c_void), ("pages", _c_void),
+                ("block_table", _c_void), ("positions", _c_void), ("token_entry", _c_void), ("slots", _c_void),
+                ("num_entries", _c_int), ("num_tokens", _c_int), ("num_pages", _c_int), ("table_width", _c_int), ("page_size", _c_int)]
+
+
+class _StoreQ4Params(ctypes.Structure):
+    _fields_ = [("qkv", _c_void), ("row_stride", ctypes.c_longlong), ("q_out", _c_void), ("k_codes", _c_void), ("v_codes", _c_void),
+                ("k_scales", _c_void), ("v_scales", _c_void), ("positions", _c_void), ("cos_table", _c_void), ("sin_table", _c_void),
+                ("slots", _c_void), ("num_slots", ctypes.c_longlong), ("table_rows", _c_int), ("num_tokens", _c_int),
+                ("num_heads", _c_int), ("num_kv_heads", _c_int), ("head_dim", _c_int), ("rot_dims", _c_int), ("style", _c_int),
+                ("page_size", _c_int)]
+
+
+class _ExpandQ4Params(ctypes.Structure):
+    _fields_ = [("k_codes", _c_void), ("v_codes", _c_void), ("k_scales", _c_void), ("v_scales", _c_void), ("k_room", _c_void),
+                ("v_room", _c_void), ("entry_starts", _c_void), ("entry_pos0", _c_void), ("block_table", _c_void),
+                ("table_width", _c_int), ("page_size", _c_int), ("num_entries", _c_int), ("num_pages", _c_int),
+                ("num_kv_heads", _c_int), ("head_dim", _c_int), ("window", _c_int), ("keep_first", _c_int), ("skip_single", _c_int)]
+
+
+class _DecodeQ4Params(ctypes.Structure):
+    _fields_ = [("q", _c_void), ("out", _c_void), ("k_codes", _c_void), ("v_codes", _c_void), ("k_scales", _c_void),
+                ("v_scales", _c_void), ("positions", _c_void), ("block_table", _c_void), ("entry_starts", _c_void),
+                ("sink_values", _c_void), ("gate", _c_void), ("partial_ml", _c_void), ("partial_out", _c_void),
+                ("gate_stride", ctypes.c_longlong), ("gate_per_head", _c_int), ("table_width", _c_int), ("page_size", _c_int),
+                ("page_shift", _c_int), ("num_pages", _c_int), ("num_entries", _c_int), ("num_heads", _c_int),
+                ("num_kv_heads", _c_int), ("head_dim", _c_int), ("scale", _c_float), ("window", _c_int), ("keep_first", _c_int),
+                ("sink", _c_int), ("chunk", _c_int), ("num_splits", _c_int)]
+
+
+def _one_device(what: str, *tensors) -> None:
+    """The tensors lie on the current device, whose stream the launch goes to."""
+    here = torch.cuda.current_device()
+    for tensor in tensors:
+        if tensor is not None and tensor.is_cuda and tensor.get_device() != here:
+            raise InvalidArgumentError(f"{what}: a tensor is on {tensor.device}, the current device is cuda:{here}")
+
+
+def _check_q4_pages(what: str, pages: Q4Pages, num_kv_heads: int, head_dim: int) -> int:
+    """The pages' page size, their shapes and types being those of the head counts and sizes."""
+    if head_dim % Q4_GROUP or not 0 < head_dim <= 256:
+        raise UnsupportedError(f"{what}: heads of 4 bits have a multiple of {Q4_GROUP} channels up to 256, not {head_dim}")
+    shape = pages.k_codes.shape
+    if len(shape) != 4 or shape[1] != num_kv_heads or shape[3] != head_dim // 2 or pages.v_codes.shape != shape \
+            or pages.k_scales.shape != (*shape[:3], head_dim // Q4_GROUP) or pages.v_scales.shape != pages.k_scales.shape:
+        raise InvalidArgumentError(f"{what}: pages of 4 bits are codes [pages, kv_heads, page_size, d / 2] and scales "
+                                   "[pages, kv_heads, page_size, d / 32]")
+    return shape[2]
+
+
+def step_maps(entry_starts: torch.Tensor, entry_pos0: torch.Tensor, *, page_size: int, block_table: torch.Tensor,
+              page_starts: Optional[torch.Tensor] = None, pages: Optional[torch.Tensor] = None,
+              positions: Optional[torch.Tensor] = None, token_entry: Optional[torch.Tensor] = None,
+              slots: Optional[torch.Tensor] = None) -> None:
+    """The maps of a step on the device, from its requests' lengths (all int32): entry e brings the tokens
+    ``entry_starts[e] .. entry_starts[e + 1] - 1`` from position ``entry_pos0[e]`` on and holds the pages ``pages[page_starts[e]
+    : page_starts[e + 1]]``.  Written are ``block_table`` [entries, width] (-1 behind an entry's pages; pages beyond the width are
+    left out) and, where given, per token its ``positions``, its ``token_entry`` and its ``slots``: page * page_size + place in
+    the page, -1 where the entry holds no page for it.  Without ``pages`` the block table is read instead.  Tokens behind the last
+    entry's are left as they were."""
+    fn = _function("cache_q4", "vipera_step_maps", [ctypes.POINTER(_MapsParams), _c_void])
+    _check_struct("cache_q4", "vipera_step_maps_params_size", _MapsParams)
+    entries = entry_pos0.numel()
+    if entry_starts.numel() != entries + 1 or block_table.dim() != 2 or block_table.shape[0] != entries:
+        raise InvalidArgumentError("step_maps: entry_starts has one item more than entry_pos0, the block table a row for each entry")
+    if (pages is None) != (page_starts is None) or (page_starts is not None and page_starts.numel() != entries + 1):
+        raise InvalidArgumentError("step_maps: pages come with page_starts, one item more than there are entries")
+    if page_size <= 0 or entries > 65535:
+        raise InvalidArgumentError("step_maps: a page holds at least one token, a step has at most 65535 entries")
+    per_token = [t for t in (positions, token_entry, slots) if t is not None]
+    tokens = per_token[0].numel() if per_token else 0
+    if any(t.numel() != tokens for t in per_token):
+        raise InvalidArgumentError("step_maps: positions, token_entry and slots hold one number for each token")
+    _one_device("step_maps", entry_starts, entry_pos0, block_table, page_starts, pages, *per_token)
+    int32 = torch.int32
+    p = _MapsParams(_gpu(entry_starts, "entry_starts", int32), _gpu(entry_pos0, "entry_pos0", int32),
+                    _opt(page_starts, "page_starts", int32), _opt(pages, "pages", int32), _gpu(block_table, "block_table", int32),
+                    _opt(positions, "positions", int32), _opt(token_entry, "token_entry", int32), _opt(slots, "slots", int32),
+                    entries, tokens, 0 if pages is None else pages.numel(), block_table.shape[1], page_size)
+    _check(fn(ctypes.byref(p), _stream()), "step_maps")
+
+
+def rope_cache_q4(qkv: torch.Tensor, q_out: torch.Tensor, pages: Q4Pages, *, num_heads: int, num_kv_heads: int, head_dim: int,
+                  positions: torch.Tensor, cos: Optional[torch.Tensor], sin: Optional[torch.Tensor], style: int,
+                  slots: Optional[torch.Tensor], rot_dims: Optional[int] = None) -> None:
+    """As rope_cache, into pages of 4 bits: rotate q and k of a float32 product whose rows begin with (heads + 2 kv_heads) * d
+    values (what follows is not read), write q to q_out [tokens, heads * d] and k and v, quantised, to their ``slots`` (int32, page *
+    page_size + place, from step_maps; a slot that is negative or outside the pool is not written).  Two tokens of a step do not
+    share a slot.  ``slots=None`` writes q alone.  Positions lie inside the tables.  Every product and sum of the rotation is
+    rounded by itself in 32 bits."""
+    fn = _function("cache_q4", "vipera_rope_cache_q4", [ctypes.POINTER(_StoreQ4Params), _c_int, _c_void])
+    _check_struct("cache_q4", "vipera_rope_cache_q4_params_size", _StoreQ4Params)
+    page_size = _check_q4_pages("rope_cache_q4", pages, num_kv_heads, head_dim)
+    rot_dims = head_dim if rot_dims is None else int(rot_dims)
+    count = qkv.shape[0]
+    if qkv.dim() != 2 or qkv.stride(1) != 1 or qkv.shape[1] < (num_heads + 2 * num_kv_heads) * head_dim:
+        raise InvalidArgumentError("rope_cache_q4: qkv rows are too short for the head counts and sizes")
+    if q_out.shape != (count, num_heads * head_dim) or positions.numel() < count or (slots is not None and slots.numel() < count):
+        raise InvalidArgumentError("rope_cache_q4: q_out, positions or slots has the wrong shape")
+    if rot_dims % 2 or not 0 <= rot_dims <= head_dim:
+        raise InvalidArgumentError("rope_cache_q4: the rotated values must be an even count within the head")
+    table_rows = 0
+    if style != ROPE_NONE and rot_dims:
+        if cos is None or sin is None or cos.dim() != 2 or cos.shape[1] != rot_dims // 2 or sin.shape != cos.shape or not cos.shape[0]:
+            raise InvalidArgumentError("rope_cache_q4: cos/sin tables of width rot_dims/2 are needed")
+        table_rows = cos.shape[0]
+    if not qkv.is_cuda or qkv.dtype != torch.float32:
+        raise InvalidArgumentError("rope_cache_q4: qkv must be float32 on a CUDA device")
+    _one_device("rope_cache_q4", qkv, q_out, *pages, positions, cos, sin, slots)
+    u8, bf16 = torch.uint8, torch.bfloat16
+    p = _StoreQ4Params(qkv.data_ptr(), qkv.stride(0), _gpu(q_out, "q_out"), _gpu(pages.k_codes, "k_codes", u8),
+                       _gpu(pages.v_codes, "v_codes", u8), _gpu(pages.k_scales, "k_scales", bf16), _gpu(pages.v_scales, "v_scales", bf16),
+                       _gpu(positions, "positions", torch.int32), _opt(cos, "cos", torch.float32), _opt(sin, "sin", torch.float32),
+                       _opt(slots, "slots", torch.int32), pages.k_codes.shape[0] * page_size if slots is not None else 0, table_rows,
+                       count, num_heads, num_kv_heads, head_dim, rot_dims, style, page_size)
+    _check(fn(ctypes.byref(p), dtype_code(q_out.dtype), _stream()), "rope_cache")
+
+
+def expand_q4(pages: Q4Pages, k_room: torch.Tensor, v_room: torch.Tensor, *, entry_starts: torch.Tensor, entry_pos0: torch.Tensor,
+              block_table: torch.Tensor, window: int = 0, keep_first: int = 0, skip_single: bool = False) -> None:
+    """What pages of 4 bits stand for, as numbers: the rows that the step's tokens see go to the same pages of ``k_room`` and ``v_room``
+    [pages, page_size, kv_heads, d] (bfloat16, which holds every row exactly, or float32), so that the block tables serve both.
+    Other rows of the rooms stay as they are.  ``window`` and ``keep_first`` as for attention; ``skip_single`` leaves entries of one
+    token out."""
+    fn = _function("cache_q4", "vipera_expand_q4", [ctypes.POINTER(_ExpandQ4Params), _c_int, _c_int, _c_void])
+    _check_struct("cache_q4", "vipera_expand_q4_params_size", _ExpandQ4Params)
+    if k_room.dim() != 4 or v_room.shape != k_room.shape or v_room.dtype != k_room.dtype:
+        raise InvalidArgumentError("expand_q4: the rooms are [pages, page_size, kv_heads, d], of one type")
+    num_pages, page_size, num_kv_heads, head_dim = k_room.shape
+    if _check_q4_pages("expand_q4", pages, num_kv_heads, head_dim) != page_size or pages.k_codes.shape[0] != num_pages:
+        raise InvalidArgumentError("expand_q4: the rooms have the cache's pages and page size")
+    entries = entry_pos0.numel()
+    if entry_starts.numel() != entries + 1 or block_table.dim() != 2 or block_table.shape[0] != entries:
+        raise InvalidArgumentError("expand_q4: entry_starts has one item more than entry_pos0, the block table a row for each entry")
+    _one_device("expand_q4", *pages, k_room, v_room, entry_starts, entry_pos0, block_table)
+    u8, bf16, int32 = torch.uint8, torch.bfloat16, torch.int32
+    p = _ExpandQ4Params(_gpu(pages.k_codes, "k_codes", u8), _gpu(pages.v_codes, "v_codes", u8), _gpu(pages.k_scales, "k_scales", bf16),
+                        _gpu(pages.v_scales, "v_scales", bf16), _gpu(k_room, "k_room"), _gpu(v_room, "v_room"),
+                        _gpu(entry_starts, "entry_starts", int32), _gpu(entry_pos0, "entry_pos0", int32),
+                        _gpu(block_table, "block_table", int32), block_table.shape[1], page_size, entries, num_pages, num_kv_heads,
+                        head_dim, max(int(window or 0), 0), int(keep_first or 0), 1 if skip_single else 0)
+    blocks = min(4 * sm_count(k_room.device), max(1, 2 * entries * block_table.shape[1]))
+    _check(fn(ctypes.byref(p), dtype_code(k_room.dtype), blocks, _stream()), "expand_q4")
+
+
+def attention_q4_takes_decode(dtype: torch.dtype, head_dim: int, page_size: int) -> bool:
+    """Whether single tokens are attended over the packed pages directly."""
+    return dtype == torch.bfloat16 and head_dim in MMA_HEAD_DIMS and page_size % 16 == 0
+
+
+def _attention_q4_decode(q, out, pages, *, positions, block_table, num_heads, num_kv_heads, head_dim, scale, max_keys, workspace,
+                         entry_starts, window, keep_first, sink, sink_values, gate, gate_offset, gate_per_head) -> None:
+    fn = _function("attention_q4", "vipera_attention_q4_decode",
+                   [ctypes.POINTER(_DecodeQ4Params), _c_void, ctypes.c_size_t, _c_void])
+    _check_struct("attention_q4", "vipera_attention_q4_params_size", _DecodeQ4Params)
+    entries = block_table.shape[0]
+    chunk, splits = decode_splits(entries, num_kv_heads, max(int(max_keys), 1), sm_count(q.device))
+    scratch = workspace.get("attention.partials", (attention_decode_scratch_floats(
+        entries, num_heads, head_dim, splits + (1 if keep_first else 0)),), torch.float32)
+    gate_pointer, gate_stride = _gate_pointer(gate, gate_offset, q.shape[0], num_heads * (1 if gate_per_head else head_dim),
+                                              "attention_q4")
+    u8, bf16, int32 = torch.uint8, torch.bfloat16, torch.int32
+    p = _DecodeQ4Params(_gpu(q, "q", bf16), _gpu(out, "out", bf16), _gpu(pages.k_codes, "k_codes", u8),
+                        _gpu(pages.v_codes, "v_codes", u8), _gpu(pages.k_scales, "k_scales", bf16),
+                        _gpu(pages.v_scales, "v_scales", bf16), _gpu(positions, "positions", int32),
+                        _gpu(block_table, "block_table", int32), _opt(entry_starts, "entry_starts", int32),
+                        _opt(sink_values, "sink_values", torch.float32), gate_pointer, None, None, gate_stride,
+                        int(bool(gate_per_head)), block_table.shape[1], pages.k_codes.shape[2], 0, pages.k_codes.shape[0], entries,
+                        num_heads, num_kv_heads, head_dim, float(scale), window, keep_first, 1 if sink else 0, chunk, splits)
+    _check(fn(ctypes.byref(p), scratch.data_ptr(), scratch.numel(), _stream()), "attention_decode", kernels=2)
+
+
+def attention_q4(q: torch.Tensor, out: torch.Tensor, pages: Q4Pages, *, entry_starts: torch.Tensor, entry_pos0: torch.Tensor,
+                 positions: torch.Tensor, token_entry: torch.Tensor, block_table: torch.Tensor, num_heads: int, num_kv_heads: int,
+                 head_dim: int, scale: float, max_keys: int, all_single: bool, any_single: bool, workspace, window: int = 0,
+                 keep_first: int = 0, sink: bool = False, sink_values: Optional[torch.Tensor] = None,
+                 gate: Optional[torch.Tensor] = None, gate_offset: int = 0, gate_per_head: bool = False, longest: int = 0) -> None:
+    """Causal grouped-query attention of every token of a step over its request's pages of 4 bits; q and out [tokens, heads * d],
+    bfloat16 or float32, the step described as for the other attentions.  ``max_keys``: no request sees more; ``all_single``: every
+    entry brings one token; ``any_single``: some entry may.  ``window``, ``keep_first``, ``sink``, ``sink_values`` and the gate as
+    for ``attention``, ``longest`` too.  ``workspace.get(name, shape, dtype)`` gives rooms that the call may use until it is
+    done on its stream.
+
+    Single tokens of bfloat16 steps with heads of 64 or 128 values and pages of a multiple of 16 tokens are attended over the packed
+    pages.  Elsewhere the rows that the step sees are expanded to the run's type first (a room as large as one layer's
+    pages in that type) and the kernels for such pages attend."""
+    page_size = _check_q4_pages("attention_q4", pages, num_kv_heads, head_dim)
+    count, entries = q.shape[0], entry_pos0.numel()
+    if num_kv_heads <= 0 or num_heads % num_kv_heads or tuple(q.shape) != (count, num_heads * head_dim) or out.shape != q.shape \
+            or out.dtype != q.dtype:
+        raise InvalidArgumentError("attention_q4: q and out must be [tokens, heads * d] of one dtype, heads a multiple of KV heads")
+    if entry_starts.numel() != entries + 1 or block_table.dim() != 2 or block_table.shape[0] != entries \
+            or positions.numel() < count or token_entry.numel() < count or (all_single and entries != count):
+        raise InvalidArgumentError("attention_q4: entries, positions and block tables do not describe the step's tokens")
+    if sink_values is not None and sink_values.numel() != num_heads:
+        raise InvalidArgumentError("attention_q4: one sink score per query head")
+    if not 0 < max_keys <= block_table.shape[1] * page_size:
+        raise InvalidArgumentError("attention_q4: the block tables reach as far as max_keys says")
+    window = int(window or 0)
+    if window < 0 or keep_first < 0:
+        raise InvalidArgumentError("attention_q4: a window and its kept first keys are counts")
+    _one_device("attention_q4", q, out, *pages, entry_starts, entry_pos0, positions, token_entry, block_table, sink_values, gate)
+    if count == 0:
+        return
+    dtype_code(q.dtype)
+    keep_first = int(keep_first) if window else 0
+    heads = dict(num_heads=num_heads, num_kv_heads=num_kv_heads, head_dim=head_dim, scale=scale, window=window)
+    endings = dict(keep_first=keep_first, sink=sink, sink_values=sink_values, gate=gate, gate_offset=gate_offset,
+                   gate_per_head=gate_per_head)
+    packed = attention_q4_takes_decode(q.dtype, head_dim, page_size)
+    if packed and all_single:
+        _attention_q4_decode(q, out, pages, positions=positions, block_table=block_table, max_keys=max_keys, workspace=workspace,
+                             entry_starts=None, **heads, **endings)
+        return
+    # what the flash kernels know of endings decides whether portions are theirs (see parts/attention.py)
+    extended = sink_values is not None or gate is not None
+    flash = (q.dtype == torch.bfloat16 and head_dim in MMA_HEAD_DIMS and
+             not (extended and (keep_first or head_dim not in TC_ATTENTION_HEAD_DIMS or os.environ.get("VIPERA_ATTENTION_TC", "1") == "0"
+                                or not attention_tc_takes_gate(gate, gate_offset, gate_per_head))))
+    apart = flash and packed and any_single     # single tokens beside portions read the packed pages
+    shape = (pages.k_codes.shape[0], page_size, num_kv_heads, head_dim)
+    k_room, v_room = (workspace.get(f"attention.q4_{name}", shape, q.dtype) for name in ("keys", "values"))
+    expand_q4(pages, k_room, v_room, entry_starts=entry_starts, entry_pos0=entry_pos0, block_table=block_table, window=window,
+              keep_first=keep_first, skip_single=apart)
+    if not flash:
+        attention(q, out, k_room, v_room, token_seq=token_entry, positions=positions, block_table=block_table,
+                  longest=longest or max_keys, **heads, **endings)
+        return
+    attention_prefill(q, out, k_room, v_room, entry_starts=entry_starts, entry_pos0=entry_pos0, block_table=block_table,
+                      num_entries=entries, skip_single=apart, **heads, **endings)
+    if apart:
+        _attention_q4_decode(q, out, pages, positions=entry_pos0, block_table=block_table, max_keys=max_keys, workspace=workspace,
+                             entry_starts=entry_starts, **heads, **endings)
 
 
 # ----------------------------------------------------------------------------------------
