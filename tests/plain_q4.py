@@ -74,12 +74,13 @@ def make_pages(num_pages, page_size, kv_heads, d, seed, device="cpu"):
 
 
 def attend(q, k_rows, v_rows, *, counts, history, tables, page_size, num_heads, num_kv_heads, d, scale, window=0, keep_first=0,
-           sink=False, sink_values=None, gate=None):
-    """(output [tokens, heads, d], how far a result of the run's arithmetic may be off for each unit of rounding): the second is the pair
-    (A, S) with A = sum_j p_j |v_j| / l and S the largest sum over channels of |q k| scale that a score of the row has."""
+           sink=False, sink_values=None, gate=None, v_steps=None):
+    """(output [tokens, heads, d], parts): `parts` is what errors of the run's arithmetic are multiples of, for each output or head:
+    ``spread`` sum_j p_j |v_j| / l, ``steps`` the same with the values' scales in the place of |v|, ``reach`` the largest sum over
+    channels of |q k| scale that a score of the row has, ``flat`` the same with the head's largest |q| in the place of |q|."""
     q = np.asarray(q, dtype=np.float64).reshape(-1, num_heads, d)
-    out, spread = np.zeros_like(q), np.zeros_like(q)
-    reach = np.zeros(q.shape[:2])
+    out, spread, steps = np.zeros_like(q), np.zeros_like(q), np.zeros_like(q)
+    reach, flat = np.zeros(q.shape[:2]), np.zeros(q.shape[:2])
     token = 0
     for e, (count, held) in enumerate(zip(counts, history)):
         for i in range(count):
@@ -88,8 +89,8 @@ def attend(q, k_rows, v_rows, *, counts, history, tables, page_size, num_heads, 
             page = np.asarray([tables[e][j // page_size] for j in seen])
             place = np.asarray(seen) % page_size
             for h in range(num_heads):
-                k = k_rows[page, h // (num_heads // num_kv_heads), place]
-                v = v_rows[page, h // (num_heads // num_kv_heads), place]
+                kv = h // (num_heads // num_kv_heads)
+                k, v = k_rows[page, kv, place], v_rows[page, kv, place]
                 s = k @ q[token, h] * scale
                 best = max(s.max(), 0.0) if sink and sink_values is None else s.max()
                 p = np.exp(s - best)
@@ -98,22 +99,31 @@ def attend(q, k_rows, v_rows, *, counts, history, tables, page_size, num_heads, 
                     total += np.exp((0.0 if sink_values is None else float(sink_values[h])) - best)
                 out[token, h] = p @ v / total
                 spread[token, h] = p @ np.abs(v) / total
+                if v_steps is not None:
+                    steps[token, h] = np.repeat(p @ np.abs(v_steps[page, kv, place]) / total, GROUP)
                 reach[token, h] = (np.abs(k) @ np.abs(q[token, h])).max() * scale
+                flat[token, h] = np.abs(k).sum(-1).max() * np.abs(q[token, h]).max() * scale
             if gate is not None:
                 factor = 1 / (1 + np.exp(-np.asarray(gate[token], dtype=np.float64).reshape(num_heads, -1)))
-                out[token] *= factor
-                spread[token] *= factor
+                for part in (out, spread, steps):
+                    part[token] *= factor
             token += 1
-    return out, spread, reach
+    return out, dict(spread=spread, steps=steps, reach=reach, flat=flat)
 
 
-def allowed(out, spread, reach, keys, d, dtype):
+def allowed(out, parts, keys, d, dtype):
     """How far each output may be off.  Scores are sums of d products and weights and sums run over `keys` keys in 32 bits, a product
     or sum off by 2^-24 of its size, on tensor cores by 2^-22: a score by (d + 8) of these times its reach, a weight and the sum by e
-    to that, a sum by one for each key.  In bfloat16 a weight is rounded twice at most (itself and times the scale) and the output once, each
-    by half a step, 2^-8; 2^-30 is for outputs next to 0."""
+    to that, a sum by one for each key.  2^-30 is for outputs next to 0.  In bfloat16 further:
+    a weight is rounded twice at most (itself and times the scale) and the output once, each by half a step, 2^-8;
+    a channel of the query is the sum of two numbers of 8 bits, within 2^-17 of the head's largest, a score within that of `flat`, a
+    weight and the sum (twice) too;
+    values are summed as codes + 136 (144 steps at most) with 136 times the weights' sum taken off: of the 2^-20 that a product of
+    17 terms may be off, one for each 16 keys that a warp walks (a quarter of its block's) and four to join the parts."""
     unit = 2.0 ** -22
-    relative = 2 * (d + 8) * reach * unit + 2 * (keys + 16) * unit
+    relative = 2 * (d + 8) * parts["reach"] * unit + 2 * (keys + 16) * unit
     if dtype == torch.bfloat16:
-        return spread * (2 * 2.0 ** -8 + 2.0 ** -15 + relative[..., None]) + np.abs(out) * 2.0 ** -8 + 2.0 ** -30
-    return spread * relative[..., None] + 2.0 ** -30
+        relative = relative + 2 * 2.0 ** -17 * parts["flat"]
+        return (parts["spread"] * (2 * 2.0 ** -8 + 2.0 ** -15 + relative[..., None]) + np.abs(out) * 2.0 ** -8
+                + parts["steps"] * (keys / 64 + 4) * 144 * 2.0 ** -20 + 2.0 ** -30)
+    return parts["spread"] * relative[..., None] + 2.0 ** -30

@@ -53,7 +53,7 @@ def entry_points(monkeypatch):
 
     monkeypatch.setattr(ops, "_function", lambda *_: no_launch)
     monkeypatch.setattr(ops, "_check_struct", lambda *_: None)
-    monkeypatch.setattr(ops, "_one_device", lambda *_: None)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
     return ops
 
 
@@ -87,7 +87,7 @@ def test_rope_cache_q4_refuses_shapes_and_sizes_it_does_not_take(entry_points):
                    dict(cos=torch.zeros(8, 16)), dict(num_kv_heads=3), dict(cos=torch.zeros(0, 32), sin=torch.zeros(0, 32))):
         with pytest.raises(InvalidArgumentError):
             ops.rope_cache_q4(qkv, q, _pages(ops), **{**good, **change})
-    for bad_qkv, bad_q in ((qkv[:, :-1], q), (qkv.t(), q), (qkv, q[:2]), (qkv.double(), q), (qkv, q)):   # the last: not on a device
+    for bad_qkv, bad_q in ((qkv[:, :-1], q), (qkv.t(), q), (qkv, q[:2]), (qkv.double(), q), (qkv, q)):   # the last: on another device
         with pytest.raises(InvalidArgumentError):
             ops.rope_cache_q4(bad_qkv, bad_q, _pages(ops), **good)
     with pytest.raises(UnsupportedError):
@@ -125,3 +125,80 @@ def test_attention_q4_refuses_steps_that_do_not_agree(entry_points):
             ops.attention_q4(q, torch.zeros_like(q), _pages(ops), **{**good, **change})
     with pytest.raises(InvalidArgumentError):
         ops.attention_q4(q, torch.zeros(3, 4 * 64), _pages(ops), **good)
+
+
+def _spec(raw):
+    from vipera_rs_b200.config import architecture_of
+
+    arch = architecture_of(raw)
+    return arch.model_spec(arch.config_from_dict(raw))
+
+
+def test_the_memory_plan_counts_packed_pages_and_one_slots_room():
+    import helpers
+    from vipera_rs_b200.engine import planner
+
+    for name in ("A", "B"):
+        spec = _spec(helpers.CONFIGS[name])
+        run = planner.plan_memory(spec, 256, 3, "bfloat16", device_bytes=10**9)
+        packed = planner.plan_memory(spec, 256, 3, "bfloat16", device_bytes=10**9, kv_type="q4")
+        assert packed["kv_bytes"] * 32 == run["kv_bytes"] * 9 and packed["kv_bytes_per_token"] * 32 == run["kv_bytes_per_token"] * 9
+        room = packed["workspace_bytes"] - run["workspace_bytes"]
+        assert room == planner.room_bytes(spec, 256, 3, 2) > 0
+    # A's two layers are alike: the room is one layer's pages, and one page more
+    spec = _spec(helpers.CONFIGS["A"])
+    assert planner.room_bytes(spec, 256, 3, 2) == planner.cache_bytes(spec, 256, 3, 2) // 2 + 16 * 2 * 2 * 64 * 2
+
+
+def test_models_whose_mixers_need_the_runs_type_refuse_4_bits():
+    import helpers
+    from nobupel_cases import MIXED
+    from vipera_rs_b200.engine import planner
+    from vipera_rs_b200.errors import InvalidArgumentError, UnsupportedError
+
+    for raw in (helpers.CONFIGS["C"], MIXED):    # heads of 48; values of another size than keys
+        with pytest.raises(UnsupportedError):
+            planner.plan_memory(_spec(raw), 64, 1, "bfloat16", device_bytes=10**9, kv_type="q4")
+    with pytest.raises(InvalidArgumentError):
+        planner.plan_memory(_spec(helpers.CONFIGS["A"]), 64, 1, "bfloat16", device_bytes=10**9, kv_type="q5")
+
+
+@pytest.mark.parametrize("option", [dict(chunk=16), dict(values_from_keys=True), dict(row_norm=True, norm_eps=1e-6), dict(talking_heads=True),
+                                    dict(out_scale=0.5), dict(value_mix="source"), dict(head_norm=True, norm_eps=1e-6), dict(value_dim=32),
+                                    dict(head_dim=48)])
+def test_attention_says_which_options_packed_pages_serve(option):
+    import vipera_rs_b200  # noqa: F401
+    from vipera_rs_b200.parts.attention import GQAttention
+
+    plain_params = dict(hidden_size=256, num_heads=4, num_kv_heads=2, head_dim=64, window=None)
+    assert GQAttention.cache_request_for(plain_params).four_bit
+    assert GQAttention.cache_request_for(dict(plain_params, window=40, keep_first=3, sink="learned", output_gate=True)).four_bit
+    assert not GQAttention.cache_request_for(dict(plain_params, **option)).four_bit
+
+
+def test_the_cut_of_the_keys_covers_them_in_whole_walks():
+    import vipera_rs_b200  # noqa: F401
+    from vipera_rs_b200.kernels import ops
+
+    for entries in (1, 3, 64, 300):
+        for tiles in (1, 8, 40):
+            for keys in (1, 128, 129, 2049, 40000, 10**6):
+                for window in (0, 1, 1024):
+                    chunk, splits = ops.q4_splits(entries, tiles, keys, window, 148)
+                    assert chunk % 128 == 0 and 0 < splits <= 128 and chunk * (splits - 1) < keys <= chunk * splits
+
+
+def test_page_lists_are_the_requests_pages_one_behind_the_other():
+    from vipera_rs_b200.build import runtime_module
+
+    manager = runtime_module().CacheManager([(16, 20, 0, 0), (16, 20, 32, 0)], 4, False)
+    for request, length in ((0, 40), (1, 5), (2, 80)):
+        manager.open(request)
+        manager.reserve(request, length)
+    manager.commit(2, 80)                    # the window's group gives pages back
+    for group in (0, 1):
+        starts, pages = manager.page_lists([2, 0, 1], group)
+        table = manager.tables([2, 0, 1], group, 8)
+        assert starts.tolist()[0] == 0 and starts.tolist()[-1] == len(pages)
+        for row, (first, last) in enumerate(zip(starts[:-1], starts[1:])):
+            assert table[row].tolist() == pages[first:last].tolist() + [-1] * (8 - (last - first))

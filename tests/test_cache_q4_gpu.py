@@ -212,6 +212,7 @@ def _attend(ops, step, dtype, heads, kv_heads, d, seed=0, window=0, keep_first=0
             gate_per_head=False, workspace=None):
     raw = plain.make_pages(step.num_pages, step.page_size, kv_heads, d, seed + 10, DEVICE)
     k_rows, v_rows = plain.rows_of(raw[0], raw[1], True), plain.rows_of(raw[2], raw[3], False)
+    v_steps = raw[3].double().cpu().numpy()
     pages = ops.Q4Pages(*raw)
     tables = [list(row) for row in step.tables]
     _hide(step, pages, window, keep_first)
@@ -225,12 +226,12 @@ def _attend(ops, step, dtype, heads, kv_heads, d, seed=0, window=0, keep_first=0
                      workspace=workspace or _workspace(), window=window, keep_first=keep_first, sink=sink,
                      sink_values=None if sink_values is None else torch.from_numpy(sink_values).to(DEVICE),
                      gate=gates, gate_offset=4, gate_per_head=gate_per_head, **step.device())
-    expected, spread, reach = plain.attend(q.double().numpy(), k_rows, v_rows, counts=step.counts, history=step.history, tables=tables,
-                                           page_size=step.page_size, num_heads=heads, num_kv_heads=kv_heads, d=d, scale=scale,
-                                           window=window, keep_first=keep_first, sink=sink, sink_values=sink_values, gate=gate)
+    expected, parts = plain.attend(q.double().numpy(), k_rows, v_rows, counts=step.counts, history=step.history, tables=tables,
+                                   page_size=step.page_size, num_heads=heads, num_kv_heads=kv_heads, d=d, scale=scale, window=window,
+                                   keep_first=keep_first, sink=sink, sink_values=sink_values, gate=gate, v_steps=v_steps)
     got = out[:tokens].double().cpu().numpy().reshape(expected.shape)
     keys = max(c + h for c, h in zip(step.counts, step.history))
-    limit = plain.allowed(expected, spread, reach, keys, d, dtype)
+    limit = plain.allowed(expected, parts, keys, d, dtype)
     assert np.isfinite(got).all()
     worst = (np.abs(got - expected) / limit).max()
     assert worst <= 1.0, worst
@@ -311,8 +312,10 @@ def test_scores_of_zero_and_equal_keys_give_the_mean(ops):
     v = plain.rows_of(pages.v_codes, pages.v_scales, False)[:, 0]
     seen = np.stack([v[step.tables[0][j // 16], j % 16] for j in range(100)])
     got = out.double().cpu().numpy().reshape(2, 64)
-    # weights of 1 are exact, times a scale too: the sums in 32 bits and the output's rounding are left
-    limit = np.abs(seen).mean(0) * 2.0 ** -14 + np.abs(seen.mean(0)) * 2.0 ** -8
+    # weights of 1 are exact, times a scale too: the sums in 32 bits (of codes + 136, see plain.allowed) and the output's rounding are left
+    steps = np.stack([pages.v_scales.double().cpu().numpy()[step.tables[0][j // 16], 0, j % 16] for j in range(100)])
+    limit = (np.abs(seen).mean(0) * 2.0 ** -14 + np.abs(seen.mean(0)) * 2.0 ** -8
+             + np.repeat(np.abs(steps).mean(0), 32) * (100 / 64 + 4) * 144 * 2.0 ** -20)
     assert (np.abs(got - seen.mean(0)) <= limit).all()
 
 
@@ -386,7 +389,7 @@ def test_a_step_as_it_is_used_eager_captured_and_on_a_stream_of_its_own(ops):
     q = _turn(inputs[3].reshape(3, -1, d)[:, :heads], cos.cpu().numpy()[held], sin.cpu().numpy()[held], d, False)
     q = torch.from_numpy(q.reshape(3, -1)).to(torch.bfloat16).double().numpy()
     tables = [list(table_pages[e * 10:e * 10 + 4]) for e in range(3)]
-    expected, spread, reach = plain.attend(q, k_rows, v_rows, counts=[1, 1, 1], history=held, tables=tables, page_size=page, num_heads=heads,
-                                           num_kv_heads=kv_heads, d=d, scale=d ** -0.5)
-    limit = plain.allowed(expected, spread, reach, 64, d, torch.bfloat16)
+    expected, parts = plain.attend(q, k_rows, v_rows, counts=[1, 1, 1], history=held, tables=tables, page_size=page, num_heads=heads,
+                                   num_kv_heads=kv_heads, d=d, scale=d ** -0.5, v_steps=pages.v_scales.double().cpu().numpy())
+    limit = plain.allowed(expected, parts, 64, d, torch.bfloat16)
     assert (np.abs(outs[3].double().cpu().numpy().reshape(expected.shape) - expected) <= limit).all()

@@ -20,10 +20,13 @@ from typing import Dict, List, Optional, Tuple
 import torch
 
 from ..build import runtime_module
-from ..errors import InvalidArgumentError
-from ..parts.base import FixedState, PagedKV, PagedKVView, StateView, bundle_views, flatten_cache_requests
+from ..errors import InvalidArgumentError, UnsupportedError
+from ..kernels.ops import Q4_GROUP, Q4Pages
+from ..parts.base import FixedState, PagedKV, PagedKVView, PagedQ4View, StateView, bundle_views, flatten_cache_requests
 
 
+KV_TYPES = ("q4",)    # kinds of pages beside those of the run's type (None)
+_Q4_ALIGN = 256       # bytes: where codes, scales and guards of 4-bit pools begin
 GUARD_WORD = 0x5A5A   # fits 16 bits: the guard regions are viewed as integers of the element's width
 
 
@@ -40,8 +43,11 @@ class CacheGroup:
     def v_dim(self) -> int:
         return self.value_dim or self.head_dim
 
-    def bytes_per_token(self, element_bytes: int) -> int:
-        return len(self.slots) * self.num_kv_heads * (self.head_dim + self.v_dim) * element_bytes
+    def bytes_per_token(self, element_bytes: int, kv_type: Optional[str] = None) -> int:
+        values = len(self.slots) * self.num_kv_heads * (self.head_dim + self.v_dim)
+        if kv_type == "q4":
+            return values // 2 + values // Q4_GROUP * 2     # a code for each value, a bfloat16 scale for each group
+        return values * element_bytes
 
 
 def plan_groups(cache_requests: Dict[int, object]) -> Tuple[List[CacheGroup], Dict[int, FixedState]]:
@@ -65,11 +71,28 @@ def plan_groups(cache_requests: Dict[int, object]) -> Tuple[List[CacheGroup], Di
     return list(groups.values()), states
 
 
+def check_kv_type(kv_type: Optional[str], cache_requests: Dict[int, object]) -> Optional[str]:
+    """None (pages of the run's type) or "q4" (pages of 4 bits), the latter where every mixer that keeps pages takes them."""
+    if kv_type is None:
+        return None
+    if kv_type not in KV_TYPES:
+        raise InvalidArgumentError(f"the cache's type is the run's or one of {', '.join(KV_TYPES)}, not {kv_type!r}")
+    paged = [(slot, r) for slot, r in flatten_cache_requests(cache_requests).items() if isinstance(r, PagedKV)]
+    if not paged:
+        raise UnsupportedError("no mixer of this model keeps pages that could be held in 4 bits")
+    for slot, request in paged:
+        if not request.four_bit:
+            raise UnsupportedError(f"cache slot {slot}: its mixer does not take pages of 4 bits")
+    return kv_type
+
+
 class CachePools:
-    """Allocates the pools and the native manager for one engine."""
+    """Allocates the pools and the native manager for one engine.  ``kv_type``: None for pages of ``dtype``, "q4" for pages of
+    4 bits (per cache slot codes and scales of the keys, then of the values, as ``ops.Q4Pages`` says)."""
 
     def __init__(self, cache_requests: Dict[int, object], *, page_size: int, num_pages, num_state_slots: int,
-                 dtype: torch.dtype, device, reuse_prefixes: bool = False):
+                 dtype: torch.dtype, device, reuse_prefixes: bool = False, kv_type: Optional[str] = None):
+        self.kv_type = check_kv_type(kv_type, cache_requests)
         self.groups, self.states = plan_groups(cache_requests)
         self.page_size = int(page_size)
         self.dtype = dtype
@@ -99,6 +122,9 @@ class CachePools:
         self._guards: List[torch.Tensor] = []
         for index, (group, pages) in enumerate(zip(self.groups, self.num_pages)):
             rows = (pages + 1) * self.page_size * group.num_kv_heads     # key (or value) rows of one slot
+            if self.kv_type == "q4":
+                self._add_q4_group(index, group, pages, rows, views)
+                continue
             count = len(group.slots) * rows * (group.head_dim + group.v_dim)
             guard = self.page_size * group.num_kv_heads * max(group.head_dim, group.v_dim)
             storage = torch.zeros(count + 2 * guard, dtype=dtype, device=device)
@@ -123,6 +149,30 @@ class CachePools:
         # what each cache slot of the schedule is handed: a view, or for a bundle a dict of views
         self.views: Dict[int, object] = {slot: bundle_views(request, slot, views)
                                          for slot, request in cache_requests.items() if request is not None}
+
+    def _add_q4_group(self, index: int, group: CacheGroup, pages: int, rows: int, views: Dict[object, object]) -> None:
+        def whole(count: int) -> int:
+            return -(-count // _Q4_ALIGN) * _Q4_ALIGN
+
+        code_bytes, scale_bytes = whole(rows * group.head_dim // 2), whole(rows * group.head_dim // Q4_GROUP * 2)
+        count = len(group.slots) * 2 * (code_bytes + scale_bytes)
+        guard = whole(self.page_size * group.num_kv_heads * group.head_dim)
+        storage = torch.zeros(count + 2 * guard, dtype=torch.uint8, device=self.device)
+        for region in (storage[:guard], storage[guard + count:]):
+            region.view(torch.int16).fill_(GUARD_WORD)
+            self._guards.append(region.view(torch.int16))
+        pool = storage[guard:guard + count]
+        self.pool_tensors.append(pool)
+        shape = (pages + 1, group.num_kv_heads, self.page_size)
+        for position, slot in enumerate(group.slots):
+            tensors, at = [], position * 2 * (code_bytes + scale_bytes)
+            for _ in range(2):                                   # keys, values
+                tensors.append(pool[at:at + rows * group.head_dim // 2].view(*shape, group.head_dim // 2))
+                at += code_bytes
+                scales = pool[at:at + rows * group.head_dim // Q4_GROUP * 2].view(torch.bfloat16)
+                tensors.append(scales.view(*shape, group.head_dim // Q4_GROUP))
+                at += scale_bytes
+            views[slot] = PagedQ4View(index, Q4Pages(*tensors), self.page_size, group.window, group.keep_first)
 
     def guards_intact(self) -> bool:
         """Whether the guard regions in front of and behind every pool still hold their word."""
@@ -149,5 +199,11 @@ class CachePools:
 
     def poison(self, value: float = float("nan")) -> None:
         """Fill every page with a value that shows when read (tests use NaN)."""
+        if self.kv_type == "q4":
+            for view in self._flat_views.values():
+                if isinstance(view, PagedQ4View):    # a row of 4 bits shows the value through its scales
+                    view.pages.k_scales.fill_(value)
+                    view.pages.v_scales.fill_(value)
+            return
         for pool in self.pool_tensors:
             pool.fill_(value)

@@ -28,9 +28,9 @@ USAGE = """usage: vipera <command> [arguments]
 commands:
   generate <model> --prompt "IDS" [--max-tokens N] [--ctx N] [--temperature T] [--top-k K]
            [--top-p P] [--min-p P] [--repetition-penalty F] [--presence-penalty F]
-           [--frequency-penalty F] [--seed S] [--dtype bfloat16|float32] [--page-size N] [--json]
+           [--frequency-penalty F] [--seed S] [--dtype bfloat16|float32] [--kv-type q4] [--page-size N] [--json]
   model-info <model> [--json]
-  plan <model> [--ctx N] [--batch N] [--dtype bfloat16|float32] [--device-bytes N] [--page-size N] [--json]
+  plan <model> [--ctx N] [--batch N] [--dtype bfloat16|float32] [--kv-type q4] [--device-bytes N] [--page-size N] [--json]
   random-weights <config.json> <out-dir> [--seed S] [--dtype bfloat16|float32]
 
 exit codes: 0 ok, 1 usage, 2 bad input, 3 infeasible, 4 internal
@@ -128,13 +128,13 @@ def model_info(args: List[str]) -> int:
 
 
 def plan_memory(model_dir: str, ctx: int, batch: int, dtype: str, device_bytes: Optional[int],
-                page_size: int = 16) -> dict:
+                page_size: int = 16, kv_type: Optional[str] = None) -> dict:
     """The memory plan of the model in ``model_dir`` (its config.json is all that is read)."""
     from .config import load_config
     from .engine import planner
 
     arch, config = load_config(model_dir)
-    return planner.plan_memory(arch.model_spec(config), ctx, batch, dtype, device_bytes, page_size)
+    return planner.plan_memory(arch.model_spec(config), ctx, batch, dtype, device_bytes, page_size, kv_type)
 
 
 def plan(args: List[str]) -> int:
@@ -145,7 +145,8 @@ def plan(args: List[str]) -> int:
     if not places:
         raise UsageError("plan needs a model path")
     report = plan_memory(places[0], found.get("ctx", 2048), found.get("batch", 1),
-                         found.get("dtype", "bfloat16"), found.get("device_bytes"), found.get("page_size", 16))
+                         found.get("dtype", "bfloat16"), found.get("device_bytes"), found.get("page_size", 16),
+                         "q4" if found.get("kv_type") == "q4" else None)
     if found.get("json"):
         print(json.dumps(report, indent=2))
     else:
@@ -190,8 +191,8 @@ def generate(args: List[str]) -> int:
         raise InvalidArgumentError("--max-tokens must be at least 1")
     dtype = found.get("dtype", "bfloat16")
     kv_type = found.get("kv_type")
-    if kv_type is not None and kv_type not in ("bf16", "bfloat16", "f32", "float32"):
-        raise InvalidArgumentError(f"--kv-type {kv_type!r}: the cache has the run's dtype; quantized caches are not built")
+    if kv_type is not None and kv_type not in ("bf16", "bfloat16", "f32", "float32", "q4"):
+        raise InvalidArgumentError(f"--kv-type {kv_type!r}: the cache has the run's dtype, or 4 bits a value and scales (q4)")
 
     from .engine.engine import Engine
     from .sampling import SamplingParams
@@ -203,7 +204,8 @@ def generate(args: List[str]) -> int:
         presence_penalty=found.get("presence_penalty", 0.0),
         frequency_penalty=found.get("frequency_penalty", 0.0), seed=found.get("seed", 0))
     engine = Engine(places[0], dtype=dtype, device=found.get("device", "cuda:0"),
-                    page_size=found.get("page_size", 16), ctx=found.get("ctx"), max_num_seqs=1)
+                    page_size=found.get("page_size", 16), ctx=found.get("ctx"), max_num_seqs=1,
+                    kv_type="q4" if kv_type == "q4" else None)
     as_json = bool(found.get("json"))
     eos = set(engine.default_eos)
 

@@ -5,17 +5,25 @@
 //
 // Both products put the packed operand on the side of 16 (keys for the scores, channels for the values) and the query
 // heads on the side of 8: a group of 8 heads or fewer costs half of the products that the other way round would
-// waste on empty rows.  Codes become bfloat16 by a mask and an OR (0x4300 | u is 128 + u) and an exact subtraction of 136;
-// the scales stay outside of them:
-//   scores   the 32 channels of a group are one accumulator's two products, which the key's scale multiplies in 32
-//            bits: s[key, head] = sum_g scale[key, g] (c[key, g, :] . q[head, g, :]), exact but for the 32-bit sums;
-//   values   the weights take the scales, w[key, head, g] = p[key, head] scale[key, g], rounded to bfloat16 a second time (2^-9 of
-//            the weight, as p itself): 2 products of pairs a group in the place of 16 on the codes.
+// waste on empty rows.  Offsets and scales of the codes stay outside of the products, and what is left of unpacking is what
+// bounds the kernel beside the memory, so it is kept short:
+//   scores   in half precision a nibble u at the bottom of 16 bits is the number u 2^-24, one at bits 4 to 7 is 16 u 2^-24 (the
+//            smallest numbers are equally spaced), so a mask makes two codes an operand and one shift serves four.  The query's
+//            channels, whose largest is brought to 2^14 .. 2^15, keep all their bits in half precision down to 2^-29 of the
+//            largest; those that meet 16 u are a 16th.  The 32 channels of a group are one accumulator's two products, which
+//            begins at -8 times the sum of the query's channels and which the key's scale multiplies in 32 bits:
+//            s[key, head] = sum_g scale[key, g] (c[key, g, :] . q[head, g, :]).  The products' sums are as exact as if the codes
+//            were 2^10: off by 2^-22 of that.
+//   values   codes become bfloat16 by a shift, a mask and an OR (0x4300 | u is 128 + u, 136 above the code); the weights take the scales, w[key, head, g] = p[key, head] scale[key, g], rounded to bfloat16 a second time (half a
+//            step of the weight, as p itself): 2 products of pairs a group in the place of 16 on the codes; a product with
+//            ones sums them, and 136 times that sum goes off at the end.
 // A score's accumulators have the keys on their rows, the second product wants them on its inner axis: movmatrix turns the
 // weights' 8 x 8 blocks in registers, so nothing passes through shared memory until the end.
 #include "attention_combine.cuh"
 #include "attention_mma.cuh"
 #include "q4.cuh"
+
+#include <cuda_fp16.h>
 
 namespace {
 
@@ -36,30 +44,60 @@ struct DecodeParams {
   int table_width, page_size, page_shift, num_pages, num_entries, num_heads, num_kv_heads, head_dim;
   float scale;
   int window, keep_first, sink, chunk, num_splits;
+  uint32_t magic;                 // set by the launcher
 };
 
 constexpr int kWarps = 4;
 constexpr int kWarpKeys = 32;   // keys a warp folds at a time: two tiles of 16
+constexpr int kStages = 4;      // such pairs of tiles on their way to shared memory for each warp
 
-__device__ __forceinline__ uint32_t sub_bf16x2(uint32_t a, uint32_t b) {
-  const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
 __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
   const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
-// The codes at bits 4 j and 16 + 4 j of a word as two bfloat16.
-__device__ __forceinline__ uint32_t codes_of(uint32_t word, int j) {
-  return sub_bf16x2(((word >> (4 * j)) & 0x000f000fu) | 0x43004300u, 0x43084308u);
-}
+// The codes at bits 4 j and 16 + 4 j of a word as two bfloat16, 128 + u each.  `magic` is 0x43004300 from a parameter: a constant
+// would be an instruction's immediate beside the mask's, and two do not fit into one.
+__device__ __forceinline__ uint32_t codes_of(uint32_t word, int j, uint32_t magic) { return ((word >> (4 * j)) & 0x000f000fu) | magic; }
+constexpr float kOffset = 136.0f;   // what such a number is above its code
+constexpr uint32_t kOnes = 0x3f803f80u;
+
 __device__ __forceinline__ uint32_t turn_8x8(uint32_t a) {
   uint32_t d;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
+__device__ __forceinline__ float exp2_near(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 __device__ __forceinline__ float low_of(uint32_t pair) { return __uint_as_float(pair << 16); }
 __device__ __forceinline__ float high_of(uint32_t pair) { return __uint_as_float(pair & 0xffff0000u); }
+// d = a . b + (x, y) for the two columns of every row, and d += a . b, of half-precision operands
+__device__ __forceinline__ void mma_half_from(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float x, float y) {
+  asm(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %10, %11};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(x), "f"(y));
+}
+__device__ __forceinline__ void mma_half(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ void cp_async_all(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 
 template <int WORDS>
 __device__ __forceinline__ void load_words(uint32_t (&to)[WORDS], const void* from) {
@@ -74,44 +112,23 @@ __device__ __forceinline__ void load_words(uint32_t (&to)[WORDS], const void* fr
   }
 }
 
-// What a warp holds of 16 keys.  Lane 4 g + t: the keys' codes and scales of keys g and g + 8 (word t of every group), the
-// values' of keys 2 t, 2 t + 1, 2 t + 8 and 2 t + 9 (unit g of every group).
+// Two tiles of 16 keys in a warp's part of shared memory.  Row r of a tile's score accumulators is key 4 (r & 1) + (r & 7) / 2 + 8 (r / 8):
+// the keys whose weights a lane's operand of the second product holds, slots 2 t, 2 t + 1, 2 t + 8 and 2 t + 9, are then keys 4 i + t, i
+// = 0 .. 3, whose rows four lanes read without a conflict; the keys' own rows lie in the order of the accumulators.
 template <int D>
-struct Tile {
-  static constexpr int G = D / 32;
-  uint32_t k[2][G];            // [key g, g + 8][group]
-  uint32_t k_scale[2][G / 2];  // pairs of groups
-  uint32_t v[4][G / 2];        // [key][pair of groups]: a unit of 16 bits a group
-  uint32_t v_scale[2][G];      // [pair of keys][first key's groups, second key's]
-  int key0;                    // its first key; -1: nothing to see
-
-  __device__ __forceinline__ void load(const DecodeParams& p, const int* table, int kv_head, int key, int first, int last, int lane) {
-    key0 = -1;
-    if (key > last || key + 15 < first) return;
-    const int index = p.page_shift >= 0 ? key >> p.page_shift : key / p.page_size;
-    if (index >= p.table_width) return;
-    const int page = table[index];
-    if (page < 0 || page >= p.num_pages) return;
-    key0 = key;
-    const size_t row = (static_cast<size_t>(page) * p.num_kv_heads + kv_head) * p.page_size + (key - index * p.page_size);
-    const int g = lane >> 2, t = lane & 3;
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const size_t at = row + g + 8 * r;
-      load_words<G>(k[r], p.k_codes + at * (D / 2) + t * 4 * G);
-      load_words<G / 2>(k_scale[r], p.k_scales + at * G);
-      load_words<G>(v_scale[r], p.v_scales + (row + 2 * t + 8 * r) * G);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) load_words<G / 2>(v[2 * r + i], p.v_codes + (row + 2 * t + 8 * r + i) * (D / 2) + g * 2 * G);
-    }
-  }
+struct Stage {
+  static constexpr int G = D / 32, kRowBytes = D / 2;
+  uint8_t k[2][16 * kRowBytes];
+  uint8_t v[2][16 * kRowBytes];
+  uint8_t k_scale[2][16 * G * 2];
+  uint8_t v_scale[2][16 * G * 2];
 };
 
 template <int D, int NT>
-__global__ void __launch_bounds__(32 * kWarps) attention_q4_decode_kernel(DecodeParams p) {
-  constexpr int G = D / 32;
+__global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) attention_q4_decode_kernel(DecodeParams p) {
+  constexpr int G = D / 32, kRowBytes = D / 2, kChunks = kRowBytes / 16;
   constexpr int kRow = D + 4;             // floats of a head's partial in shared memory
-  extern __shared__ __align__(16) float merge[];   // [warp][8 NT heads][kRow]
+  extern __shared__ __align__(128) uint8_t shared[];   // the warps' stages; then [warp][8 NT heads][kRow] floats
   pdl_wait();
   // only now: the kernel behind reads the positions before its own wait, and they may come from the kernel ahead
   pdl_launch_dependents();
@@ -135,130 +152,268 @@ __global__ void __launch_bounds__(32 * kWarps) attention_q4_decode_kernel(Decode
   const int end = kept_split ? last + 1 : min((split + 1) * p.chunk, position + 1);
   if (begin >= end) return;   // a split without visible keys: the combine kernel skips it too
 
-  uint32_t q[NT][G][4];       // lane (g, t): channels 32 group + 8 t .. + 7 of head 8 nt + g
+  // --- the way of the rows into shared memory: 16 bytes a lane, kStages - 1 pairs of tiles ahead ---
+  Stage<D>* stages = reinterpret_cast<Stage<D>*>(shared) + warp * kStages;
+  const int warp_begin = begin + warp * kWarpKeys;
+  const int steps = warp_begin < end ? (end - warp_begin + kWarps * kWarpKeys - 1) / (kWarps * kWarpKeys) : 0;
+  // the page of the tile that is this lane's among 32: tile i of step j is key warp_begin + 128 j + 16 i; a tile
+  // without a visible key, and one whose page is not held, has none and is filled with zeros
+  const auto page_of = [&](int tile) {
+    const int key = warp_begin + (tile >> 1) * (kWarps * kWarpKeys) + (tile & 1) * 16;
+    if (key >= end || key > last || key + 15 < first) return -1;
+    const int index = p.page_shift >= 0 ? key >> p.page_shift : key / p.page_size;
+    const int page = index < p.table_width ? table[index] : -1;
+    return page < p.num_pages ? page : -1;
+  };
+  int pages_now = page_of(lane), pages_next = steps > 16 ? page_of(32 + lane) : -1;
+  const uint32_t page_rows = static_cast<uint32_t>(p.num_kv_heads) * p.page_size;   // rows of a page
+  const uint8_t* k_head = p.k_codes + static_cast<size_t>(kv_head) * p.page_size * kRowBytes + lane * 16;
+  const uint8_t* v_head = p.v_codes + static_cast<size_t>(kv_head) * p.page_size * kRowBytes + lane * 16;
+  // a lane's piece of the scales: tile, keys' or values', place
+  constexpr int kScaleChunks = 16 * G * 2 / 16;
+  const int scale_tile = lane / (2 * kScaleChunks), scale_values = lane / kScaleChunks & 1, scale_chunk = lane % kScaleChunks;
+  const uint8_t* scale_head = reinterpret_cast<const uint8_t*>(scale_values ? p.v_scales : p.k_scales) +
+                              static_cast<size_t>(kv_head) * p.page_size * G * 2 + scale_chunk * 16;
+  const uint32_t stages_at = smem_addr(stages);
+  uint32_t k_to, v_to, scale_to;   // where a lane's piece goes within a stage (pieces of 8 keys, or of 16 where a row has two)
+  {
+    const int key = lane / kChunks, chunk = lane % kChunks;   // key of the first 8 (16)
+    const int row = 2 * (key & 3) + ((key >> 2) & 1) + 8 * (key >> 3);
+    k_to = stages_at + offsetof(Stage<D>, k) + row * kRowBytes + chunk * 16;
+    v_to = stages_at + offsetof(Stage<D>, v) + key * kRowBytes + (kChunks == 4 ? chunk ^ (key & 2) : chunk) * 16;
+    scale_to = stages_at + (scale_values ? offsetof(Stage<D>, v_scale) : offsetof(Stage<D>, k_scale)) +
+               scale_tile * (16 * G * 2) + scale_chunk * 16;
+  }
+  const bool one_tile_a_page = p.page_size == 16;
+  constexpr uint32_t kStageBytes = sizeof(Stage<D>);
+  const auto fetch = [&](int j) {
+    if (j < steps) {
+      const uint32_t stage = (j % kStages) * kStageBytes;
+      const int pages = (j & 16) ? pages_next : pages_now;
+      const int page[2] = {__shfl_sync(0xffffffffu, pages, (2 * j) & 31), __shfl_sync(0xffffffffu, pages, (2 * j + 1) & 31)};
+      uint32_t place[2] = {0, 0};
+      if (!one_tile_a_page) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int key = warp_begin + j * (kWarps * kWarpKeys) + 16 * i;
+          place[i] = p.page_shift >= 0 ? key & (p.page_size - 1) : key % p.page_size;
+        }
+      }
+      constexpr int kPieces = 16 * kChunks / 32;    // of 32 lanes a tile
+      const bool all = (page[0] | page[1]) >= 0;    // every tile but the first and the last of a walk
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint64_t from = static_cast<uint64_t>(static_cast<uint32_t>(all ? page[i] : max(page[i], 0))) * (page_rows * kRowBytes) +
+                              place[i] * kRowBytes;
+#pragma unroll
+        for (int c = 0; c < kPieces; ++c) {
+          if (all) {
+            cp_async_all(k_to + stage + i * 16 * kRowBytes + c * 512, k_head + from + c * 512);
+            cp_async_all(v_to + stage + i * 16 * kRowBytes + c * 512, v_head + from + c * 512);
+          } else {
+            cp_async_16(k_to + stage + i * 16 * kRowBytes + c * 512, k_head + from + c * 512, page[i] >= 0);
+            cp_async_16(v_to + stage + i * 16 * kRowBytes + c * 512, v_head + from + c * 512, page[i] >= 0);
+          }
+        }
+      }
+      if (lane < 4 * kScaleChunks) {
+        const int mine = scale_tile ? page[1] : page[0];
+        cp_async_16(scale_to + stage, scale_head + static_cast<uint64_t>(static_cast<uint32_t>(max(mine, 0))) * (page_rows * G * 2) +
+                                          (scale_tile ? place[1] : place[0]) * (G * 2), mine >= 0);
+      }
+    }
+    cp_async_commit();
+  };
+
+#pragma unroll
+  for (int j = 0; j < kStages - 1; ++j) fetch(j);
+
+  // --- the queries in half precision: lane (g, t) has channels 32 group + 8 t .. + 7 of head 8 nt + g ---
+  uint32_t q[NT][G][4];       // neighbouring channels, the second and fourth pair a 16th
+  float q_offset[NT][G][2];   // -8 times the sum of a group's channels, of heads 2 t and 2 t + 1
+  float q_factor[NT][2];      // what a product has to be multiplied by, of the same heads; in units of log2
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const int h = head0 + nt * 8 + g;
+    float largest = 0.0f;
+    bool fine = true;
 #pragma unroll
     for (int gr = 0; gr < G; ++gr) {
       q[nt][gr][0] = q[nt][gr][1] = q[nt][gr][2] = q[nt][gr][3] = 0;
       if (h < group)
         load_words<4>(q[nt][gr], p.q + (static_cast<size_t>(token) * p.num_heads + kv_head * group + h) * D + 32 * gr + 8 * t);
     }
+#pragma unroll
+    for (int gr = 0; gr < G; ++gr)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        largest = fmaxf(largest, fmaxf(fabsf(low_of(q[nt][gr][w])), fabsf(high_of(q[nt][gr][w]))));
+        fine = fine && fabsf(low_of(q[nt][gr][w])) < INFINITY && fabsf(high_of(q[nt][gr][w])) < INFINITY;
+      }
+#pragma unroll
+    for (int offset = 1; offset <= 2; offset <<= 1) {
+      largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, offset));
+      fine = __shfl_xor_sync(0xffffffffu, static_cast<int>(fine), offset) && fine;
+    }
+    // the largest to 2^14 .. 2^15 (a number that is not finite: everything NaN)
+    const int exponent = static_cast<int>(__float_as_uint(largest) >> 23) - 127;
+    const int up = min(max(14 - exponent, -110), 110);
+    const float lift = fine ? __uint_as_float(static_cast<uint32_t>(127 + up) << 23) : __int_as_float(0x7fffffff);
+    const float factor = p.scale * kLog2e * __uint_as_float(static_cast<uint32_t>(127 - up) << 23) * 0x1p24f;   // a code is u 2^-24
+    q_factor[nt][0] = __shfl_sync(0xffffffffu, factor, 8 * t);
+    q_factor[nt][1] = __shfl_sync(0xffffffffu, factor, 8 * t + 4);
+#pragma unroll
+    for (int gr = 0; gr < G; ++gr) {
+      float total = 0.0f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float lo = low_of(q[nt][gr][w]) * lift, hi = high_of(q[nt][gr][w]) * lift;
+        total += lo + hi;
+        q[nt][gr][w] = w & 1 ? pack_half(lo * 0.0625f, hi * 0.0625f) : pack_half(lo, hi);
+      }
+      total += __shfl_xor_sync(0xffffffffu, total, 1);
+      total += __shfl_xor_sync(0xffffffffu, total, 2);
+      q_offset[nt][gr][0] = -8.0f * 0x1p-24f * __shfl_sync(0xffffffffu, total, 8 * t);
+      q_offset[nt][gr][1] = -8.0f * 0x1p-24f * __shfl_sync(0xffffffffu, total, 8 * t + 4);
+    }
   }
-  float o[NT][2 * G][4];      // channels 32 gr + 4 g + 2 h and the next (rows g, g + 8), heads 2 t and 2 t + 1
-  float most[NT][2], sum[NT][2];
+  const uint32_t magic = p.magic;
+  float o[NT][2 * G][4];      // channels 32 gr + 4 g + 2 h and the next (rows g, g + 8), heads 2 t and 2 t + 1, of codes + 136
+  float w_sum[NT][G / 2][4];  // sums of the scaled weights: rows below 8 of a pair's first group, rows above of its second
+  float most[NT][2], base[NT][2], sum[NT][2];   // base: most, or 0 where nothing has been seen
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     most[nt][0] = most[nt][1] = -INFINITY;
+    base[nt][0] = base[nt][1] = 0.0f;
     sum[nt][0] = sum[nt][1] = 0.0f;
 #pragma unroll
-    for (int m = 0; m < 2 * G; ++m)
+    for (int i = 0; i < 4; ++i) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[nt][m][i] = 0.0f;
+      for (int m = 0; m < 2 * G; ++m) o[nt][m][i] = 0.0f;
+#pragma unroll
+      for (int pair = 0; pair < G / 2; ++pair) w_sum[nt][pair][i] = 0.0f;
+    }
   }
-  const float scale_log2 = p.scale * kLog2e;
+  const uint32_t ones[2][4] = {{kOnes, 0, kOnes, 0}, {0, kOnes, 0, kOnes}};
+  const int row_key = 4 * (g & 1) + (g >> 1);                       // the key of accumulator row g
+  const uint32_t v_from = t * kRowBytes + (kChunks == 4 ? ((g >> 1) ^ (t & 2)) * 16 + (g & 1) * 8 : g * (2 * G));
 
-  for (int key0 = begin + warp * kWarpKeys; key0 < end; key0 += kWarps * kWarpKeys) {
-    Tile<D> tile[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) tile[i].load(p, table, kv_head, key0 + 16 * i, first, last, lane);
-    float s[2][NT][4];        // keys g (0, 1) and g + 8 (2, 3), heads 2 t and 2 t + 1; in units of log2
+  for (int j = 0; j < steps; ++j) {
+    if (j > 0 && (j & 15) == 0) {   // the next 32 tiles' pages; those behind are on their way
+      if (j & 16) pages_now = page_of(2 * j + 32 + lane);
+      else pages_next = page_of(2 * j + 32 + lane);
+    }
+    fetch(j + kStages - 1);
+    cp_async_wait<kStages - 1>();
+    __syncwarp();
+    const Stage<D>& from = stages[j % kStages];
+    const int key0 = warp_begin + j * (kWarps * kWarpKeys);
+    float s[2][NT][4];        // rows g (0, 1) and g + 8 (2, 3), heads 2 t and 2 t + 1; in units of log2
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
+      uint32_t k[2][G], scale[2][G / 2];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) s[i][nt][c] = tile[i].key0 < 0 ? -INFINITY : 0.0f;
-      if (tile[i].key0 < 0) continue;
+      for (int r = 0; r < 2; ++r) {
+        load_words<G>(k[r], from.k[i] + (g + 8 * r) * kRowBytes + t * 4 * G);
+        load_words<G / 2>(scale[r], from.k_scale[i] + (row_key + 8 * r) * (G * 2));
+      }
 #pragma unroll
       for (int gr = 0; gr < G; ++gr) {
-        uint32_t a[2][4];
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          a[half][0] = codes_of(tile[i].k[0][gr], 2 * half);
-          a[half][1] = codes_of(tile[i].k[1][gr], 2 * half);
-          a[half][2] = codes_of(tile[i].k[0][gr], 2 * half + 1);
-          a[half][3] = codes_of(tile[i].k[1][gr], 2 * half + 1);
-        }
-        const uint32_t pair0 = tile[i].k_scale[0][gr / 2], pair1 = tile[i].k_scale[1][gr / 2];
-        const float scale0 = gr & 1 ? high_of(pair0) : low_of(pair0), scale1 = gr & 1 ? high_of(pair1) : low_of(pair1);
+        const uint32_t k0 = k[0][gr], k1 = k[1][gr], l0 = k0 >> 8, l1 = k1 >> 8;
+        const uint32_t a[4] = {k0 & 0x000f000fu, k1 & 0x000f000fu, k0 & 0x00f000f0u, k1 & 0x00f000f0u};
+        const uint32_t b[4] = {l0 & 0x000f000fu, l1 & 0x000f000fu, l0 & 0x00f000f0u, l1 & 0x00f000f0u};
+        const float scale0 = gr & 1 ? high_of(scale[0][gr / 2]) : low_of(scale[0][gr / 2]);
+        const float scale1 = gr & 1 ? high_of(scale[1][gr / 2]) : low_of(scale[1][gr / 2]);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-          mma_16816(acc, a[0], q[nt][gr][0], q[nt][gr][1]);
-          mma_16816(acc, a[1], q[nt][gr][2], q[nt][gr][3]);
-          s[i][nt][0] = fmaf(scale0, acc[0], s[i][nt][0]);
-          s[i][nt][1] = fmaf(scale0, acc[1], s[i][nt][1]);
-          s[i][nt][2] = fmaf(scale1, acc[2], s[i][nt][2]);
-          s[i][nt][3] = fmaf(scale1, acc[3], s[i][nt][3]);
+          float acc[4];
+          mma_half_from(acc, a, q[nt][gr][0], q[nt][gr][1], q_offset[nt][gr][0], q_offset[nt][gr][1]);
+          mma_half(acc, b, q[nt][gr][2], q[nt][gr][3]);
+          s[i][nt][0] = gr ? fmaf(scale0, acc[0], s[i][nt][0]) : scale0 * acc[0];
+          s[i][nt][1] = gr ? fmaf(scale0, acc[1], s[i][nt][1]) : scale0 * acc[1];
+          s[i][nt][2] = gr ? fmaf(scale1, acc[2], s[i][nt][2]) : scale1 * acc[2];
+          s[i][nt][3] = gr ? fmaf(scale1, acc[3], s[i][nt][3]) : scale1 * acc[3];
         }
       }
-      const bool whole = tile[i].key0 >= first && tile[i].key0 + 15 <= last;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) s[i][nt][c] *= scale_log2;
-      if (!whole) {
+        for (int c = 0; c < 4; ++c) s[i][nt][c] *= q_factor[nt][c & 1];
+    }
+    const bool whole = key0 >= first && key0 + kWarpKeys - 1 <= last;
+    if (!whole) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const int key = tile[i].key0 + g + 8 * r;
+          const int key = key0 + 16 * i + 8 * r + row_key;
           if (key < first || key > last) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) s[i][nt][2 * r] = s[i][nt][2 * r + 1] = -INFINITY;
           }
-          // a hidden key's weight is 0, and its scale must not make that NaN
-#pragma unroll
-          for (int n = 0; n < 2; ++n) {
-            const int value_key = tile[i].key0 + 2 * t + 8 * r + n;
-            if (value_key < first || value_key > last) {
-#pragma unroll
-              for (int w = 0; w < G / 2; ++w) tile[i].v_scale[r][n * (G / 2) + w] = 0;
-            }
-          }
         }
-      }
     }
-    // the running maximum of each head, over the eight lanes that hold its keys
-    float now[NT][2], safe[NT][2];
+    // Weights are taken against a maximum that follows when a score is 2^8 above it, so that most steps need no word among the
+    // eight lanes that hold a head's keys.
+    float high[NT][2];
     bool grown = false;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        float m = fmaxf(fmaxf(s[0][nt][c], s[0][nt][2 + c]), fmaxf(s[1][nt][c], s[1][nt][2 + c]));
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-        now[nt][c] = m = fmaxf(m, most[nt][c]);
-        safe[nt][c] = m == -INFINITY ? 0.0f : m;
-        grown = grown || m > most[nt][c];
+        high[nt][c] = fmaxf(fmaxf(s[0][nt][c], s[0][nt][2 + c]), fmaxf(s[1][nt][c], s[1][nt][2 + c]));
+        grown = grown || high[nt][c] > most[nt][c] + 8.0f;
       }
     if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          const float shrink = exp2f(most[nt][c] - safe[nt][c]);
+          float m = fmaxf(high[nt][c], most[nt][c]);
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+          base[nt][c] = m == -INFINITY ? 0.0f : m;
+          const float shrink = exp2_near(most[nt][c] - base[nt][c]);
+          most[nt][c] = m;
           sum[nt][c] *= shrink;
 #pragma unroll
-          for (int m = 0; m < 2 * G; ++m) {
-            o[nt][m][c] *= shrink;
-            o[nt][m][2 + c] *= shrink;
+          for (int n = 0; n < 2 * G; ++n) {
+            o[nt][n][c] *= shrink;
+            o[nt][n][2 + c] *= shrink;
           }
-          most[nt][c] = now[nt][c];
+#pragma unroll
+          for (int pair = 0; pair < G / 2; ++pair) {
+            w_sum[nt][pair][c] *= shrink;
+            w_sum[nt][pair][2 + c] *= shrink;
+          }
         }
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      if (tile[i].key0 < 0) continue;
-      uint32_t w[NT][2];      // weights of head g: keys 2 t, 2 t + 1 and 2 t + 8, 2 t + 9
+      uint32_t v[4][G / 2], scale[4][G / 2];     // of keys 4 n + t: a unit of 16 bits a group, and a scale
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        load_words<G / 2>(v[n], from.v[i] + v_from + 4 * n * kRowBytes);
+        load_words<G / 2>(scale[n], from.v_scale[i] + (4 * n + t) * (G * 2));
+      }
+      if (!whole) {   // a hidden key's weight is 0, and its scale must not make that NaN
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const int key = key0 + 16 * i + 4 * n + t;
+          if (key < first || key > last) {
+#pragma unroll
+            for (int w = 0; w < G / 2; ++w) scale[n][w] = 0;
+          }
+        }
+      }
+      uint32_t w[NT][2];      // weights of head g: keys t, 4 + t and 8 + t, 12 + t
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float weight[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          weight[c] = exp2f(s[i][nt][c] - safe[nt][c & 1]);
+          weight[c] = exp2_near(s[i][nt][c] - base[nt][c & 1]);
           sum[nt][c & 1] += weight[c];
         }
         w[nt][0] = turn_8x8(pack_bf16(weight[0], weight[1]));
@@ -266,32 +421,40 @@ __global__ void __launch_bounds__(32 * kWarps) attention_q4_decode_kernel(Decode
       }
 #pragma unroll
       for (int gr = 0; gr < G; ++gr) {
-        uint32_t pairs[2], scales[2];   // of the keys 2 t, 2 t + 1 and of 2 t + 8, 2 t + 9
+        const uint32_t pick = gr & 1 ? 0x7632u : 0x5410u;
+        uint32_t pairs[2], b[NT][2];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const uint32_t pick = gr & 1 ? 0x7632u : 0x5410u;
-          pairs[r] = __byte_perm(tile[i].v[2 * r][gr / 2], tile[i].v[2 * r + 1][gr / 2], pick);
-          scales[r] = __byte_perm(tile[i].v_scale[r][gr / 2], tile[i].v_scale[r][G / 2 + gr / 2], pick);
-        }
-        uint32_t b[NT][2];
+          pairs[r] = __byte_perm(v[2 * r][gr / 2], v[2 * r + 1][gr / 2], pick);
+          const uint32_t scales = __byte_perm(scale[2 * r][gr / 2], scale[2 * r + 1][gr / 2], pick);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          b[nt][0] = mul_bf16x2(w[nt][0], scales[0]);
-          b[nt][1] = mul_bf16x2(w[nt][1], scales[1]);
+          for (int nt = 0; nt < NT; ++nt) b[nt][r] = mul_bf16x2(w[nt][r], scales);
         }
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           uint32_t a[4];
-          a[0] = codes_of(pairs[0], 2 * half);
-          a[1] = codes_of(pairs[0], 2 * half + 1);
-          a[2] = codes_of(pairs[1], 2 * half);
-          a[3] = codes_of(pairs[1], 2 * half + 1);
+          a[0] = codes_of(pairs[0], 2 * half, magic);
+          a[1] = codes_of(pairs[0], 2 * half + 1, magic);
+          a[2] = codes_of(pairs[1], 2 * half, magic);
+          a[3] = codes_of(pairs[1], 2 * half + 1, magic);
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma_16816(o[nt][2 * gr + half], a, b[nt][0], b[nt][1]);
+          for (int nt = 0; nt < NT; ++nt) mma_bf16(o[nt][2 * gr + half], a, b[nt][0], b[nt][1]);
         }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) mma_bf16(w_sum[nt][gr / 2], ones[gr & 1], b[nt][0], b[nt][1]);
       }
     }
+    __syncwarp();   // the stage is free
   }
+  cp_async_wait<0>();
+  __syncthreads();  // the stages become the warps' partials
+  float* merge = reinterpret_cast<float*>(shared);
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int m = 0; m < 2 * G; ++m)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) o[nt][m][c] = fmaf(-kOffset, w_sum[nt][m / 4][(m & 2) + (c & 1)], o[nt][m][c]);
 
   // each warp leaves its partial in shared memory
   float* mine = merge + warp * (8 * NT * kRow);
@@ -355,8 +518,12 @@ __global__ void __launch_bounds__(32 * kWarps) attention_q4_decode_kernel(Decode
 
 template <int D, int NT>
 int launch(const DecodeParams& p, cudaStream_t s) {
-  constexpr int kSmem = kWarps * 8 * NT * (D + 4) * 4;
-  static_assert(kSmem <= 48 * 1024, "shared memory that needs no opt-in");
+  constexpr int kSmem = kWarps * kStages * static_cast<int>(sizeof(Stage<D>));
+  static_assert(kWarps * 8 * NT * (D + 4) * 4 <= kSmem, "the warps' partials fit in their stages");
+  if (kSmem > 48 * 1024) {   // every device has to be asked
+    cudaError_t error = cudaFuncSetAttribute(attention_q4_decode_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    if (error != cudaSuccess) return static_cast<int>(error);
+  }
   const int group = p.num_heads / p.num_kv_heads, head_tiles = (group + 8 * NT - 1) / (8 * NT);
   const dim3 grid(p.num_entries, p.num_kv_heads * head_tiles, p.num_splits + (p.keep_first > 0 ? 1 : 0));
   int status = vipera_launch(attention_q4_decode_kernel<D, NT>, grid, 32 * kWarps, kSmem, s, p);
@@ -391,6 +558,7 @@ VIPERA_API int vipera_attention_q4_decode(const DecodeParams* given, float* scra
     return VIPERA_BAD_ARGUMENT;
   p.partial_ml = scratch;
   p.partial_out = scratch + pairs;
+  p.magic = 0x43004300u;
   p.page_shift = -1;
   if ((p.page_size & (p.page_size - 1)) == 0)
     for (p.page_shift = 0; (1 << p.page_shift) < p.page_size;) ++p.page_shift;

@@ -237,6 +237,17 @@ PYBIND11_MODULE(_vipera_runtime, m) {
              }
              return n;
            })
+      // The pages of several requests one behind the other: (where each request's begin, one item more than requests; the
+      // pages, -1 where a window has given one back).
+      .def("page_lists", [](const CacheManager& c, const std::vector<int64_t>& requests, int g) {
+        std::vector<int32_t> starts(1, 0), pages;
+        for (int64_t request : requests) {
+          const std::vector<int32_t>& table = c.table(request, g);
+          pages.insert(pages.end(), table.begin(), table.end());
+          starts.push_back(static_cast<int32_t>(pages.size()));
+        }
+        return py::make_tuple(to_array(starts), to_array(pages));
+      })
       // Block tables of several requests as one [len(requests), width] int32 array; logical
       // pages a request does not hold are -1.
       .def("tables", [](const CacheManager& c, const std::vector<int64_t>& requests, int g, int width) {

@@ -121,6 +121,8 @@ class Engine:
     ``lookahead``: while a step of greedy decoding runs, the step after it is launched already
     where the scheduler can foresee it, so that the host's share of a step (scheduling, input
     copies, the launch, reading tokens back) hides behind the device's.
+    ``kv_type="q4"`` holds keys and values in 4 bits (codes of groups of 32 channels with a scale each, 4.5 bits a value) for
+    models whose attention takes such pages; None: in the run's type.
     ``ctx`` is the context length each of ``max_num_seqs`` requests can reach with the
     pages allocated (default: the smaller of the model's limit and 2048, as the reference's
     ``--ctx``, bins/vipera/src/main.rs:655-663); ``num_pages`` overrides that sizing.
@@ -130,7 +132,7 @@ class Engine:
                  num_pages: Optional[int] = None, ctx: Optional[int] = None, max_num_seqs: int = 4,
                  max_tokens_per_step: int = 2048, max_portion: Optional[int] = None,
                  max_model_len: Optional[int] = None, decode_graphs: bool = True, prefix_cache: bool = True,
-                 lookahead: bool = True):
+                 lookahead: bool = True, kv_type: Optional[str] = None):
         if isinstance(model, str):
             model = load_model(model, dtype, device)
         self.model = model
@@ -142,7 +144,7 @@ class Engine:
             num_pages = max_num_seqs * ((ctx + page_size - 1) // page_size)
         self.pools = CachePools(model.cache_requests, page_size=page_size, num_pages=num_pages,
                                 num_state_slots=max_num_seqs, dtype=model.dtype, device=model.device,
-                                reuse_prefixes=prefix_cache)
+                                reuse_prefixes=prefix_cache, kv_type=kv_type)
         self.runner = ModelRunner(model, self.pools, max_model_len=self.max_model_len)
         self.runner.decode_graphs = decode_graphs
         runtime = runtime_module()

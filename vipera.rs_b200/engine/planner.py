@@ -11,7 +11,7 @@ from __future__ import annotations
 
 from typing import Dict, Optional
 
-from ..cache.pools import plan_groups
+from ..cache.pools import check_kv_type, plan_groups
 from ..config.registry import BLOCKS
 from ..config.spec import ModelSpec
 from ..parts.model import model_schema
@@ -59,15 +59,19 @@ def parameter_count(spec: ModelSpec) -> int:
     return total
 
 
-def cache_bytes(spec: ModelSpec, ctx: int, batch: int, element_bytes: int, page_size: int = 16) -> int:
+def _group_tokens(group, ctx: int, page_size: int) -> int:
+    """Tokens that a request of `ctx` tokens holds pages for in a group, whole pages of them."""
+    tokens = ctx if not group.window else min(ctx, group.window + page_size)
+    return -(-tokens // page_size) * page_size
+
+
+def cache_bytes(spec: ModelSpec, ctx: int, batch: int, element_bytes: int, page_size: int = 16, kv_type: Optional[str] = None) -> int:
     """Pages for `batch` requests of `ctx` tokens in every group of layers (a windowed group
     holds a window and a page's slack per request), and the fixed-size states."""
     groups, states = plan_groups(spec_cache_requests(spec))
     total = 0
     for group in groups:
-        tokens = ctx if not group.window else min(ctx, group.window + page_size)
-        pages = -(-tokens // page_size)
-        total += batch * pages * page_size * group.bytes_per_token(element_bytes)
+        total += batch * _group_tokens(group, ctx, page_size) * group.bytes_per_token(element_bytes, kv_type)
     for state in states.values():
         count = 1
         for extent in state.shape:
@@ -76,9 +80,17 @@ def cache_bytes(spec: ModelSpec, ctx: int, batch: int, element_bytes: int, page_
     return total
 
 
-def kv_bytes_per_token(spec: ModelSpec, element_bytes: int) -> int:
+def kv_bytes_per_token(spec: ModelSpec, element_bytes: int, kv_type: Optional[str] = None) -> int:
     groups, _ = plan_groups(spec_cache_requests(spec))
-    return sum(group.bytes_per_token(element_bytes) for group in groups)
+    return sum(group.bytes_per_token(element_bytes, kv_type) for group in groups)
+
+
+def room_bytes(spec: ModelSpec, ctx: int, batch: int, element_bytes: int, page_size: int = 16) -> int:
+    """What attention over pages of 4 bits expands a layer's rows to where it does not read them packed: one cache slot's pages in the
+    run's type, of the group where they are the largest (layers share the room)."""
+    groups, _ = plan_groups(spec_cache_requests(spec))
+    return max((batch * _group_tokens(group, ctx, page_size) + page_size) * group.bytes_per_token(element_bytes) // len(group.slots)
+               for group in groups)
 
 
 def workspace_bytes(spec: ModelSpec, batch: int, element_bytes: int, tokens: int = PLANNED_STEP_TOKENS) -> int:
@@ -92,13 +104,16 @@ def workspace_bytes(spec: ModelSpec, batch: int, element_bytes: int, tokens: int
 
 
 def plan_memory(spec: ModelSpec, ctx: int, batch: int, dtype: str, device_bytes: Optional[int] = None,
-                page_size: int = 16) -> dict:
+                page_size: int = 16, kv_type: Optional[str] = None) -> dict:
     """Weights + cache + workspace against the device's memory; what does not fit is listed in
-    ``violations``, and ``feasible`` says whether the list is empty."""
+    ``violations``, and ``feasible`` says whether the list is empty.  ``kv_type`` as the engine's."""
     element = _element_bytes(dtype)
+    kv_type = check_kv_type(kv_type, spec_cache_requests(spec))
     weights = weight_bytes(spec, element)
-    kv = cache_bytes(spec, ctx, batch, element, page_size)
+    kv = cache_bytes(spec, ctx, batch, element, page_size, kv_type)
     workspace = workspace_bytes(spec, batch, element)
+    if kv_type:
+        workspace += room_bytes(spec, ctx, batch, element, page_size)
     if device_bytes is None:
         try:
             import torch
@@ -119,7 +134,7 @@ def plan_memory(spec: ModelSpec, ctx: int, batch: int, dtype: str, device_bytes:
                            "available_bytes": device_bytes,
                            "message": f"{required} bytes needed, {device_bytes} on the device"})
     return {"architecture": spec.architecture, "ctx": ctx, "batch_size": batch, "dtype": dtype,
-            "weight_bytes": weights, "kv_bytes": kv, "kv_bytes_per_token": kv_bytes_per_token(spec, element),
+            "weight_bytes": weights, "kv_bytes": kv, "kv_bytes_per_token": kv_bytes_per_token(spec, element, kv_type),
             "workspace_bytes": workspace, "reserve_bytes": DEVICE_RESERVE_BYTES,
             "predicted_device_bytes": required, "device_bytes": int(device_bytes),
             "feasible": not violations, "violations": violations}

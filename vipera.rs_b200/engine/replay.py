@@ -21,11 +21,12 @@ from .runner import ModelRunner, StepInput
 
 class Replayer:
     def __init__(self, model_dir: str, dtype: str, *, max_tokens: int, page_size: int = 64,
-                 device: str = "cuda:0", max_live: int = 4):
+                 device: str = "cuda:0", max_live: int = 4, kv_type: Optional[str] = None):
         self.model = load_model(model_dir, dtype, device)
         pages = max(1, (int(max_tokens) + page_size - 1) // page_size)
         self.pools = CachePools(self.model.cache_requests, page_size=page_size, num_pages=pages,
-                                num_state_slots=max_live, dtype=self.model.dtype, device=self.model.device)
+                                num_state_slots=max_live, dtype=self.model.dtype, device=self.model.device,
+                                kv_type=kv_type)
         if os.environ.get("VIPERA_POISON_CACHE") == "1":
             # Unwritten cache memory reads as NaN, so a key that was never stored shows.
             self.pools.poison()

@@ -166,10 +166,10 @@ class ModelRunner:
         if step.logit_rows.size and (int(step.logit_rows.min()) < 0 or int(step.logit_rows.max()) >= total):
             raise InvalidArgumentError("a wanted row lies outside the step's tokens")
 
-    def _host_arrays(self, step: StepInput, widths=None):
+    def _host_arrays(self, step: StepInput, widths):
         """The step's description as host arrays, checked: per token (positions, entry), per
         entry (starts, first position, state slot, fresh), wanted rows, and per group the block
-        tables, as wide as `widths` says or as the longest request needs."""
+        tables, as wide as `widths` says."""
         self.validate(step)
         counts = np.asarray(step.counts, dtype=np.int32)
         pos0 = np.asarray(step.pos0, dtype=np.int32)
@@ -184,8 +184,7 @@ class ModelRunner:
         tables = []
         for g in range(self.manager.num_groups):
             page_size = self._page_sizes[g]
-            width = widths[g] if widths is not None else _round_up_pow2((max_len + page_size - 1) // page_size)
-            table = self.manager.tables(list(step.requests), g, width)
+            table = self.manager.tables(list(step.requests), g, widths[g])
             # Every position of the step must have its page.
             last_page = (pos0 + counts - 1) // page_size
             if (table[np.arange(entries), last_page] < 0).any():
@@ -196,32 +195,59 @@ class ModelRunner:
         return counts, pos0, starts, token_entry, positions, rows, tables, slots, fresh, max_len
 
     def build_context(self, step: StepInput, dtype: torch.dtype) -> StepContext:
-        counts, pos0, starts, token_entry, positions, rows, tables, slots, fresh, max_len = self._host_arrays(step)
-        entries, total = counts.shape[0], int(starts[-1])
-        pieces = [step.tokens.astype(np.int32, copy=False), positions, token_entry, starts, pos0, slots, fresh, rows]
-        pieces += [t.reshape(-1) for t in tables]
-        sizes = [p.shape[0] for p in pieces]
-        host, dev = self._staging(sum(sizes))
+        """The step's description for the device.  Only lengths and the requests' pages are copied there; positions, the tokens'
+        entries and the block tables are built from them on the device."""
+        from ..kernels import ops
+
+        self.validate(step)
+        counts = np.asarray(step.counts, dtype=np.int32)
+        pos0 = np.asarray(step.pos0, dtype=np.int32)
+        entries, total = counts.shape[0], int(counts.sum())
+        starts = np.zeros(entries + 1, dtype=np.int32)
+        np.cumsum(counts, out=starts[1:])
+        rows = np.asarray(step.logit_rows, dtype=np.int32)
+        slots = np.asarray([self.manager.state_slot(r) for r in step.requests], dtype=np.int32)
+        max_len = int((pos0 + counts).max())
+        pieces = [step.tokens.astype(np.int32, copy=False), starts, pos0, slots, np.asarray(step.fresh, dtype=np.int32), rows]
+        widths = []
+        for g, page_size in enumerate(self._page_sizes):
+            page_starts, pages = self.manager.page_lists(list(step.requests), g)
+            # Every position of the step must have its page.
+            last = page_starts[:-1] + (pos0 + counts - 1) // page_size
+            if (last >= page_starts[1:]).any() or (pages[last] < 0).any():
+                raise InvalidArgumentError("a request of the step has no page reserved for its last position")
+            widths.append(_round_up_pow2(max((max_len + page_size - 1) // page_size, int(np.diff(page_starts).max()))))
+            pieces += [page_starts, pages]
+        # what the device builds lies behind what is copied: positions, the tokens' entries, the tables
+        sizes = [p.shape[0] for p in pieces] + [total, total] + [entries * width for width in widths]
+        offsets = np.concatenate([[0], np.cumsum(sizes)]).astype(np.int64).tolist()
+        host, dev = self._staging(offsets[-1])
         if self._copy_pending:
             self._copy_done.synchronize()
         view = host.numpy()
-        offsets, cursor = [], 0
-        for piece, size in zip(pieces, sizes):
-            view[cursor:cursor + size] = piece
-            offsets.append(cursor)
-            cursor += size
-        dev[:cursor].copy_(host[:cursor], non_blocking=True)
+        for piece, offset in zip(pieces, offsets):
+            view[offset:offset + piece.shape[0]] = piece
+        copied = offsets[len(pieces)]
+        dev[:copied].copy_(host[:copied], non_blocking=True)
         self._copy_done.record()
         self._copy_pending = True
 
         def part(index):
-            return dev[offsets[index]:offsets[index] + sizes[index]]
+            return dev[offsets[index]:offsets[index + 1]]
 
-        block_tables = [part(8 + g).view(entries, tables[g].shape[1]) for g in range(len(tables))]
+        behind = len(pieces)
+        positions, token_entry = part(behind), part(behind + 1)
+        block_tables = [part(behind + 2 + g).view(entries, width) for g, width in enumerate(widths)]
+        if not block_tables:     # nothing is kept in pages
+            ops.step_maps(part(1), part(2), page_size=1, block_table=dev[:0].view(entries, 0), positions=positions, token_entry=token_entry)
+        for g, table in enumerate(block_tables):
+            per_token = {} if g else dict(positions=positions, token_entry=token_entry)
+            ops.step_maps(part(1), part(2), page_size=self._page_sizes[g], block_table=table, page_starts=part(6 + 2 * g),
+                          pages=part(7 + 2 * g), **per_token)
         return StepContext(
-            num_tokens=total, num_entries=entries, tokens=part(0), positions=part(1), token_entry=part(2),
-            entry_starts=part(3), entry_pos0=part(4), state_slots=part(5), fresh=part(6),
-            block_tables=block_tables, logit_rows=part(7) if rows.size else None, num_logit_rows=int(rows.size),
+            num_tokens=total, num_entries=entries, tokens=part(0), positions=positions, token_entry=token_entry,
+            entry_starts=part(1), entry_pos0=part(2), state_slots=part(3), fresh=part(4),
+            block_tables=block_tables, logit_rows=part(5) if rows.size else None, num_logit_rows=int(rows.size),
             host_counts=[int(c) for c in counts], host_pos0=[int(p) for p in pos0],
             max_count=int(counts.max()), max_kv_len=max_len, all_single=bool((counts == 1).all()),
             any_single=bool((counts == 1).any()), dtype=self.model.dtype, workspace=self.workspace,
@@ -229,6 +255,14 @@ class ModelRunner:
 
     def forward(self, ctx: StepContext) -> Optional[torch.Tensor]:
         """The model's forward pass for a prepared step."""
+        if self.pools.kv_type == "q4":
+            # where the step's rows go, once for all layers of a group
+            from ..kernels import ops
+
+            ctx.slots = []
+            for g, table in enumerate(ctx.block_tables):
+                ctx.slots.append(self.workspace.get(f"step.slots.{g}", (ctx.num_tokens,), torch.int32))
+                ops.step_maps(ctx.entry_starts, ctx.entry_pos0, page_size=self._page_sizes[g], block_table=table, slots=ctx.slots[g])
         return self.model.forward(ctx, self.pools.views)
 
     def run(self, step: StepInput) -> Optional[torch.Tensor]:

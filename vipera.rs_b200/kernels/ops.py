@@ -1091,24 +1091,49 @@ class _DecodeQ4Params(ctypes.Structure):
                 ("gate_stride", ctypes.c_longlong), ("gate_per_head", _c_int), ("table_width", _c_int), ("page_size", _c_int),
                 ("page_shift", _c_int), ("num_pages", _c_int), ("num_entries", _c_int), ("num_heads", _c_int),
                 ("num_kv_heads", _c_int), ("head_dim", _c_int), ("scale", _c_float), ("window", _c_int), ("keep_first", _c_int),
-                ("sink", _c_int), ("chunk", _c_int), ("num_splits", _c_int)]
+                ("sink", _c_int), ("chunk", _c_int), ("num_splits", _c_int), ("magic", ctypes.c_uint)]
 
 
-def _one_device(what: str, *tensors) -> None:
-    """The tensors lie on the current device, whose stream the launch goes to."""
-    here = torch.cuda.current_device()
-    for tensor in tensors:
-        if tensor is not None and tensor.is_cuda and tensor.get_device() != here:
-            raise InvalidArgumentError(f"{what}: a tensor is on {tensor.device}, the current device is cuda:{here}")
+def _place(what: str, tensor: torch.Tensor, dtype: torch.dtype, here: int) -> int:
+    """The address of a contiguous tensor of `dtype` on device `here`, the current one, whose stream the launch goes to."""
+    if tensor.dtype is not dtype or not tensor.is_contiguous() or tensor.get_device() != here:
+        if tensor.dtype is not dtype:
+            raise InvalidArgumentError(f"{what}: a tensor is {tensor.dtype} in the place of {dtype}")
+        if not tensor.is_contiguous():
+            raise InvalidArgumentError(f"{what}: tensors must be contiguous")
+        if not tensor.is_cuda:
+            raise InternalError(f"{what}: a tensor is not on a CUDA device; this engine has no CPU path")
+        raise InvalidArgumentError(f"{what}: a tensor is on {tensor.device}, the current device is cuda:{here}")
+    return tensor.data_ptr()
+
+
+def _place_pages(what: str, pages: Q4Pages, here: int):
+    """The addresses of the pages' parts: codes of keys and values, scales of keys and values."""
+    k_codes, k_scales, v_codes, v_scales = pages
+    return (_place(what, k_codes, torch.uint8, here), _place(what, v_codes, torch.uint8, here),
+            _place(what, k_scales, torch.bfloat16, here), _place(what, v_scales, torch.bfloat16, here))
+
+
+@functools.lru_cache(maxsize=None)
+def _sm_count_of(index: int) -> int:
+    return sm_count(torch.device("cuda", index))
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # absent in a torch without CUDA
+
+
+def _stream_of(here: int) -> int:
+    return _raw_stream(here) if _raw_stream is not None else torch.cuda.current_stream(here).cuda_stream
 
 
 def _check_q4_pages(what: str, pages: Q4Pages, num_kv_heads: int, head_dim: int) -> int:
     """The pages' page size, their shapes and types being those of the head counts and sizes."""
     if head_dim % Q4_GROUP or not 0 < head_dim <= 256:
         raise UnsupportedError(f"{what}: heads of 4 bits have a multiple of {Q4_GROUP} channels up to 256, not {head_dim}")
-    shape = pages.k_codes.shape
-    if len(shape) != 4 or shape[1] != num_kv_heads or shape[3] != head_dim // 2 or pages.v_codes.shape != shape \
-            or pages.k_scales.shape != (*shape[:3], head_dim // Q4_GROUP) or pages.v_scales.shape != pages.k_scales.shape:
+    k_codes, k_scales, v_codes, v_scales = pages
+    shape, groups = k_codes.shape, k_scales.shape
+    if len(shape) != 4 or len(groups) != 4 or shape[1] != num_kv_heads or shape[3] * 2 != head_dim or v_codes.shape != shape \
+            or groups[3] * Q4_GROUP != head_dim or groups[:3] != shape[:3] or v_scales.shape != groups:
         raise InvalidArgumentError(f"{what}: pages of 4 bits are codes [pages, kv_heads, page_size, d / 2] and scales "
                                    "[pages, kv_heads, page_size, d / 32]")
     return shape[2]
@@ -1133,17 +1158,15 @@ def step_maps(entry_starts: torch.Tensor, entry_pos0: torch.Tensor, *, page_size
         raise InvalidArgumentError("step_maps: pages come with page_starts, one item more than there are entries")
     if page_size <= 0 or entries > 65535:
         raise InvalidArgumentError("step_maps: a page holds at least one token, a step has at most 65535 entries")
-    per_token = [t for t in (positions, token_entry, slots) if t is not None]
-    tokens = per_token[0].numel() if per_token else 0
-    if any(t.numel() != tokens for t in per_token):
+    counts = {t.numel() for t in (positions, token_entry, slots) if t is not None}
+    tokens = counts.pop() if counts else 0
+    if counts:
         raise InvalidArgumentError("step_maps: positions, token_entry and slots hold one number for each token")
-    _one_device("step_maps", entry_starts, entry_pos0, block_table, page_starts, pages, *per_token)
-    int32 = torch.int32
-    p = _MapsParams(_gpu(entry_starts, "entry_starts", int32), _gpu(entry_pos0, "entry_pos0", int32),
-                    _opt(page_starts, "page_starts", int32), _opt(pages, "pages", int32), _gpu(block_table, "block_table", int32),
-                    _opt(positions, "positions", int32), _opt(token_entry, "token_entry", int32), _opt(slots, "slots", int32),
-                    entries, tokens, 0 if pages is None else pages.numel(), block_table.shape[1], page_size)
-    _check(fn(ctypes.byref(p), _stream()), "step_maps")
+    here, int32, what = torch.cuda.current_device(), torch.int32, "step_maps"
+    at = [None if t is None else _place(what, t, int32, here)
+          for t in (entry_starts, entry_pos0, page_starts, pages, block_table, positions, token_entry, slots)]
+    p = _MapsParams(*at, entries, tokens, 0 if pages is None else pages.numel(), block_table.shape[1], page_size)
+    _check(fn(p, _stream_of(here)), what)
 
 
 def rope_cache_q4(qkv: torch.Tensor, q_out: torch.Tensor, pages: Q4Pages, *, num_heads: int, num_kv_heads: int, head_dim: int,
@@ -1170,16 +1193,16 @@ def rope_cache_q4(qkv: torch.Tensor, q_out: torch.Tensor, pages: Q4Pages, *, num
         if cos is None or sin is None or cos.dim() != 2 or cos.shape[1] != rot_dims // 2 or sin.shape != cos.shape or not cos.shape[0]:
             raise InvalidArgumentError("rope_cache_q4: cos/sin tables of width rot_dims/2 are needed")
         table_rows = cos.shape[0]
-    if not qkv.is_cuda or qkv.dtype != torch.float32:
-        raise InvalidArgumentError("rope_cache_q4: qkv must be float32 on a CUDA device")
-    _one_device("rope_cache_q4", qkv, q_out, *pages, positions, cos, sin, slots)
-    u8, bf16 = torch.uint8, torch.bfloat16
-    p = _StoreQ4Params(qkv.data_ptr(), qkv.stride(0), _gpu(q_out, "q_out"), _gpu(pages.k_codes, "k_codes", u8),
-                       _gpu(pages.v_codes, "v_codes", u8), _gpu(pages.k_scales, "k_scales", bf16), _gpu(pages.v_scales, "v_scales", bf16),
-                       _gpu(positions, "positions", torch.int32), _opt(cos, "cos", torch.float32), _opt(sin, "sin", torch.float32),
-                       _opt(slots, "slots", torch.int32), pages.k_codes.shape[0] * page_size if slots is not None else 0, table_rows,
-                       count, num_heads, num_kv_heads, head_dim, rot_dims, style, page_size)
-    _check(fn(ctypes.byref(p), dtype_code(q_out.dtype), _stream()), "rope_cache")
+    here, int32, what = torch.cuda.current_device(), torch.int32, "rope_cache_q4"
+    if qkv.dtype is not torch.float32 or qkv.get_device() != here:     # its rows may lie apart
+        raise InvalidArgumentError("rope_cache_q4: qkv must be float32 on the current CUDA device")
+    k_codes, v_codes, k_scales, v_scales = _place_pages(what, pages, here)
+    cos_at, sin_at = (_place(what, cos, torch.float32, here), _place(what, sin, torch.float32, here)) if table_rows else (None, None)
+    p = _StoreQ4Params(qkv.data_ptr(), qkv.stride(0), _place(what, q_out, q_out.dtype, here), k_codes, v_codes, k_scales, v_scales,
+                       _place(what, positions, int32, here), cos_at, sin_at, None if slots is None else _place(what, slots, int32, here),
+                       0 if slots is None else pages.k_codes.shape[0] * page_size, table_rows, count, num_heads, num_kv_heads, head_dim,
+                       rot_dims, style, page_size)
+    _check(fn(p, dtype_code(q_out.dtype), _stream_of(here)), "rope_cache")
 
 
 def expand_q4(pages: Q4Pages, k_room: torch.Tensor, v_room: torch.Tensor, *, entry_starts: torch.Tensor, entry_pos0: torch.Tensor,
@@ -1198,20 +1221,45 @@ def expand_q4(pages: Q4Pages, k_room: torch.Tensor, v_room: torch.Tensor, *, ent
     entries = entry_pos0.numel()
     if entry_starts.numel() != entries + 1 or block_table.dim() != 2 or block_table.shape[0] != entries:
         raise InvalidArgumentError("expand_q4: entry_starts has one item more than entry_pos0, the block table a row for each entry")
-    _one_device("expand_q4", *pages, k_room, v_room, entry_starts, entry_pos0, block_table)
-    u8, bf16, int32 = torch.uint8, torch.bfloat16, torch.int32
-    p = _ExpandQ4Params(_gpu(pages.k_codes, "k_codes", u8), _gpu(pages.v_codes, "v_codes", u8), _gpu(pages.k_scales, "k_scales", bf16),
-                        _gpu(pages.v_scales, "v_scales", bf16), _gpu(k_room, "k_room"), _gpu(v_room, "v_room"),
-                        _gpu(entry_starts, "entry_starts", int32), _gpu(entry_pos0, "entry_pos0", int32),
-                        _gpu(block_table, "block_table", int32), block_table.shape[1], page_size, entries, num_pages, num_kv_heads,
+    here, int32, what = torch.cuda.current_device(), torch.int32, "expand_q4"
+    width = block_table.shape[1]
+    p = _ExpandQ4Params(*_place_pages(what, pages, here), _place(what, k_room, k_room.dtype, here), _place(what, v_room, k_room.dtype, here),
+                        _place(what, entry_starts, int32, here), _place(what, entry_pos0, int32, here),
+                        _place(what, block_table, int32, here), width, page_size, entries, num_pages, num_kv_heads,
                         head_dim, max(int(window or 0), 0), int(keep_first or 0), 1 if skip_single else 0)
-    blocks = min(4 * sm_count(k_room.device), max(1, 2 * entries * block_table.shape[1]))
-    _check(fn(ctypes.byref(p), dtype_code(k_room.dtype), blocks, _stream()), "expand_q4")
+    _check(fn(p, dtype_code(k_room.dtype), min(4 * _sm_count_of(here), max(1, 2 * entries * width)), _stream_of(here)), what)
 
 
 def attention_q4_takes_decode(dtype: torch.dtype, head_dim: int, page_size: int) -> bool:
     """Whether single tokens are attended over the packed pages directly."""
     return dtype == torch.bfloat16 and head_dim in MMA_HEAD_DIMS and page_size % 16 == 0
+
+
+# The packed kernel's blocks: three an SM at once, and a walk's time in microseconds: what a block costs beside its keys, and what each 128
+# of them cost where one, two or three blocks share an SM (fitted to launches at batch 1 to 64 and 2,048 to 32,768 keys).
+Q4_BLOCKS_PER_SM = 3
+Q4_BLOCK_FIXED, Q4_BLOCK_KEYS, Q4_SPLIT_JOIN = 2.2, (0.0, 0.8, 1.25, 1.75), 0.05
+
+
+@functools.lru_cache(maxsize=4096)
+def q4_splits(num_entries: int, num_head_tiles: int, max_keys: int, window: int, sm_count: int):
+    """How a step of single tokens over packed pages cuts its keys: (keys per split, splits), the cut that a model of the
+    launch's time likes best: whole waves of blocks, then what is left, for keys as many as a query sees."""
+    base, slots = num_entries * num_head_tiles, Q4_BLOCKS_PER_SM * sm_count
+    seen = min(max_keys, window + 127) if window else max_keys
+    best = None
+    for wanted in range(1, 65):
+        units = max(-(-seen // (128 * wanted)), -(-max_keys // (128 * 128)))     # at most 128 splits
+        if best is not None and units == best[1]:
+            continue
+        splits, total = -(-max_keys // (128 * units)), -(-seen // (128 * units))
+        full, rest = divmod(base * total, slots)
+        time = full * (Q4_BLOCK_FIXED + units * Q4_BLOCK_KEYS[3]) + Q4_SPLIT_JOIN * total
+        if rest:
+            time += Q4_BLOCK_FIXED + units * Q4_BLOCK_KEYS[-(-rest // sm_count)]
+        if best is None or time < best[0] - 1e-9:
+            best = (time, units, splits)
+    return 128 * best[1], best[2]
 
 
 def _attention_q4_decode(q, out, pages, *, positions, block_table, num_heads, num_kv_heads, head_dim, scale, max_keys, workspace,
@@ -1220,20 +1268,21 @@ def _attention_q4_decode(q, out, pages, *, positions, block_table, num_heads, nu
                    [ctypes.POINTER(_DecodeQ4Params), _c_void, ctypes.c_size_t, _c_void])
     _check_struct("attention_q4", "vipera_attention_q4_params_size", _DecodeQ4Params)
     entries = block_table.shape[0]
-    chunk, splits = decode_splits(entries, num_kv_heads, max(int(max_keys), 1), sm_count(q.device))
+    here, int32, what = torch.cuda.current_device(), torch.int32, "attention_q4"
+    width = block_table.shape[1]
+    group = num_heads // num_kv_heads
+    chunk, splits = q4_splits(entries, num_kv_heads * -(-group // (8 if group <= 8 else 16)), max_keys, window, _sm_count_of(here))
     scratch = workspace.get("attention.partials", (attention_decode_scratch_floats(
         entries, num_heads, head_dim, splits + (1 if keep_first else 0)),), torch.float32)
-    gate_pointer, gate_stride = _gate_pointer(gate, gate_offset, q.shape[0], num_heads * (1 if gate_per_head else head_dim),
-                                              "attention_q4")
-    u8, bf16, int32 = torch.uint8, torch.bfloat16, torch.int32
-    p = _DecodeQ4Params(_gpu(q, "q", bf16), _gpu(out, "out", bf16), _gpu(pages.k_codes, "k_codes", u8),
-                        _gpu(pages.v_codes, "v_codes", u8), _gpu(pages.k_scales, "k_scales", bf16),
-                        _gpu(pages.v_scales, "v_scales", bf16), _gpu(positions, "positions", int32),
-                        _gpu(block_table, "block_table", int32), _opt(entry_starts, "entry_starts", int32),
-                        _opt(sink_values, "sink_values", torch.float32), gate_pointer, None, None, gate_stride,
-                        int(bool(gate_per_head)), block_table.shape[1], pages.k_codes.shape[2], 0, pages.k_codes.shape[0], entries,
-                        num_heads, num_kv_heads, head_dim, float(scale), window, keep_first, 1 if sink else 0, chunk, splits)
-    _check(fn(ctypes.byref(p), scratch.data_ptr(), scratch.numel(), _stream()), "attention_decode", kernels=2)
+    gate_pointer, gate_stride = (None, 0) if gate is None else _gate_pointer(
+        gate, gate_offset, q.shape[0], num_heads * (1 if gate_per_head else head_dim), what)
+    p = _DecodeQ4Params(_place(what, q, torch.bfloat16, here), _place(what, out, torch.bfloat16, here), *_place_pages(what, pages, here),
+                        _place(what, positions, int32, here), _place(what, block_table, int32, here),
+                        None if entry_starts is None else _place(what, entry_starts, int32, here),
+                        None if sink_values is None else _place(what, sink_values, torch.float32, here), gate_pointer, None, None,
+                        gate_stride, 1 if gate_per_head else 0, width, pages.k_codes.shape[2], 0, pages.k_codes.shape[0], entries,
+                        num_heads, num_kv_heads, head_dim, scale, window, keep_first, 1 if sink else 0, chunk, splits, 0)
+    _check(fn(p, scratch.data_ptr(), scratch.numel(), _stream_of(here)), "attention_decode", kernels=2)
 
 
 def attention_q4(q: torch.Tensor, out: torch.Tensor, pages: Q4Pages, *, entry_starts: torch.Tensor, entry_pos0: torch.Tensor,
@@ -1265,7 +1314,6 @@ def attention_q4(q: torch.Tensor, out: torch.Tensor, pages: Q4Pages, *, entry_st
     window = int(window or 0)
     if window < 0 or keep_first < 0:
         raise InvalidArgumentError("attention_q4: a window and its kept first keys are counts")
-    _one_device("attention_q4", q, out, *pages, entry_starts, entry_pos0, positions, token_entry, block_table, sink_values, gate)
     if count == 0:
         return
     dtype_code(q.dtype)

@@ -21,7 +21,7 @@ from ..config.registry import MIXERS, POSITION_ENCODINGS
 from ..errors import UnsupportedError
 from ..kernels import ops
 from ..weights import TensorSpec
-from .base import Mixer, PagedKV
+from .base import Mixer, PagedKV, PagedQ4View
 from .linear import Linear, NormedInput
 from .rotary import QueryFactor
 
@@ -57,9 +57,10 @@ class GQAttention(Mixer):
     ``(1 - b) v + b v_source`` with ``b = <prefix>.vmix.weight`` (a single number) and ``v_source`` what
     the source layer published for the same token earlier in the step (both kinds hold the tensor;
     the source does not read it).  Handed no stream, the mixer leaves its output as rows (``rows_name``: the
-    buffer they are in)."""
+    buffer they are in).  Pages of 4 bits (a ``PagedQ4View``) are taken where ``_takes_four_bits`` says: keys and values of one
+    size of whole groups of 32, windows, kept first keys, sinks, gates and every position encoding among the options."""
 
-    kernels = ("rope_cache", "attention", "attention_mma", "attention_tc")
+    kernels = ("rope_cache", "attention", "attention_mma", "attention_tc", "cache_q4", "attention_q4")
     takes_lazy_input = True
     leaves_rows = True   # forward(ctx, h, None, ...) returns (rows [tokens, hidden] float32, 1)
     # With mixed head weights: steps of this many tokens and more that bring portions run every
@@ -239,6 +240,10 @@ class GQAttention(Mixer):
         # the tensor-core attention kernels serve bfloat16 with head sizes 64 and 128; everything
         # else runs through the general kernel
         own = ["rope_cache", "attention"]
+        if self._takes_four_bits(self.params):
+            own.append("cache_q4")
+            if self.dtype == torch.bfloat16 and self.head_dim in ops.MMA_HEAD_DIMS:
+                own.append("attention_q4")
         if self.talk is not None:
             own.append("attention_talk")
             if self.dtype == torch.bfloat16 and self.head_dim in ops.MMA_HEAD_DIMS and self.value_dim == self.head_dim:
@@ -265,7 +270,14 @@ class GQAttention(Mixer):
         window = params.get("window")
         return PagedKV(int(params["num_kv_heads"]), head_dim, window,
                        value_dim=value_dim if value_dim != head_dim else None,
-                       keep_first=int(params.get("keep_first") or 0) if window else 0)
+                       keep_first=int(params.get("keep_first") or 0) if window else 0, four_bit=cls._takes_four_bits(params))
+
+    @classmethod
+    def _takes_four_bits(cls, params) -> bool:
+        d, dv = cls._stored_sizes(params)
+        return (d == dv and d % ops.Q4_GROUP == 0 and d <= 256 and float(params.get("out_scale", 1.0)) == 1.0
+                and not any(params.get(key) for key in ("chunk", "values_from_keys", "row_norm", "head_norm", "query_temperature",
+                                                        "talking_heads", "value_mix")))
 
     @classmethod
     def workspace_bytes(cls, params, tokens, element_bytes):
@@ -311,6 +323,8 @@ class GQAttention(Mixer):
         q = ws.get("attention.q", (count, heads * d), ctx.dtype)
         table = ctx.block_tables[cache.group]
         style = self.position.style
+        if isinstance(cache, PagedQ4View):
+            return self._forward_q4(ctx, h, residual, cache, writes_cache, q, table)
         if self.common_form and self.qkv.takes_small(count) and style in (ops.ROPE_NONE, ops.ROPE_NEOX):
             # few tokens: one kernel for norm, q/k/v product, bias, rotation and cache write
             cos, sin = self.position.tables()
@@ -390,6 +404,34 @@ class GQAttention(Mixer):
                            page_size=cache.page_size, write_cache=writes_cache, value_dim=dv, rot_dims=self.rot_dims)
         mixed = ws.get("attention.out", (count, heads * dv), ctx.dtype)
         self._attend(ctx, q, mixed, cache, table, gate=qkv if self.gated else None)
+        return self._output(ctx, mixed, residual)
+
+    def _forward_q4(self, ctx, h, residual, cache, writes_cache, q, table):
+        """The same over pages of 4 bits: the rotation's kernel quantises what it writes."""
+        count, heads, kv_heads, d = ctx.num_tokens, self.num_heads, self.num_kv_heads, self.head_dim
+        qkv = ctx.workspace.get("attention.qkv", (count, self.qkv.out_features), torch.float32)
+        self.qkv(ctx, h, epilogue=ops.EPI_STORE, out=qkv)
+        style, cos, sin = self.position.style, None, None
+        if style is None:
+            self.position.apply(ctx, qkv[:, : heads * d].unflatten(1, (heads, d)),
+                                qkv[:, heads * d : (heads + kv_heads) * d].unflatten(1, (kv_heads, d)))
+            style = ops.ROPE_NONE
+        else:
+            cos, sin = self.position.tables()
+        ops.rope_cache_q4(qkv, q, cache.pages, num_heads=heads, num_kv_heads=kv_heads, head_dim=d,
+                          rot_dims=self.rot_dims if style != ops.ROPE_NONE else 0, positions=ctx.positions, cos=cos, sin=sin,
+                          style=style, slots=ctx.slots[cache.group] if writes_cache else None)
+        mixed = ctx.workspace.get("attention.out", (count, heads * d), ctx.dtype)
+        if ctx.host_counts:
+            longest = self._longest(np.asarray(ctx.host_counts, dtype=np.int64), np.asarray(ctx.host_pos0, dtype=np.int64))
+        else:
+            longest = ctx.extras.get("forms", {}).get("attention.longest", 0)
+        ops.attention_q4(q, mixed, cache.pages, entry_starts=ctx.entry_starts, entry_pos0=ctx.entry_pos0, positions=ctx.positions,
+                         token_entry=ctx.token_entry, block_table=table, num_heads=heads, num_kv_heads=kv_heads, head_dim=d,
+                         scale=self.scale, max_keys=max(ctx.max_kv_len, 1), all_single=ctx.all_single, any_single=ctx.any_single,
+                         workspace=ctx.workspace, window=self.window or 0, keep_first=self.keep_first, sink=self.sink,
+                         sink_values=self.sink_values, gate=qkv if self.gated else None, gate_offset=self.gate_offset,
+                         gate_per_head=self.gate_per_head, longest=longest)
         return self._output(ctx, mixed, residual)
 
     def _attend(self, ctx, q, mixed, cache, table, gate=None):

@@ -44,6 +44,8 @@ class PagedKV:
     window: Optional[int] = None  # None: all keys; w: a query at p reads p-w+1 .. p
     value_dim: Optional[int] = None  # size of a value row where it differs from a key row's
     keep_first: int = 0           # with a window: keys 0 .. keep_first-1 stay visible to every later query
+    # Whether the mixer can also work over pages of 4 bits (it is then handed a PagedQ4View where the pools are of that kind).
+    four_bit: bool = field(default=False, compare=False)
 
 
 @dataclass(frozen=True)
@@ -108,6 +110,18 @@ class PagedKVView:
         self.group = group
         self.k = k
         self.v = v
+        self.page_size = page_size
+        self.window = window
+        self.keep_first = keep_first
+
+
+class PagedQ4View:
+    """The pages of one cache slot where the cache is held in 4 bits: ``pages`` is an ``ops.Q4Pages``; the cache slots of a
+    step's tokens are ``ctx.slots[group]``."""
+
+    def __init__(self, group: int, pages, page_size: int, window: Optional[int], keep_first: int = 0):
+        self.group = group
+        self.pages = pages
         self.page_size = page_size
         self.window = window
         self.keep_first = keep_first
@@ -189,6 +203,8 @@ class StepContext:
     logits_all_rows: bool = False  # the wanted rows are all the step's tokens, in order
     pending: Optional[Any] = None  # branches that have yet to join the stream (see block.PendingJoin)
     extras: Dict[str, Any] = field(default_factory=dict)
+    # Per group of pages of 4 bits: [tokens] page * page_size + place of each token's row (-1: no page); else empty.
+    slots: List[torch.Tensor] = field(default_factory=list)
 
 
 class Part:
