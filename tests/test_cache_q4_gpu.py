@@ -256,11 +256,22 @@ def test_windows_kept_keys_and_sinks(ops, window, keep_first, sink, d):
     _attend(ops, Step([1, 1, 1], [300, 39, 0], 16, seed=window), torch.bfloat16, 8, 2, d, window=window, keep_first=keep_first, sink=sink)
 
 
+@pytest.fixture(params=["packed", "expanded"])
+def form(ops, request, monkeypatch):
+    """Which way bfloat16 portions take: over the packed pages, or over rows that are expanded first."""
+    if request.param == "expanded":
+        monkeypatch.setattr(ops, "Q4_ROWS_FIRST", 0)
+        assert not ops.attention_q4_takes_rows(torch.bfloat16, 64, 16, 2, 2, 1)
+    else:
+        assert ops.attention_q4_takes_rows(torch.bfloat16, 64, 16, 60 * 8, 8, 1)
+    return request.param
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("counts, history", [([1, 1], [70, 3]), ([20, 1, 40], [33, 64, 0])])
 @pytest.mark.parametrize("per_head", [False, True])
 @pytest.mark.parametrize("keep_first", [0, 4])
-def test_learned_sinks_and_gates(ops, dtype, counts, history, per_head, keep_first):
+def test_learned_sinks_and_gates(ops, form, dtype, counts, history, per_head, keep_first):
     heads, d = 4, 64
     rng = np.random.default_rng(8)
     gate = rng.standard_normal((sum(counts), heads * (1 if per_head else d))).astype(np.float32)
@@ -272,13 +283,23 @@ def test_learned_sinks_and_gates(ops, dtype, counts, history, per_head, keep_fir
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("heads, kv_heads, d, page_size", [(6, 2, 128, 16), (7, 1, 64, 32), (4, 2, 96, 16), (3, 3, 32, 5), (2, 1, 256, 16), (6, 2, 64, 24)])
 @pytest.mark.parametrize("counts, history, window", [([50], [0], 0), ([1, 33, 1, 2], [40, 70, 0, 15], 0), ([20, 1], [100, 64], 30)])
-def test_portions_and_mixed_steps(ops, dtype, heads, kv_heads, d, page_size, counts, history, window):
+def test_portions_and_mixed_steps(ops, form, dtype, heads, kv_heads, d, page_size, counts, history, window):
     _attend(ops, Step(counts, history, page_size, seed=d), dtype, heads, kv_heads, d, window=window)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("window, keep_first", [(1, 3), (8, 0), (33, 64), (20, 5), (500, 4), (40, 30)])
+@pytest.mark.parametrize("heads, kv_heads, d", [(3, 1, 64), (8, 2, 128)])
+def test_portions_with_windows_and_kept_keys(ops, form, dtype, window, keep_first, heads, kv_heads, d):
+    """Rows of one block see different keys: the window leaves keys behind in the middle of a portion."""
+    _attend(ops, Step([20, 1, 41], [33, 64, 0], 16), dtype, heads, kv_heads, d, window=window, keep_first=keep_first, sink=keep_first == 5)
+
+
 def test_a_long_history_in_many_splits(ops):
-    """Thousands of keys, the longest beside a short one."""
+    """Thousands of keys, the longest beside a short one, of single tokens and of portions."""
     _attend(ops, Step([1, 1], [9000, 5], 16), torch.bfloat16, 2, 1, 64)
+    for dtype in (torch.bfloat16, torch.float32):
+        _attend(ops, Step([3, 1], [5000, 5], 16), dtype, 2, 1, 64)
 
 
 def test_values_that_are_not_finite_show_where_they_are_seen(ops):
@@ -291,6 +312,16 @@ def test_values_that_are_not_finite_show_where_they_are_seen(ops):
         out = torch.zeros_like(q)
         ops.attention_q4(q, out, pages, num_heads=4, num_kv_heads=1, head_dim=64, scale=0.125, workspace=_workspace(), **step.device())
         assert out[1].isnan().all() and out[[0, 2]].isfinite().all()
+    # in a portion the tokens in front of a NaN key or value do not see it
+    for dtype in (torch.bfloat16, torch.float32):
+        for which in ("k_scales", "v_scales"):
+            step = Step([6, 3], [40, 8], 16)
+            pages = ops.Q4Pages(*plain.make_pages(step.num_pages, 16, 1, 64, 3, DEVICE))
+            getattr(pages, which)[step.tables[0][43 // 16], 0, 43 % 16] = float("nan")     # its fourth token
+            q = torch.randn(9, 4 * 64, device=DEVICE).to(dtype)
+            out = torch.zeros_like(q)
+            ops.attention_q4(q, out, pages, num_heads=4, num_kv_heads=1, head_dim=64, scale=0.125, workspace=_workspace(), **step.device())
+            assert out[3:6].isnan().all() and out[[0, 1, 2, 6, 7, 8]].isfinite().all()
     # every key of a whole split is NaN
     step = Step([1], [700], 16)
     pages = ops.Q4Pages(*plain.make_pages(step.num_pages, 16, 1, 64, 3, DEVICE))

@@ -112,6 +112,43 @@ __device__ __forceinline__ void load_words(uint32_t (&to)[WORDS], const void* fr
   }
 }
 
+// The warps' partials of one row ([warp][ROWS][D + 4] floats: outputs, maximum, sum) become the block's: 32 kWarps / ROWS threads a row,
+// `part` one of them.
+template <int D, int ROWS>
+__device__ __forceinline__ void merge_warps(const float* merge, int row, int part, float* ml, float* out) {
+  constexpr int kRow = D + 4, kColumns = D * ROWS / (32 * kWarps);
+  float m[kWarps], best = -INFINITY, total = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    m[w] = merge[(w * ROWS + row) * kRow + D];
+    best = fmaxf(best, m[w]);
+  }
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    // a warp that saw no key has sum 0; one whose scores are all NaN has no maximum either, and a sum that is NaN
+    m[w] = best == -INFINITY ? 1.0f : exp2f(m[w] - best);
+    total += merge[(w * ROWS + row) * kRow + D + 1] * m[w];
+  }
+  if (part == 0) {
+    ml[0] = best == -INFINITY && total != total ? 0.0f : best;   // the combine kernel passes over -inf
+    ml[1] = total;
+  }
+#pragma unroll
+  for (int c = 0; c < kColumns; c += 4) {
+    const int column = part * kColumns + c;
+    float4 value = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float4 v = *reinterpret_cast<const float4*>(merge + (w * ROWS + row) * kRow + column);
+      value.x += m[w] * v.x;
+      value.y += m[w] * v.y;
+      value.z += m[w] * v.z;
+      value.w += m[w] * v.w;
+    }
+    *reinterpret_cast<float4*>(out + column) = value;
+  }
+}
+
 // Two tiles of 16 keys in a warp's part of shared memory.  Row r of a tile's score accumulators is key 4 (r & 1) + (r & 7) / 2 + 8 (r / 8):
 // the keys whose weights a lane's operand of the second product holds, slots 2 t, 2 t + 1, 2 t + 8 and 2 t + 9, are then keys 4 i + t, i
 // = 0 .. 3, whose rows four lanes read without a conflict; the keys' own rows lie in the order of the accumulators.
@@ -480,40 +517,11 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) attention_q4_dec
   }
   __syncthreads();
   // and the block merges them: a few threads a head
-  constexpr int kThreadsOfHead = 32 * kWarps / (8 * NT), kColumns = D / kThreadsOfHead;
-  const int head = threadIdx.x / kThreadsOfHead, part = threadIdx.x % kThreadsOfHead;
+  constexpr int kThreadsOfHead = 32 * kWarps / (8 * NT);
+  const int head = threadIdx.x / kThreadsOfHead;
   if (head0 + head >= group) return;
-  float m[kWarps], best = -INFINITY, total = 0.0f;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    m[w] = merge[(w * 8 * NT + head) * kRow + D];
-    best = fmaxf(best, m[w]);
-  }
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    // a warp that saw no key has sum 0; one whose scores are all NaN has no maximum either, and a sum that is NaN
-    m[w] = best == -INFINITY ? 1.0f : exp2f(m[w] - best);
-    total += merge[(w * 8 * NT + head) * kRow + D + 1] * m[w];
-  }
   const size_t at = (static_cast<size_t>(entry) * p.num_heads + kv_head * group + head0 + head) * places + split;
-  if (part == 0) {
-    p.partial_ml[2 * at] = best == -INFINITY && total != total ? 0.0f : best;   // the combine kernel passes over -inf
-    p.partial_ml[2 * at + 1] = total;
-  }
-#pragma unroll
-  for (int c = 0; c < kColumns; c += 4) {
-    const int column = part * kColumns + c;
-    float4 value = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const float4 v = *reinterpret_cast<const float4*>(merge + (w * 8 * NT + head) * kRow + column);
-      value.x += m[w] * v.x;
-      value.y += m[w] * v.y;
-      value.z += m[w] * v.z;
-      value.w += m[w] * v.w;
-    }
-    *reinterpret_cast<float4*>(p.partial_out + at * D + column) = value;
-  }
+  merge_warps<D, 8 * NT>(merge, head, threadIdx.x % kThreadsOfHead, p.partial_ml + 2 * at, p.partial_out + at * D);
 }
 
 template <int D, int NT>
@@ -533,6 +541,12 @@ int launch(const DecodeParams& p, cudaStream_t s) {
                        D, 0, s, p.partial_ml, p.partial_out, p.num_splits, p.out, p.num_heads, p.positions, p.window, p.chunk,
                        p.entry_starts, p.keep_first, p.sink, p.sink_values, p.gate, p.gate_stride, p.gate_per_head);
 }
+
+}  // namespace
+
+#include "attention_q4_rows.cuh"
+
+namespace {
 
 bool on_16_bytes(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
@@ -566,4 +580,39 @@ VIPERA_API int vipera_attention_q4_decode(const DecodeParams* given, float* scra
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (p.head_dim == 128) return wide ? launch<128, 2>(p, s) : launch<128, 1>(p, s);
   return wide ? launch<64, 2>(p, s) : launch<64, 1>(p, s);
+}
+
+VIPERA_API int vipera_attention_q4_rows_params_size() { return static_cast<int>(sizeof(RowsParams)); }
+
+// Attention of every token of a step, q of `dtype` and out too: partials per (token, head, place) in `scratch`, then the endings that
+// the combine kernel knows (`positions` [tokens]; sink, sink_values and gate as for the kernel of single tokens).
+VIPERA_API int vipera_attention_q4_rows(const RowsParams* given, void* out, int dtype, int head_dim, const int* positions, int sink,
+                                        const float* sink_values, const float* gate, long long gate_stride, int gate_per_head,
+                                        float* scratch, size_t scratch_floats, void* stream) {
+  RowsParams p = *given;
+  if (p.num_entries <= 0 || p.num_tokens <= 0) return VIPERA_OK;
+  if (p.num_heads <= 0 || p.num_kv_heads <= 0 || p.num_heads % p.num_kv_heads || p.keep_first < 0 || p.page_size <= 0 ||
+      p.page_size % 16 || p.num_heads > 65535 || p.num_splits <= 0 || p.num_splits > 128 || p.chunk <= 0 || p.chunk % 64 ||
+      (head_dim != 64 && head_dim != 128))
+    return VIPERA_BAD_SHAPE;
+  if (p.window <= 0) p.keep_first = 0;
+  if (sink_values) sink = 1;
+  const size_t rows = static_cast<size_t>(p.num_tokens) * p.num_heads * (p.num_splits + (p.keep_first > 0 ? 1 : 0));
+  const size_t pairs = (2 * rows + 3) / 4 * 4;
+  if (!scratch || scratch_floats < pairs + rows * head_dim || !on_16_bytes(scratch) || !on_16_bytes(p.k_codes) ||
+      !on_16_bytes(p.v_codes) || !on_16_bytes(p.k_scales) || !on_16_bytes(p.v_scales))
+    return VIPERA_BAD_ARGUMENT;
+  p.partial_ml = scratch;
+  p.partial_out = scratch + pairs;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  int status = VIPERA_BAD_DTYPE;
+  const bool wide = dtype == VIPERA_F32;
+  if (wide) status = head_dim == 128 ? launch_rows<128, float, 1>(p, s) : launch_rows<64, float, 2>(p, s);
+  else if (dtype == VIPERA_BF16) status = head_dim == 128 ? launch_rows<128, __nv_bfloat16, 2>(p, s) : launch_rows<64, __nv_bfloat16, 2>(p, s);
+  if (status != VIPERA_OK) return status;
+  const auto combine = head_dim == 128 ? (wide ? attention_combine_kernel<128, true, true> : attention_combine_kernel<128, true, false>)
+                                       : (wide ? attention_combine_kernel<64, true, true> : attention_combine_kernel<64, true, false>);
+  return vipera_launch(combine, dim3(p.num_tokens, p.num_heads), head_dim, 0, s, p.partial_ml, p.partial_out, p.num_splits,
+                       static_cast<__nv_bfloat16*>(out), p.num_heads, positions, p.window, p.chunk, static_cast<const int*>(nullptr),
+                       p.keep_first, sink, sink_values, gate, gate_stride, gate_per_head);
 }

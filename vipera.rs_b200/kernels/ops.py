@@ -1094,6 +1094,14 @@ class _DecodeQ4Params(ctypes.Structure):
                 ("sink", _c_int), ("chunk", _c_int), ("num_splits", _c_int), ("magic", ctypes.c_uint)]
 
 
+class _RowsQ4Params(ctypes.Structure):
+    _fields_ = [("q", _c_void), ("k_codes", _c_void), ("v_codes", _c_void), ("k_scales", _c_void), ("v_scales", _c_void),
+                ("entry_starts", _c_void), ("entry_pos0", _c_void), ("block_table", _c_void), ("partial_ml", _c_void),
+                ("partial_out", _c_void), ("table_width", _c_int), ("page_size", _c_int), ("num_pages", _c_int), ("num_entries", _c_int),
+                ("num_tokens", _c_int), ("num_heads", _c_int), ("num_kv_heads", _c_int), ("scale", _c_float), ("window", _c_int),
+                ("keep_first", _c_int), ("chunk", _c_int), ("num_splits", _c_int)]
+
+
 def _place(what: str, tensor: torch.Tensor, dtype: torch.dtype, here: int) -> int:
     """The address of a contiguous tensor of `dtype` on device `here`, the current one, whose stream the launch goes to."""
     if tensor.dtype is not dtype or not tensor.is_contiguous() or tensor.get_device() != here:
@@ -1285,6 +1293,57 @@ def _attention_q4_decode(q, out, pages, *, positions, block_table, num_heads, nu
     _check(fn(p, scratch.data_ptr(), scratch.numel(), _stream_of(here)), "attention_decode", kernels=2)
 
 
+Q4_ROWS = {(torch.float32, 128): 8, (torch.float32, 64): 16, (torch.bfloat16, 128): 16, (torch.bfloat16, 64): 16}   # (token, head) rows of a block
+
+
+# bfloat16 portions of few (token, head) rows read the packed pages; more of them pay for rows that are expanded once and read by the
+# flash kernel, whose blocks of 128 tokens and a head walk a whole history each.  Fitted to both forms timed at 28, 12 and 14 heads (the
+# latter of 64), 1 and 8 requests, 2 to 256 tokens each behind 0 to 20,000: one request of 64 tokens and 28 heads behind 4,000
+# keys takes 66 and 86 microseconds, of 128 tokens 115 and 63; eight of 16 behind 4,000 keys 121 and 199, of 64 342 and 199.
+Q4_ROWS_FIRST, Q4_ROWS_MORE, Q4_ROWS_HALF = 1800, 15, 1.4
+
+
+def attention_q4_takes_rows(dtype: torch.dtype, head_dim: int, page_size: int, rows: int, heads: int, portions: int) -> bool:
+    """Whether a step of `rows` (token, head) rows, portions of `portions` requests, reads the packed pages: 32-bit steps always do (where
+    the heads and pages are those the kernel is built for), bfloat16 ones with few rows."""
+    if head_dim not in MMA_HEAD_DIMS or page_size % 16:
+        return False
+    most = (Q4_ROWS_FIRST + Q4_ROWS_MORE * heads * (portions - 1)) * (Q4_ROWS_HALF if head_dim == 64 else 1.0)
+    return dtype == torch.float32 or (Q4_ROWS_FIRST > 0 and rows <= most)
+
+
+@functools.lru_cache(maxsize=4096)
+def q4_rows_splits(tiles: int, max_keys: int, sm_count: int):
+    """How the kernel of any number of tokens cuts its keys, `tiles` blocks' worth of rows there: four blocks an SM where the keys
+    give that many cuts of 64 keys."""
+    wanted = max(1, min(64, 4 * sm_count // tiles))
+    chunk = 64 * max(1, -(-max_keys // (64 * wanted)))
+    return chunk, -(-max_keys // chunk)
+
+
+def _attention_q4_rows(q, out, pages, *, entry_starts, entry_pos0, positions, block_table, num_heads, num_kv_heads, head_dim, scale,
+                       max_keys, workspace, window, keep_first, sink, sink_values, gate, gate_offset, gate_per_head) -> None:
+    fn = _function("attention_q4", "vipera_attention_q4_rows",
+                   [ctypes.POINTER(_RowsQ4Params), _c_void, _c_int, _c_int, _c_void, _c_int, _c_void, _c_void, ctypes.c_longlong, _c_int,
+                    _c_void, ctypes.c_size_t, _c_void])
+    _check_struct("attention_q4", "vipera_attention_q4_rows_params_size", _RowsQ4Params)
+    here, int32, what = torch.cuda.current_device(), torch.int32, "attention_q4"
+    count, entries, dtype = q.shape[0], entry_pos0.numel(), q.dtype
+    rows = Q4_ROWS[dtype, head_dim]
+    chunk, splits = q4_rows_splits(num_kv_heads * -(-count * (num_heads // num_kv_heads) // rows), max_keys, _sm_count_of(here))
+    scratch = workspace.get("attention.partials", (attention_decode_scratch_floats(
+        count, num_heads, head_dim, splits + (1 if keep_first else 0)),), torch.float32)
+    gate_pointer, gate_stride = (None, 0) if gate is None else _gate_pointer(
+        gate, gate_offset, count, num_heads * (1 if gate_per_head else head_dim), what)
+    p = _RowsQ4Params(_place(what, q, dtype, here), *_place_pages(what, pages, here), _place(what, entry_starts, int32, here),
+                      _place(what, entry_pos0, int32, here), _place(what, block_table, int32, here), None, None, block_table.shape[1],
+                      pages.k_codes.shape[2], pages.k_codes.shape[0], entries, count, num_heads, num_kv_heads, scale, window, keep_first,
+                      chunk, splits)
+    _check(fn(p, _place(what, out, dtype, here), dtype_code(dtype), head_dim, _place(what, positions, int32, here), 1 if sink else 0,
+              None if sink_values is None else _place(what, sink_values, torch.float32, here), gate_pointer, gate_stride,
+              1 if gate_per_head else 0, scratch.data_ptr(), scratch.numel(), _stream_of(here)), "attention", kernels=2)
+
+
 def attention_q4(q: torch.Tensor, out: torch.Tensor, pages: Q4Pages, *, entry_starts: torch.Tensor, entry_pos0: torch.Tensor,
                  positions: torch.Tensor, token_entry: torch.Tensor, block_table: torch.Tensor, num_heads: int, num_kv_heads: int,
                  head_dim: int, scale: float, max_keys: int, all_single: bool, any_single: bool, workspace, window: int = 0,
@@ -1296,9 +1355,9 @@ def attention_q4(q: torch.Tensor, out: torch.Tensor, pages: Q4Pages, *, entry_st
     for ``attention``, ``longest`` too.  ``workspace.get(name, shape, dtype)`` gives rooms that the call may use until it is
     done on its stream.
 
-    Single tokens of bfloat16 steps with heads of 64 or 128 values and pages of a multiple of 16 tokens are attended over the packed
-    pages.  Elsewhere the rows that the step sees are expanded to the run's type first (a room as large as one layer's
-    pages in that type) and the kernels for such pages attend."""
+    With heads of 64 or 128 values and pages of a multiple of 16 tokens, single tokens, short portions and all of a 32-bit step are
+    attended over the packed pages.  Elsewhere the rows that the step sees are expanded to the run's type first (a room as large as one
+    layer's pages in that type) and the kernels for such pages attend."""
     page_size = _check_q4_pages("attention_q4", pages, num_kv_heads, head_dim)
     count, entries = q.shape[0], entry_pos0.numel()
     if num_kv_heads <= 0 or num_heads % num_kv_heads or tuple(q.shape) != (count, num_heads * head_dim) or out.shape != q.shape \
@@ -1325,6 +1384,10 @@ def attention_q4(q: torch.Tensor, out: torch.Tensor, pages: Q4Pages, *, entry_st
     if packed and all_single:
         _attention_q4_decode(q, out, pages, positions=positions, block_table=block_table, max_keys=max_keys, workspace=workspace,
                              entry_starts=None, **heads, **endings)
+        return
+    if attention_q4_takes_rows(q.dtype, head_dim, page_size, count * num_heads, num_heads, 1 if any_single else entries):
+        _attention_q4_rows(q, out, pages, entry_starts=entry_starts, entry_pos0=entry_pos0, positions=positions, block_table=block_table,
+                           max_keys=max_keys, workspace=workspace, **heads, **endings)
         return
     # what the flash kernels know of endings decides whether portions are theirs (see parts/attention.py)
     extended = sink_values is not None or gate is not None
