@@ -176,16 +176,16 @@ def test_attention_says_which_options_packed_pages_serve(option):
     assert not GQAttention.cache_request_for(dict(plain_params, **option)).four_bit
 
 
-def test_the_cut_of_the_keys_covers_them_in_whole_walks():
+def test_keys_are_shared_by_a_clusters_blocks_and_cut_into_whole_walks():
     import vipera_rs_b200  # noqa: F401
     from vipera_rs_b200.kernels import ops
 
-    for entries in (1, 3, 64, 300):
-        for tiles in (1, 8, 40):
-            for keys in (1, 128, 129, 2049, 40000, 10**6):
-                for window in (0, 1, 1024):
-                    chunk, splits = ops.q4_splits(entries, tiles, keys, window, 148)
-                    assert chunk % 128 == 0 and 0 < splits <= 128 and chunk * (splits - 1) < keys <= chunk * splits
+    for tiles in (1, 3, 8, 64, 300, 12000):
+        for keys in (1, 128, 129, 2049, 40000, 10**6):
+            shares = ops.q4_shares(tiles, 1, keys, 148)
+            assert shares in (1, 2, 4, 8, 16) and (shares == 1 or keys > 64 * shares)    # no more than there are walks for, but for one
+            chunk, splits = ops.q4_rows_splits(tiles, keys, 148)
+            assert chunk % 64 == 0 and 0 < splits <= 64 and chunk * (splits - 1) < keys <= chunk * splits
 
 
 def test_page_lists_are_the_requests_pages_one_behind_the_other():

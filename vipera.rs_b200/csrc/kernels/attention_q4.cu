@@ -1,7 +1,9 @@
 // Attention of single tokens over pages of 4 bits (formats: q4.cuh), split over the keys, on mma.sync m16n8k16.
 //
-// A block is (entry, KV head and up to 8 NT of its query heads, split of the keys); its four warps fold 32 keys at a time each with a
-// running (max, sum, output) and merge at the end; attention_combine_kernel joins the splits.
+// A block is (entry, KV head and up to 8 NT of its query heads, share of the visible keys); its four warps fold 32 keys at a time each
+// with a running (max, sum, output) and merge at the end.  The blocks of an (entry, KV head) are a cluster that joins its shares
+// through distributed shared memory and writes the output: one launch, nothing passes through memory, and shares are cut
+// from the entry's own keys, so that blocks of one cluster carry equal loads.
 //
 // Both products put the packed operand on the side of 16 (keys for the scores, channels for the values) and the query
 // heads on the side of 8: a group of 8 heads or fewer costs half of the products that the other way round would
@@ -37,13 +39,11 @@ struct DecodeParams {
   const int* entry_starts;        // null: token i is entry i
   const float* sink_values;
   const float* gate;
-  float* partial_ml;
-  float* partial_out;
   long long gate_stride;
   int gate_per_head;
   int table_width, page_size, page_shift, num_pages, num_entries, num_heads, num_kv_heads, head_dim;
   float scale;
-  int window, keep_first, sink, chunk, num_splits;
+  int window, keep_first, sink, shares;
   uint32_t magic;                 // set by the launcher
 };
 
@@ -94,6 +94,24 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], 
 __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// a float, and four of them, at `local` (a shared-memory address of this block) in the block of rank `rank`
+__device__ __forceinline__ float cluster_load(uint32_t local, uint32_t rank) {
+  uint32_t remote;
+  float value;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(value) : "r"(remote) : "memory");
+  return value;
+}
+__device__ __forceinline__ float4 cluster_load_4(uint32_t local, uint32_t rank) {
+  uint32_t remote;
+  float4 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(remote) : "memory");
+  return v;
 }
 __device__ __forceinline__ void cp_async_all(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -170,36 +188,37 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) attention_q4_dec
   // only now: the kernel behind reads the positions before its own wait, and they may come from the kernel ahead
   pdl_launch_dependents();
   const int group = p.num_heads / p.num_kv_heads, head_tiles = (group + 8 * NT - 1) / (8 * NT);
-  const int entry = blockIdx.x, split = blockIdx.z;
+  const int entry = blockIdx.x, share = blockIdx.z;
   const int kv_head = blockIdx.y / head_tiles, head0 = (blockIdx.y - kv_head * head_tiles) * 8 * NT;
   int token = entry;
   if (p.entry_starts) {
     token = p.entry_starts[entry];
-    if (p.entry_starts[entry + 1] - token != 1) return;
+    if (p.entry_starts[entry + 1] - token != 1) return;   // the whole cluster's
   }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int position = p.positions[entry];
   const int* table = p.block_table + static_cast<size_t>(entry) * p.table_width;
-  const int window_first = first_visible_key(position, p.window);
-  const bool kept_split = split == p.num_splits;   // the kept first keys that the window has left behind
-  const int places = p.num_splits + (p.keep_first > 0 ? 1 : 0);
-  const int first = kept_split ? 0 : window_first;
-  const int last = kept_split ? min(p.keep_first, window_first) - 1 : position;
-  const int begin = kept_split ? 0 : max(split * p.chunk, first / 32 * 32);
-  const int end = kept_split ? last + 1 : min((split + 1) * p.chunk, position + 1);
-  if (begin >= end) return;   // a split without visible keys: the combine kernel skips it too
+  // The visible keys in tiles of 16: those of the kept first keys that the window has left behind, then those of the window.
+  const int first = first_visible_key(position, p.window), kept = p.window > 0 ? min(p.keep_first, first) : 0;
+  const int kept_tiles = (kept + 15) >> 4, first_tile = first >> 4;
+  const int tiles = kept_tiles + max((position >> 4) - first_tile + 1, 0);
+  const int each = (tiles + 8 * p.shares - 1) / (8 * p.shares) * 8;      // of a block: whole steps of its warps
+  const int tiles_end = min((share + 1) * each, tiles);
+  const auto key_of = [&](int tile) { return 16 * (tile < kept_tiles ? tile : tile - kept_tiles + first_tile); };
+  const auto low_key = [&](int tile) { return tile < kept_tiles ? 0 : first; };
+  const auto high_key = [&](int tile) { return tile < kept_tiles ? kept - 1 : position; };
 
   // --- the way of the rows into shared memory: 16 bytes a lane, kStages - 1 pairs of tiles ahead ---
   Stage<D>* stages = reinterpret_cast<Stage<D>*>(shared) + warp * kStages;
-  const int warp_begin = begin + warp * kWarpKeys;
-  const int steps = warp_begin < end ? (end - warp_begin + kWarps * kWarpKeys - 1) / (kWarps * kWarpKeys) : 0;
-  // the page of the tile that is this lane's among 32: tile i of step j is key warp_begin + 128 j + 16 i; a tile
-  // without a visible key, and one whose page is not held, has none and is filled with zeros
-  const auto page_of = [&](int tile) {
-    const int key = warp_begin + (tile >> 1) * (kWarps * kWarpKeys) + (tile & 1) * 16;
-    if (key >= end || key > last || key + 15 < first) return -1;
-    const int index = p.page_shift >= 0 ? key >> p.page_shift : key / p.page_size;
-    const int page = index < p.table_width ? table[index] : -1;
+  const int warp_tile = share * each + 2 * warp;     // step j has tiles warp_tile + 8 j and the next
+  const int steps = warp_tile < tiles_end ? (tiles_end - warp_tile + 7) >> 3 : 0;
+  // the page of the tile that is this lane's among 32 of the warp's; a tile that is not the block's, and one whose page is not held, has
+  // none and is filled with zeros
+  const auto page_of = [&](int index) {
+    const int tile = warp_tile + (index >> 1) * 8 + (index & 1);
+    if (tile >= tiles_end) return -1;
+    const int key = key_of(tile), place = p.page_shift >= 0 ? key >> p.page_shift : key / p.page_size;
+    const int page = place < p.table_width ? table[place] : -1;
     return page < p.num_pages ? page : -1;
   };
   int pages_now = page_of(lane), pages_next = steps > 16 ? page_of(32 + lane) : -1;
@@ -232,7 +251,7 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) attention_q4_dec
       if (!one_tile_a_page) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const int key = warp_begin + j * (kWarps * kWarpKeys) + 16 * i;
+          const int key = key_of(warp_tile + 8 * j + i);
           place[i] = p.page_shift >= 0 ? key & (p.page_size - 1) : key % p.page_size;
         }
       }
@@ -344,7 +363,7 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) attention_q4_dec
     cp_async_wait<kStages - 1>();
     __syncwarp();
     const Stage<D>& from = stages[j % kStages];
-    const int key0 = warp_begin + j * (kWarps * kWarpKeys);
+    const int tile0 = warp_tile + 8 * j;
     float s[2][NT][4];        // rows g (0, 1) and g + 8 (2, 3), heads 2 t and 2 t + 1; in units of log2
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -377,14 +396,16 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) attention_q4_dec
 #pragma unroll
         for (int c = 0; c < 4; ++c) s[i][nt][c] *= q_factor[nt][c & 1];
     }
-    const bool whole = key0 >= first && key0 + kWarpKeys - 1 <= last;
+    // every step but those with a border: all 32 keys are seen
+    const int key0 = key_of(tile0);
+    const bool whole = tile0 >= kept_tiles && key0 >= first && key0 + kWarpKeys - 1 <= position && tile0 + 1 < tiles_end;
     if (!whole) {
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const int key = key0 + 16 * i + 8 * r + row_key;
-          if (key < first || key > last) {
+          const int key = key_of(tile0 + i) + 8 * r + row_key;
+          if (tile0 + i >= tiles_end || key < low_key(tile0 + i) || key > high_key(tile0 + i)) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) s[i][nt][2 * r] = s[i][nt][2 * r + 1] = -INFINITY;
           }
@@ -437,8 +458,8 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) attention_q4_dec
       if (!whole) {   // a hidden key's weight is 0, and its scale must not make that NaN
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
-          const int key = key0 + 16 * i + 4 * n + t;
-          if (key < first || key > last) {
+          const int key = key_of(tile0 + i) + 4 * n + t;
+          if (tile0 + i >= tiles_end || key < low_key(tile0 + i) || key > high_key(tile0 + i)) {
 #pragma unroll
             for (int w = 0; w < G / 2; ++w) scale[n][w] = 0;
           }
@@ -516,30 +537,71 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) attention_q4_dec
     }
   }
   __syncthreads();
-  // and the block merges them: a few threads a head
-  constexpr int kThreadsOfHead = 32 * kWarps / (8 * NT);
-  const int head = threadIdx.x / kThreadsOfHead;
-  if (head0 + head >= group) return;
-  const size_t at = (static_cast<size_t>(entry) * p.num_heads + kv_head * group + head0 + head) * places + split;
-  merge_warps<D, 8 * NT>(merge, head, threadIdx.x % kThreadsOfHead, p.partial_ml + 2 * at, p.partial_out + at * D);
+  // the block merges them, a few threads a head
+  float* joined = merge + kWarps * 8 * NT * kRow;     // [8 NT heads][kRow]
+  {
+    constexpr int kThreadsOfHead = 32 * kWarps / (8 * NT);
+    const int head = threadIdx.x / kThreadsOfHead;
+    merge_warps<D, 8 * NT>(merge, head, threadIdx.x % kThreadsOfHead, joined + head * kRow + D, joined + head * kRow);
+  }
+  // and the cluster its blocks: every thread has four channels of a head at a time
+  cluster_sync_all();
+  const int heads_here = min(8 * NT, group - head0);
+  const uint32_t joined_at = smem_addr(joined);
+  for (int i = share * static_cast<int>(blockDim.x) + threadIdx.x; i < heads_here * (D / 4); i += p.shares * blockDim.x) {
+    const int h = i / (D / 4), column = (i - h * (D / 4)) * 4, head = kv_head * group + head0 + h;
+    float best = -INFINITY, total = 0.0f;
+    for (int c = 0; c < p.shares; ++c) best = fmaxf(best, cluster_load(joined_at + (h * kRow + D) * 4, c));
+    float4 value = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+    for (int c = 0; c < p.shares; ++c) {
+      const float m = cluster_load(joined_at + (h * kRow + D) * 4, c), l = cluster_load(joined_at + (h * kRow + D + 1) * 4, c);
+      const float4 v = cluster_load_4(joined_at + (h * kRow + column) * 4, c);
+      const float w = m == -INFINITY ? 0.0f : exp2f(m - best);    // a share without visible keys
+      total += l * w;
+      value.x += v.x * w;
+      value.y += v.y * w;
+      value.z += v.z * w;
+      value.w += v.w * w;
+    }
+    if (p.sink) total += exp2f((p.sink_values ? p.sink_values[head] * kLog2e : 0.0f) - best);
+    float out[4] = {value.x / total, value.y / total, value.z / total, value.w / total};
+    if (p.gate) {
+      const float* gate = p.gate + static_cast<size_t>(token) * p.gate_stride + (p.gate_per_head ? head : head * D + column);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) out[c] *= 1.0f / (1.0f + expf(-gate[p.gate_per_head ? 0 : c]));
+    }
+    store_four_as<__nv_bfloat16>(p.out + (static_cast<size_t>(token) * p.num_heads + head) * D + column, out[0], out[1], out[2], out[3]);
+  }
+  cluster_sync_all();   // nobody's shared memory goes while others read it
 }
 
 template <int D, int NT>
 int launch(const DecodeParams& p, cudaStream_t s) {
   constexpr int kSmem = kWarps * kStages * static_cast<int>(sizeof(Stage<D>));
-  static_assert(kWarps * 8 * NT * (D + 4) * 4 <= kSmem, "the warps' partials fit in their stages");
-  if (kSmem > 48 * 1024) {   // every device has to be asked
-    cudaError_t error = cudaFuncSetAttribute(attention_q4_decode_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
-    if (error != cudaSuccess) return static_cast<int>(error);
-  }
+  static_assert((kWarps + 1) * 8 * NT * (D + 4) * 4 <= kSmem, "the partials fit in the stages");
+  const auto kernel = attention_q4_decode_kernel<D, NT>;
+  cudaError_t error = cudaSuccess;      // every device has to be asked
+  if (kSmem > 48 * 1024) error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  if (error == cudaSuccess && p.shares > 8) error = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (error != cudaSuccess) return static_cast<int>(error);
   const int group = p.num_heads / p.num_kv_heads, head_tiles = (group + 8 * NT - 1) / (8 * NT);
-  const dim3 grid(p.num_entries, p.num_kv_heads * head_tiles, p.num_splits + (p.keep_first > 0 ? 1 : 0));
-  int status = vipera_launch(attention_q4_decode_kernel<D, NT>, grid, 32 * kWarps, kSmem, s, p);
-  if (status != VIPERA_OK) return status;
-  const bool ending = p.keep_first > 0 || p.sink || p.gate;
-  return vipera_launch(ending ? attention_combine_kernel<D, true> : attention_combine_kernel<D>, dim3(p.num_entries, p.num_heads),
-                       D, 0, s, p.partial_ml, p.partial_out, p.num_splits, p.out, p.num_heads, p.positions, p.window, p.chunk,
-                       p.entry_starts, p.keep_first, p.sink, p.sink_values, p.gate, p.gate_stride, p.gate_per_head);
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(p.num_entries, p.num_kv_heads * head_tiles, p.shares);
+  config.blockDim = dim3(32 * kWarps);
+  config.dynamicSmemBytes = kSmem;
+  config.stream = s;
+  cudaLaunchAttribute attributes[2];
+  attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attributes[0].val.programmaticStreamSerializationAllowed = vipera_pdl_enabled() ? 1 : 0;
+  attributes[1].id = cudaLaunchAttributeClusterDimension;
+  attributes[1].val.clusterDim.x = 1;
+  attributes[1].val.clusterDim.y = 1;
+  attributes[1].val.clusterDim.z = static_cast<unsigned>(p.shares);
+  config.attrs = attributes;
+  config.numAttrs = 2;
+  error = cudaLaunchKernelEx(&config, kernel, p);
+  return error == cudaSuccess ? VIPERA_OK : static_cast<int>(error);
 }
 
 }  // namespace
@@ -554,24 +616,19 @@ bool on_16_bytes(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) =
 
 VIPERA_API int vipera_attention_q4_params_size() { return static_cast<int>(sizeof(DecodeParams)); }
 
-// Attention of the entries that bring one token (all of them where entry_starts is null).  `scratch` holds the splits'
-// partials, (2 + d) floats per (entry, head, place); p->partial_ml and p->partial_out are set here.
-VIPERA_API int vipera_attention_q4_decode(const DecodeParams* given, float* scratch, size_t scratch_floats, void* stream) {
+// Attention of the entries that bring one token (all of them where entry_starts is null); p->shares blocks, a power of two up to
+// 16, share an entry's keys.
+VIPERA_API int vipera_attention_q4_decode(const DecodeParams* given, void* stream) {
   DecodeParams p = *given;
   if (p.num_entries <= 0) return VIPERA_OK;
   if (p.num_heads <= 0 || p.num_kv_heads <= 0 || p.num_heads % p.num_kv_heads || p.keep_first < 0 || p.page_size <= 0 ||
-      p.page_size % 16 || p.num_heads > 65535 || p.num_splits <= 0 || p.num_splits > 128 || p.chunk <= 0 ||
-      p.chunk % (kWarps * kWarpKeys) || (p.head_dim != 64 && p.head_dim != 128))
+      p.page_size % 16 || p.num_heads > 65535 || p.shares <= 0 || p.shares > 16 || (p.shares & (p.shares - 1)) ||
+      (p.head_dim != 64 && p.head_dim != 128))
     return VIPERA_BAD_SHAPE;
-  if (p.window <= 0) p.keep_first = 0;
   if (p.sink_values) p.sink = 1;
-  const size_t rows = static_cast<size_t>(p.num_entries) * p.num_heads * (p.num_splits + (p.keep_first > 0 ? 1 : 0));
-  const size_t pairs = (2 * rows + 3) / 4 * 4;
-  if (!scratch || scratch_floats < pairs + rows * p.head_dim || !on_16_bytes(scratch) || !on_16_bytes(p.q) || !on_16_bytes(p.k_codes) ||
-      !on_16_bytes(p.v_codes) || !on_16_bytes(p.k_scales) || !on_16_bytes(p.v_scales))
+  if (!on_16_bytes(p.q) || !on_16_bytes(p.k_codes) || !on_16_bytes(p.v_codes) || !on_16_bytes(p.k_scales) || !on_16_bytes(p.v_scales) ||
+      (reinterpret_cast<uintptr_t>(p.out) & 7))
     return VIPERA_BAD_ARGUMENT;
-  p.partial_ml = scratch;
-  p.partial_out = scratch + pairs;
   p.magic = 0x43004300u;
   p.page_shift = -1;
   if ((p.page_size & (p.page_size - 1)) == 0)

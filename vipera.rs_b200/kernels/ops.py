@@ -1087,11 +1087,10 @@ class _ExpandQ4Params(ctypes.Structure):
 class _DecodeQ4Params(ctypes.Structure):
     _fields_ = [("q", _c_void), ("out", _c_void), ("k_codes", _c_void), ("v_codes", _c_void), ("k_scales", _c_void),
                 ("v_scales", _c_void), ("positions", _c_void), ("block_table", _c_void), ("entry_starts", _c_void),
-                ("sink_values", _c_void), ("gate", _c_void), ("partial_ml", _c_void), ("partial_out", _c_void),
-                ("gate_stride", ctypes.c_longlong), ("gate_per_head", _c_int), ("table_width", _c_int), ("page_size", _c_int),
-                ("page_shift", _c_int), ("num_pages", _c_int), ("num_entries", _c_int), ("num_heads", _c_int),
+                ("sink_values", _c_void), ("gate", _c_void), ("gate_stride", ctypes.c_longlong), ("gate_per_head", _c_int),
+                ("table_width", _c_int), ("page_size", _c_int), ("page_shift", _c_int), ("num_pages", _c_int), ("num_entries", _c_int), ("num_heads", _c_int),
                 ("num_kv_heads", _c_int), ("head_dim", _c_int), ("scale", _c_float), ("window", _c_int), ("keep_first", _c_int),
-                ("sink", _c_int), ("chunk", _c_int), ("num_splits", _c_int), ("magic", ctypes.c_uint)]
+                ("sink", _c_int), ("shares", _c_int), ("magic", ctypes.c_uint)]
 
 
 class _RowsQ4Params(ctypes.Structure):
@@ -1246,51 +1245,45 @@ def attention_q4_takes_decode(dtype: torch.dtype, head_dim: int, page_size: int)
 # The packed kernel's blocks: three an SM at once, and a walk's time in microseconds: what a block costs beside its keys, and what each 128
 # of them cost where one, two or three blocks share an SM (fitted to launches at batch 1 to 64 and 2,048 to 32,768 keys).
 Q4_BLOCKS_PER_SM = 3
-Q4_BLOCK_FIXED, Q4_BLOCK_KEYS, Q4_SPLIT_JOIN = 2.2, (0.0, 0.8, 1.25, 1.75), 0.05
+Q4_BLOCK_FIXED, Q4_BLOCK_KEYS = 2.2, (0.0, 0.8, 1.25, 1.75)
 
 
 @functools.lru_cache(maxsize=4096)
-def q4_splits(num_entries: int, num_head_tiles: int, max_keys: int, window: int, sm_count: int):
-    """How a step of single tokens over packed pages cuts its keys: (keys per split, splits), the cut that a model of the
-    launch's time likes best: whole waves of blocks, then what is left, for keys as many as a query sees."""
-    base, slots = num_entries * num_head_tiles, Q4_BLOCKS_PER_SM * sm_count
-    seen = min(max_keys, window + 127) if window else max_keys
-    best = None
-    for wanted in range(1, 65):
-        units = max(-(-seen // (128 * wanted)), -(-max_keys // (128 * 128)))     # at most 128 splits
-        if best is not None and units == best[1]:
-            continue
-        splits, total = -(-max_keys // (128 * units)), -(-seen // (128 * units))
-        full, rest = divmod(base * total, slots)
-        time = full * (Q4_BLOCK_FIXED + units * Q4_BLOCK_KEYS[3]) + Q4_SPLIT_JOIN * total
+def q4_shares(num_entries: int, num_head_tiles: int, seen: int, sm_count: int) -> int:
+    """How many blocks share an entry's keys in a step of single tokens over packed pages, `seen` of them at most: the power of two up to
+    16 (a cluster's blocks) that a model of the launch's time likes best, whole waves of blocks and then what is left."""
+    base, slots, best = num_entries * num_head_tiles, Q4_BLOCKS_PER_SM * sm_count, None
+    for shares in (1, 2, 4, 8, 16):
+        units = -(-seen // (128 * shares))
+        full, rest = divmod(base * shares, slots)
+        time = full * (Q4_BLOCK_FIXED + units * Q4_BLOCK_KEYS[3])
         if rest:
             time += Q4_BLOCK_FIXED + units * Q4_BLOCK_KEYS[-(-rest // sm_count)]
         if best is None or time < best[0] - 1e-9:
-            best = (time, units, splits)
-    return 128 * best[1], best[2]
+            best = (time, shares)
+    return best[1]
 
 
-def _attention_q4_decode(q, out, pages, *, positions, block_table, num_heads, num_kv_heads, head_dim, scale, max_keys, workspace,
-                         entry_starts, window, keep_first, sink, sink_values, gate, gate_offset, gate_per_head) -> None:
+def _attention_q4_decode(q, out, pages, *, positions, block_table, num_heads, num_kv_heads, head_dim, scale, max_keys, entry_starts,
+                         window, keep_first, sink, sink_values, gate, gate_offset, gate_per_head) -> None:
     fn = _function("attention_q4", "vipera_attention_q4_decode",
-                   [ctypes.POINTER(_DecodeQ4Params), _c_void, ctypes.c_size_t, _c_void])
+                   [ctypes.POINTER(_DecodeQ4Params), _c_void])
     _check_struct("attention_q4", "vipera_attention_q4_params_size", _DecodeQ4Params)
     entries = block_table.shape[0]
     here, int32, what = torch.cuda.current_device(), torch.int32, "attention_q4"
     width = block_table.shape[1]
     group = num_heads // num_kv_heads
-    chunk, splits = q4_splits(entries, num_kv_heads * -(-group // (8 if group <= 8 else 16)), max_keys, window, _sm_count_of(here))
-    scratch = workspace.get("attention.partials", (attention_decode_scratch_floats(
-        entries, num_heads, head_dim, splits + (1 if keep_first else 0)),), torch.float32)
+    shares = q4_shares(entries, num_kv_heads * -(-group // (8 if group <= 8 else 16)),
+                       min(max_keys, window + keep_first) if window else max_keys, _sm_count_of(here))
     gate_pointer, gate_stride = (None, 0) if gate is None else _gate_pointer(
         gate, gate_offset, q.shape[0], num_heads * (1 if gate_per_head else head_dim), what)
     p = _DecodeQ4Params(_place(what, q, torch.bfloat16, here), _place(what, out, torch.bfloat16, here), *_place_pages(what, pages, here),
                         _place(what, positions, int32, here), _place(what, block_table, int32, here),
                         None if entry_starts is None else _place(what, entry_starts, int32, here),
-                        None if sink_values is None else _place(what, sink_values, torch.float32, here), gate_pointer, None, None,
-                        gate_stride, 1 if gate_per_head else 0, width, pages.k_codes.shape[2], 0, pages.k_codes.shape[0], entries,
-                        num_heads, num_kv_heads, head_dim, scale, window, keep_first, 1 if sink else 0, chunk, splits, 0)
-    _check(fn(p, scratch.data_ptr(), scratch.numel(), _stream_of(here)), "attention_decode", kernels=2)
+                        None if sink_values is None else _place(what, sink_values, torch.float32, here), gate_pointer, gate_stride,
+                        1 if gate_per_head else 0, width, pages.k_codes.shape[2], 0, pages.k_codes.shape[0], entries,
+                        num_heads, num_kv_heads, head_dim, scale, window, keep_first, 1 if sink else 0, shares, 0)
+    _check(fn(p, _stream_of(here)), "attention_decode")
 
 
 Q4_ROWS = {(torch.float32, 128): 8, (torch.float32, 64): 16, (torch.bfloat16, 128): 16, (torch.bfloat16, 64): 16}   # (token, head) rows of a block
@@ -1382,7 +1375,7 @@ def attention_q4(q: torch.Tensor, out: torch.Tensor, pages: Q4Pages, *, entry_st
                    gate_per_head=gate_per_head)
     packed = attention_q4_takes_decode(q.dtype, head_dim, page_size)
     if packed and all_single:
-        _attention_q4_decode(q, out, pages, positions=positions, block_table=block_table, max_keys=max_keys, workspace=workspace,
+        _attention_q4_decode(q, out, pages, positions=positions, block_table=block_table, max_keys=max_keys,
                              entry_starts=None, **heads, **endings)
         return
     if attention_q4_takes_rows(q.dtype, head_dim, page_size, count * num_heads, num_heads, 1 if any_single else entries):
@@ -1406,7 +1399,7 @@ def attention_q4(q: torch.Tensor, out: torch.Tensor, pages: Q4Pages, *, entry_st
     attention_prefill(q, out, k_room, v_room, entry_starts=entry_starts, entry_pos0=entry_pos0, block_table=block_table,
                       num_entries=entries, skip_single=apart, **heads, **endings)
     if apart:
-        _attention_q4_decode(q, out, pages, positions=entry_pos0, block_table=block_table, max_keys=max_keys, workspace=workspace,
+        _attention_q4_decode(q, out, pages, positions=entry_pos0, block_table=block_table, max_keys=max_keys,
                              entry_starts=entry_starts, **heads, **endings)
 
 
