@@ -73,12 +73,11 @@ __device__ __forceinline__ float exp2_near(float x) {
 }
 __device__ __forceinline__ float low_of(uint32_t pair) { return __uint_as_float(pair << 16); }
 __device__ __forceinline__ float high_of(uint32_t pair) { return __uint_as_float(pair & 0xffff0000u); }
-// d = a . b + (x, y) for the two columns of every row, and d += a . b, of half-precision operands
-__device__ __forceinline__ void mma_half_from(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float x, float y) {
-  asm(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %10, %11};"
+// d = a . b + c, and d += a . b, of half-precision operands
+__device__ __forceinline__ void mma_half_from(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float4& c) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(x), "f"(y));
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c.x), "f"(c.y), "f"(c.z), "f"(c.w));
 }
 __device__ __forceinline__ void mma_half(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm(
@@ -183,7 +182,10 @@ template <int D, int NT>
 __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) attention_q4_decode_kernel(DecodeParams p) {
   constexpr int G = D / 32, kRowBytes = D / 2, kChunks = kRowBytes / 16;
   constexpr int kRow = D + 4;             // floats of a head's partial in shared memory
-  extern __shared__ __align__(128) uint8_t shared[];   // the warps' stages; then [warp][8 NT heads][kRow] floats
+  extern __shared__ __align__(128) uint8_t shared[];   // the queries, then the warps' stages; at last [warp][8 NT heads][kRow] floats
+  uint4* queries = reinterpret_cast<uint4*>(shared);                                   // [NT][G][lane]
+  float4* offsets = reinterpret_cast<float4*>(shared + NT * G * 512);                  // [NT][G][t]
+  constexpr int kQueryBytes = NT * G * (512 + 64);
   pdl_wait();
   // only now: the kernel behind reads the positions before its own wait, and they may come from the kernel ahead
   pdl_launch_dependents();
@@ -209,7 +211,7 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) attention_q4_dec
   const auto high_key = [&](int tile) { return tile < kept_tiles ? kept - 1 : position; };
 
   // --- the way of the rows into shared memory: 16 bytes a lane, kStages - 1 pairs of tiles ahead ---
-  Stage<D>* stages = reinterpret_cast<Stage<D>*>(shared) + warp * kStages;
+  Stage<D>* stages = reinterpret_cast<Stage<D>*>(shared + kQueryBytes) + warp * kStages;
   const int warp_tile = share * each + 2 * warp;     // step j has tiles warp_tile + 8 j and the next
   const int steps = warp_tile < tiles_end ? (tiles_end - warp_tile + 7) >> 3 : 0;
   // the page of the tile that is this lane's among 32 of the warp's; a tile that is not the block's, and one whose page is not held, has
@@ -285,26 +287,27 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) attention_q4_dec
   for (int j = 0; j < kStages - 1; ++j) fetch(j);
 
   // --- the queries in half precision: lane (g, t) has channels 32 group + 8 t .. + 7 of head 8 nt + g ---
-  uint32_t q[NT][G][4];       // neighbouring channels, the second and fourth pair a 16th
-  float q_offset[NT][G][2];   // -8 times the sum of a group's channels, of heads 2 t and 2 t + 1
-  float q_factor[NT][2];      // what a product has to be multiplied by, of the same heads; in units of log2
+  // in shared memory, a piece of 16 bytes a lane: neighbouring channels, the second and fourth pair a 16th; and, for heads 2 t and 2 t + 1,
+  // -8 times the sum of a group's channels, as what accumulators begin with
+  float q_factor[NT][2];      // what a product has to be multiplied by, of heads 2 t and 2 t + 1; in units of log2
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const int h = head0 + nt * 8 + g;
+    uint32_t q[G][4];
     float largest = 0.0f;
     bool fine = true;
 #pragma unroll
     for (int gr = 0; gr < G; ++gr) {
-      q[nt][gr][0] = q[nt][gr][1] = q[nt][gr][2] = q[nt][gr][3] = 0;
+      q[gr][0] = q[gr][1] = q[gr][2] = q[gr][3] = 0;
       if (h < group)
-        load_words<4>(q[nt][gr], p.q + (static_cast<size_t>(token) * p.num_heads + kv_head * group + h) * D + 32 * gr + 8 * t);
+        load_words<4>(q[gr], p.q + (static_cast<size_t>(token) * p.num_heads + kv_head * group + h) * D + 32 * gr + 8 * t);
     }
 #pragma unroll
     for (int gr = 0; gr < G; ++gr)
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        largest = fmaxf(largest, fmaxf(fabsf(low_of(q[nt][gr][w])), fabsf(high_of(q[nt][gr][w]))));
-        fine = fine && fabsf(low_of(q[nt][gr][w])) < INFINITY && fabsf(high_of(q[nt][gr][w])) < INFINITY;
+        largest = fmaxf(largest, fmaxf(fabsf(low_of(q[gr][w])), fabsf(high_of(q[gr][w]))));
+        fine = fine && fabsf(low_of(q[gr][w])) < INFINITY && fabsf(high_of(q[gr][w])) < INFINITY;
       }
 #pragma unroll
     for (int offset = 1; offset <= 2; offset <<= 1) {
@@ -320,19 +323,22 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) attention_q4_dec
     q_factor[nt][1] = __shfl_sync(0xffffffffu, factor, 8 * t + 4);
 #pragma unroll
     for (int gr = 0; gr < G; ++gr) {
+      if (gr % kWarps != warp) continue;      // every warp a group
       float total = 0.0f;
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        const float lo = low_of(q[nt][gr][w]) * lift, hi = high_of(q[nt][gr][w]) * lift;
+        const float lo = low_of(q[gr][w]) * lift, hi = high_of(q[gr][w]) * lift;
         total += lo + hi;
-        q[nt][gr][w] = w & 1 ? pack_half(lo * 0.0625f, hi * 0.0625f) : pack_half(lo, hi);
+        q[gr][w] = w & 1 ? pack_half(lo * 0.0625f, hi * 0.0625f) : pack_half(lo, hi);
       }
       total += __shfl_xor_sync(0xffffffffu, total, 1);
       total += __shfl_xor_sync(0xffffffffu, total, 2);
-      q_offset[nt][gr][0] = -8.0f * 0x1p-24f * __shfl_sync(0xffffffffu, total, 8 * t);
-      q_offset[nt][gr][1] = -8.0f * 0x1p-24f * __shfl_sync(0xffffffffu, total, 8 * t + 4);
+      const float x = -8.0f * 0x1p-24f * __shfl_sync(0xffffffffu, total, 8 * t), y = -8.0f * 0x1p-24f * __shfl_sync(0xffffffffu, total, 8 * t + 4);
+      queries[(nt * G + gr) * 32 + lane] = make_uint4(q[gr][0], q[gr][1], q[gr][2], q[gr][3]);
+      if (g == 0) offsets[(nt * G + gr) * 4 + t] = make_float4(x, y, x, y);
     }
   }
+  __syncthreads();
   const uint32_t magic = p.magic;
   float o[NT][2 * G][4];      // channels 32 gr + 4 g + 2 h and the next (rows g, g + 8), heads 2 t and 2 t + 1, of codes + 136
   float w_sum[NT][G / 2][4];  // sums of the scaled weights: rows below 8 of a pair's first group, rows above of its second
@@ -365,26 +371,30 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) attention_q4_dec
     const Stage<D>& from = stages[j % kStages];
     const int tile0 = warp_tile + 8 * j;
     float s[2][NT][4];        // rows g (0, 1) and g + 8 (2, 3), heads 2 t and 2 t + 1; in units of log2
+    uint32_t k[2][2][G], k_scale[2][2][G / 2];       // [tile][row g, g + 8]
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      uint32_t k[2][G], scale[2][G / 2];
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        load_words<G>(k[r], from.k[i] + (g + 8 * r) * kRowBytes + t * 4 * G);
-        load_words<G / 2>(scale[r], from.k_scale[i] + (row_key + 8 * r) * (G * 2));
+        load_words<G>(k[i][r], from.k[i] + (g + 8 * r) * kRowBytes + t * 4 * G);
+        load_words<G / 2>(k_scale[i][r], from.k_scale[i] + (row_key + 8 * r) * (G * 2));
       }
 #pragma unroll
-      for (int gr = 0; gr < G; ++gr) {
-        const uint32_t k0 = k[0][gr], k1 = k[1][gr], l0 = k0 >> 8, l1 = k1 >> 8;
-        const uint32_t a[4] = {k0 & 0x000f000fu, k1 & 0x000f000fu, k0 & 0x00f000f0u, k1 & 0x00f000f0u};
-        const uint32_t b[4] = {l0 & 0x000f000fu, l1 & 0x000f000fu, l0 & 0x00f000f0u, l1 & 0x00f000f0u};
-        const float scale0 = gr & 1 ? high_of(scale[0][gr / 2]) : low_of(scale[0][gr / 2]);
-        const float scale1 = gr & 1 ? high_of(scale[1][gr / 2]) : low_of(scale[1][gr / 2]);
+    for (int gr = 0; gr < G; ++gr)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
+      for (int nt = 0; nt < NT; ++nt) {
+        const uint4 q = queries[(nt * G + gr) * 32 + lane];
+        const float4 offset = offsets[(nt * G + gr) * 4 + t];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t k0 = k[i][0][gr], k1 = k[i][1][gr], l0 = k0 >> 8, l1 = k1 >> 8;
+          const uint32_t a[4] = {k0 & 0x000f000fu, k1 & 0x000f000fu, k0 & 0x00f000f0u, k1 & 0x00f000f0u};
+          const uint32_t b[4] = {l0 & 0x000f000fu, l1 & 0x000f000fu, l0 & 0x00f000f0u, l1 & 0x00f000f0u};
+          const float scale0 = gr & 1 ? high_of(k_scale[i][0][gr / 2]) : low_of(k_scale[i][0][gr / 2]);
+          const float scale1 = gr & 1 ? high_of(k_scale[i][1][gr / 2]) : low_of(k_scale[i][1][gr / 2]);
           float acc[4];
-          mma_half_from(acc, a, q[nt][gr][0], q[nt][gr][1], q_offset[nt][gr][0], q_offset[nt][gr][1]);
-          mma_half(acc, b, q[nt][gr][2], q[nt][gr][3]);
+          mma_half_from(acc, a, q.x, q.y, offset);
+          mma_half(acc, b, q.z, q.w);
           s[i][nt][0] = gr ? fmaf(scale0, acc[0], s[i][nt][0]) : scale0 * acc[0];
           s[i][nt][1] = gr ? fmaf(scale0, acc[1], s[i][nt][1]) : scale0 * acc[1];
           s[i][nt][2] = gr ? fmaf(scale1, acc[2], s[i][nt][2]) : scale1 * acc[2];
@@ -392,10 +402,11 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) attention_q4_dec
         }
       }
 #pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int c = 0; c < 4; ++c) s[i][nt][c] *= q_factor[nt][c & 1];
-    }
     // every step but those with a border: all 32 keys are seen
     const int key0 = key_of(tile0);
     const bool whole = tile0 >= kept_tiles && key0 >= first && key0 + kWarpKeys - 1 <= position && tile0 + 1 < tiles_end;
@@ -506,7 +517,7 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) attention_q4_dec
   }
   cp_async_wait<0>();
   __syncthreads();  // the stages become the warps' partials
-  float* merge = reinterpret_cast<float*>(shared);
+  float* merge = reinterpret_cast<float*>(shared + kQueryBytes);
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -578,8 +589,8 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) attention_q4_dec
 
 template <int D, int NT>
 int launch(const DecodeParams& p, cudaStream_t s) {
-  constexpr int kSmem = kWarps * kStages * static_cast<int>(sizeof(Stage<D>));
-  static_assert((kWarps + 1) * 8 * NT * (D + 4) * 4 <= kSmem, "the partials fit in the stages");
+  constexpr int kStageBytes = kWarps * kStages * static_cast<int>(sizeof(Stage<D>)), kSmem = kStageBytes + NT * D / 32 * (512 + 64);
+  static_assert((kWarps + 1) * 8 * NT * (D + 4) * 4 <= kStageBytes, "the partials fit in the stages");
   const auto kernel = attention_q4_decode_kernel<D, NT>;
   cudaError_t error = cudaSuccess;      // every device has to be asked
   if (kSmem > 48 * 1024) error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
