@@ -182,8 +182,9 @@ def test_keys_are_shared_by_a_clusters_blocks_and_cut_into_whole_walks():
 
     for tiles in (1, 3, 8, 64, 300, 12000):
         for keys in (1, 128, 129, 2049, 40000, 10**6):
-            shares = ops.q4_shares(tiles, 1, keys, 148)
-            assert shares in (1, 2, 4, 8, 16) and (shares == 1 or keys > 64 * shares)    # no more than there are walks for, but for one
+            shares = ops.q4_shares(tiles, keys, 148)
+            assert (shares == 0) == (tiles >= 148 and keys > 1024)       # in even runs where there are many and long ones
+            assert shares in (0, 1, 2, 4, 8, 16) and (shares < 2 or keys > 64 * shares)    # no more than there are walks for, but for one
             chunk, splits = ops.q4_rows_splits(tiles, keys, 148)
             assert chunk % 64 == 0 and 0 < splits <= 64 and chunk * (splits - 1) < keys <= chunk * splits
 

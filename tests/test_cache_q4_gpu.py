@@ -238,21 +238,31 @@ def _attend(ops, step, dtype, heads, kv_heads, d, seed=0, window=0, keep_first=0
     assert (out[tokens:] == 7.0).all()          # rows behind the step's last token
 
 
+@pytest.fixture(params=["cluster", "runs"])
+def deal(ops, request, monkeypatch):
+    """How single tokens' keys are shared: by the blocks of a cluster, or dealt out in even runs as where requests are many."""
+    ops.q4_shares.cache_clear()
+    monkeypatch.setattr(ops, "Q4_RUNS_FROM", 0.0 if request.param == "runs" else 1e9)
+    monkeypatch.setattr(ops, "Q4_RUNS_KEYS", 0)
+    yield request.param
+    ops.q4_shares.cache_clear()
+
+
 @pytest.mark.parametrize("heads, kv_heads, d", [(12, 2, 128), (14, 2, 64), (4, 4, 128), (20, 1, 128), (5, 1, 64), (16, 1, 64), (40, 2, 64)])
-@pytest.mark.parametrize("history", [[0], [15, 16, 17, 0, 31], [300, 127, 128, 1, 129]])
-def test_single_tokens_over_packed_pages(ops, heads, kv_heads, d, history):
+@pytest.mark.parametrize("history", [[0], [15, 16, 17, 0, 31], [300, 127, 128, 1, 129], [5] * 40 + [1500]])
+def test_single_tokens_over_packed_pages(ops, deal, heads, kv_heads, d, history):
     _attend(ops, Step([1] * len(history), history, 16, seed=heads), torch.bfloat16, heads, kv_heads, d)
 
 
 @pytest.mark.parametrize("page_size", [32, 48, 64])
-def test_single_tokens_over_pages_of_other_sizes(ops, page_size):
+def test_single_tokens_over_pages_of_other_sizes(ops, deal, page_size):
     _attend(ops, Step([1, 1], [200, 47], page_size), torch.bfloat16, 6, 2, 128)
 
 
 @pytest.mark.parametrize("window, keep_first", [(1, 0), (16, 0), (100, 4), (40, 37), (1000, 5), (33, 64)])
 @pytest.mark.parametrize("sink", [False, True])
 @pytest.mark.parametrize("d", [64, 128])
-def test_windows_kept_keys_and_sinks(ops, window, keep_first, sink, d):
+def test_windows_kept_keys_and_sinks(ops, deal, window, keep_first, sink, d):
     _attend(ops, Step([1, 1, 1], [300, 39, 0], 16, seed=window), torch.bfloat16, 8, 2, d, window=window, keep_first=keep_first, sink=sink)
 
 
@@ -295,14 +305,28 @@ def test_portions_with_windows_and_kept_keys(ops, form, dtype, window, keep_firs
     _attend(ops, Step([20, 1, 41], [33, 64, 0], 16), dtype, heads, kv_heads, d, window=window, keep_first=keep_first, sink=keep_first == 5)
 
 
-def test_a_long_history_in_many_splits(ops):
+def test_single_tokens_beside_portions_in_either_deal(ops, deal, monkeypatch):
+    """The entries of one token of a mixed step, the others skipped: none of them first, some last, several in a row."""
+    monkeypatch.setattr(ops, "Q4_ROWS_FIRST", 0)
+    _attend(ops, Step([5, 1, 1, 40, 1, 3, 1], [9, 300, 0, 0, 77, 20, 500], 16), torch.bfloat16, 6, 2, 64)
+    _attend(ops, Step([1, 20, 2], [130, 10, 0], 16), torch.bfloat16, 4, 2, 128, window=50, keep_first=7)
+
+
+def test_many_requests_take_the_even_runs(ops):
+    ops.q4_shares.cache_clear()
+    assert ops.q4_shares(180, 1200, ops._sm_count_of(0)) == 0
+    rng = np.random.default_rng(12)
+    _attend(ops, Step([1] * 90, [int(x) for x in rng.integers(0, 300, 89)] + [1199], 16), torch.bfloat16, 4, 2, 64)
+
+
+def test_a_long_history_in_many_splits(ops, deal):
     """Thousands of keys, the longest beside a short one, of single tokens and of portions."""
     _attend(ops, Step([1, 1], [9000, 5], 16), torch.bfloat16, 2, 1, 64)
     for dtype in (torch.bfloat16, torch.float32):
         _attend(ops, Step([3, 1], [5000, 5], 16), dtype, 2, 1, 64)
 
 
-def test_values_that_are_not_finite_show_where_they_are_seen(ops):
+def test_values_that_are_not_finite_show_where_they_are_seen(ops, deal):
     """A NaN key or value makes the outputs of the tokens that see it NaN, and of no others."""
     for which in ("k_scales", "v_scales"):
         step = Step([1, 1, 1], [200, 40, 40], 16)
@@ -333,7 +357,7 @@ def test_values_that_are_not_finite_show_where_they_are_seen(ops):
     assert out.isnan().all()
 
 
-def test_scores_of_zero_and_equal_keys_give_the_mean(ops):
+def test_scores_of_zero_and_equal_keys_give_the_mean(ops, deal):
     """A query of zeros weighs its keys alike: scores whose maximum is exactly 0."""
     step = Step([1], [99], 16)
     pages = ops.Q4Pages(*plain.make_pages(step.num_pages, 16, 1, 64, 4, DEVICE))

@@ -1,9 +1,9 @@
 // Attention of single tokens over pages of 4 bits (formats: q4.cuh), split over the keys, on mma.sync m16n8k16.
 //
 // A block is (entry, KV head and up to 8 NT of its query heads, share of the visible keys); its four warps fold 32 keys at a time each
-// with a running (max, sum, output) and merge at the end.  The blocks of an (entry, KV head) are a cluster that joins its shares
-// through distributed shared memory and writes the output: one launch, nothing passes through memory, and shares are cut
-// from the entry's own keys, so that blocks of one cluster carry equal loads.
+// with a running (max, sum, output) and merge at the end.  Where (entry, KV head) pairs are few, a cluster shares the keys of one and joins
+// its parts through distributed shared memory: one launch, and nothing passes through memory.  Where they are many, the keys
+// of all pairs are dealt to the blocks in even runs, and a second kernel joins the pairs that several runs share.
 //
 // Both products put the packed operand on the side of 16 (keys for the scores, channels for the values) and the query
 // heads on the side of 8: a group of 8 heads or fewer costs half of the products that the other way round would
@@ -49,7 +49,7 @@ struct DecodeParams {
 
 constexpr int kWarps = 4;
 constexpr int kWarpKeys = 32;   // keys a warp folds at a time: two tiles of 16
-constexpr int kStages = 4;      // such pairs of tiles on their way to shared memory for each warp
+constexpr int kStages = 3;      // such pairs of tiles on their way to shared memory for each warp
 
 __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
   const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
@@ -178,48 +178,61 @@ struct Stage {
   uint8_t v_scale[2][16 * G * 2];
 };
 
-template <int D, int NT>
-__global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) attention_q4_decode_kernel(DecodeParams p) {
-  constexpr int G = D / 32, kRowBytes = D / 2, kChunks = kRowBytes / 16;
-  constexpr int kRow = D + 4;             // floats of a head's partial in shared memory
-  extern __shared__ __align__(128) uint8_t shared[];   // the queries, then the warps' stages; at last [warp][8 NT heads][kRow] floats
-  uint4* queries = reinterpret_cast<uint4*>(shared);                                   // [NT][G][lane]
-  float4* offsets = reinterpret_cast<float4*>(shared + NT * G * 512);                  // [NT][G][t]
-  constexpr int kQueryBytes = NT * G * (512 + 64);
-  pdl_wait();
-  // only now: the kernel behind reads the positions before its own wait, and they may come from the kernel ahead
-  pdl_launch_dependents();
-  const int group = p.num_heads / p.num_kv_heads, head_tiles = (group + 8 * NT - 1) / (8 * NT);
-  const int entry = blockIdx.x, share = blockIdx.z;
-  const int kv_head = blockIdx.y / head_tiles, head0 = (blockIdx.y - kv_head * head_tiles) * 8 * NT;
-  int token = entry;
-  if (p.entry_starts) {
-    token = p.entry_starts[entry];
-    if (p.entry_starts[entry + 1] - token != 1) return;   // the whole cluster's
+// The visible keys of a query in tiles of 16: those of the kept first keys that the window has left behind, then those of the window.
+struct Visible {
+  int position, first, kept, kept_tiles, first_tile, tiles;
+  __device__ __forceinline__ Visible(const DecodeParams& p, int at) {
+    position = at;
+    first = first_visible_key(position, p.window);
+    kept = p.window > 0 ? min(p.keep_first, first) : 0;
+    kept_tiles = (kept + 15) >> 4;
+    first_tile = first >> 4;
+    tiles = kept_tiles + max((position >> 4) - first_tile + 1, 0);
   }
+  __device__ __forceinline__ int key_of(int tile) const { return 16 * (tile < kept_tiles ? tile : tile - kept_tiles + first_tile); }
+  __device__ __forceinline__ bool hides(int tile, int key) const {
+    return tile < kept_tiles ? key >= kept : key < first || key > position;
+  }
+};
+
+// What a block has in shared memory: the queries, the warps' stages, and, at the end of a walk in the place of the stages, the warps' partials
+// [warp][8 NT heads][D + 4] and behind them what they join to, `joined` [8 NT heads][D + 4]: outputs, maximum, sum.
+template <int D, int NT>
+struct Shared {
+  static constexpr int kRow = D + 4, kQueryBytes = NT * (D / 32) * (512 + 64);
+  static constexpr int kStageBytes = kWarps * kStages * static_cast<int>(sizeof(Stage<D>)), kBytes = kQueryBytes + kStageBytes;
+  static_assert((kWarps + 1) * 8 * NT * kRow * 4 <= kStageBytes, "the partials fit in the stages");
+  uint8_t* at;
+  __device__ __forceinline__ uint4* queries() const { return reinterpret_cast<uint4*>(at); }                                // [NT][G][lane]
+  __device__ __forceinline__ float4* offsets() const { return reinterpret_cast<float4*>(at + NT * (D / 32) * 512); }        // [NT][G][t]
+  __device__ __forceinline__ Stage<D>* stages() const { return reinterpret_cast<Stage<D>*>(at + kQueryBytes); }
+  __device__ __forceinline__ float* merge() const { return reinterpret_cast<float*>(at + kQueryBytes); }
+  __device__ __forceinline__ float* joined() const { return merge() + kWarps * 8 * NT * kRow; }
+};
+
+// The block's walk over tiles tile_begin (a multiple of 8) to tiles_end - 1 of what the query heads head0 .. of a KV head see; it leaves the
+// heads' outputs, maxima and sums in `joined`, to be read behind a barrier.
+template <int D, int NT>
+__device__ __forceinline__ void walk(const DecodeParams& p, const Shared<D, NT> shared, const Visible seen, int entry, int token, int kv_head,
+                                     int head0, int tile_begin, int tiles_end) {
+  constexpr int G = D / 32, kRowBytes = D / 2, kChunks = kRowBytes / 16;
+  constexpr int kRow = D + 4;
+  uint4* queries = shared.queries();
+  float4* offsets = shared.offsets();
+  const int group = p.num_heads / p.num_kv_heads;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int position = p.positions[entry];
   const int* table = p.block_table + static_cast<size_t>(entry) * p.table_width;
-  // The visible keys in tiles of 16: those of the kept first keys that the window has left behind, then those of the window.
-  const int first = first_visible_key(position, p.window), kept = p.window > 0 ? min(p.keep_first, first) : 0;
-  const int kept_tiles = (kept + 15) >> 4, first_tile = first >> 4;
-  const int tiles = kept_tiles + max((position >> 4) - first_tile + 1, 0);
-  const int each = (tiles + 8 * p.shares - 1) / (8 * p.shares) * 8;      // of a block: whole steps of its warps
-  const int tiles_end = min((share + 1) * each, tiles);
-  const auto key_of = [&](int tile) { return 16 * (tile < kept_tiles ? tile : tile - kept_tiles + first_tile); };
-  const auto low_key = [&](int tile) { return tile < kept_tiles ? 0 : first; };
-  const auto high_key = [&](int tile) { return tile < kept_tiles ? kept - 1 : position; };
 
   // --- the way of the rows into shared memory: 16 bytes a lane, kStages - 1 pairs of tiles ahead ---
-  Stage<D>* stages = reinterpret_cast<Stage<D>*>(shared + kQueryBytes) + warp * kStages;
-  const int warp_tile = share * each + 2 * warp;     // step j has tiles warp_tile + 8 j and the next
+  Stage<D>* stages = shared.stages() + warp * kStages;
+  const int warp_tile = tile_begin + 2 * warp;     // step j has tiles warp_tile + 8 j and the next
   const int steps = warp_tile < tiles_end ? (tiles_end - warp_tile + 7) >> 3 : 0;
   // the page of the tile that is this lane's among 32 of the warp's; a tile that is not the block's, and one whose page is not held, has
   // none and is filled with zeros
   const auto page_of = [&](int index) {
     const int tile = warp_tile + (index >> 1) * 8 + (index & 1);
     if (tile >= tiles_end) return -1;
-    const int key = key_of(tile), place = p.page_shift >= 0 ? key >> p.page_shift : key / p.page_size;
+    const int key = seen.key_of(tile), place = p.page_shift >= 0 ? key >> p.page_shift : key / p.page_size;
     const int page = place < p.table_width ? table[place] : -1;
     return page < p.num_pages ? page : -1;
   };
@@ -253,7 +266,7 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) attention_q4_dec
       if (!one_tile_a_page) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const int key = key_of(warp_tile + 8 * j + i);
+          const int key = seen.key_of(warp_tile + 8 * j + i);
           place[i] = p.page_shift >= 0 ? key & (p.page_size - 1) : key % p.page_size;
         }
       }
@@ -408,15 +421,14 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) attention_q4_dec
 #pragma unroll
         for (int c = 0; c < 4; ++c) s[i][nt][c] *= q_factor[nt][c & 1];
     // every step but those with a border: all 32 keys are seen
-    const int key0 = key_of(tile0);
-    const bool whole = tile0 >= kept_tiles && key0 >= first && key0 + kWarpKeys - 1 <= position && tile0 + 1 < tiles_end;
+    const int key0 = seen.key_of(tile0);
+    const bool whole = tile0 >= seen.kept_tiles && key0 >= seen.first && key0 + kWarpKeys - 1 <= seen.position && tile0 + 1 < tiles_end;
     if (!whole) {
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const int key = key_of(tile0 + i) + 8 * r + row_key;
-          if (tile0 + i >= tiles_end || key < low_key(tile0 + i) || key > high_key(tile0 + i)) {
+          if (tile0 + i >= tiles_end || seen.hides(tile0 + i, seen.key_of(tile0 + i) + 8 * r + row_key)) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) s[i][nt][2 * r] = s[i][nt][2 * r + 1] = -INFINITY;
           }
@@ -469,8 +481,7 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) attention_q4_dec
       if (!whole) {   // a hidden key's weight is 0, and its scale must not make that NaN
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
-          const int key = key_of(tile0 + i) + 4 * n + t;
-          if (tile0 + i >= tiles_end || key < low_key(tile0 + i) || key > high_key(tile0 + i)) {
+          if (tile0 + i >= tiles_end || seen.hides(tile0 + i, seen.key_of(tile0 + i) + 4 * n + t)) {
 #pragma unroll
             for (int w = 0; w < G / 2; ++w) scale[n][w] = 0;
           }
@@ -517,7 +528,7 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) attention_q4_dec
   }
   cp_async_wait<0>();
   __syncthreads();  // the stages become the warps' partials
-  float* merge = reinterpret_cast<float*>(shared + kQueryBytes);
+  float* merge = shared.merge();
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -549,54 +560,264 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) attention_q4_dec
   }
   __syncthreads();
   // the block merges them, a few threads a head
-  float* joined = merge + kWarps * 8 * NT * kRow;     // [8 NT heads][kRow]
-  {
-    constexpr int kThreadsOfHead = 32 * kWarps / (8 * NT);
-    const int head = threadIdx.x / kThreadsOfHead;
-    merge_warps<D, 8 * NT>(merge, head, threadIdx.x % kThreadsOfHead, joined + head * kRow + D, joined + head * kRow);
+  float* joined = shared.joined();
+  constexpr int kThreadsOfHead = 32 * kWarps / (8 * NT);
+  const int head = threadIdx.x / kThreadsOfHead;
+  merge_warps<D, 8 * NT>(merge, head, threadIdx.x % kThreadsOfHead, joined + head * kRow + D, joined + head * kRow);
+}
+
+// Four channels of a head's output: the ending's sink and gate, and the store.
+template <int D>
+__device__ __forceinline__ void finish(const DecodeParams& p, int token, int head, int column, float best, float total, const float4& value) {
+  if (p.sink) total += exp2f((p.sink_values ? p.sink_values[head] * kLog2e : 0.0f) - best);
+  float out[4] = {value.x / total, value.y / total, value.z / total, value.w / total};
+  if (p.gate) {
+    const float* gate = p.gate + static_cast<size_t>(token) * p.gate_stride + (p.gate_per_head ? head : head * D + column);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) out[c] *= 1.0f / (1.0f + expf(-gate[p.gate_per_head ? 0 : c]));
   }
-  // and the cluster its blocks: every thread has four channels of a head at a time
+  store_four_as<__nv_bfloat16>(p.out + (static_cast<size_t>(token) * p.num_heads + head) * D + column, out[0], out[1], out[2], out[3]);
+}
+
+// One more part joins a row's four channels: its weights were taken against another maximum.
+struct Join {
+  float best = -INFINITY, total = 0.0f;
+  float4 value = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  __device__ __forceinline__ void add(float m, float l, const float4& v) {
+    const float w = m == -INFINITY ? 0.0f : exp2f(m - best);    // -inf: a part without visible keys
+    total += l * w;
+    value.x += v.x * w;
+    value.y += v.y * w;
+    value.z += v.z * w;
+    value.w += v.w * w;
+  }
+};
+
+// Few (entry, KV head) pairs: the blocks of a cluster share the keys of one, each a part as large, and join their parts.
+template <int D, int NT>
+__global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) attention_q4_cluster_kernel(DecodeParams p) {
+  constexpr int kRow = D + 4;
+  extern __shared__ __align__(128) uint8_t shared_at[];
+  const Shared<D, NT> shared{shared_at};
+  pdl_wait();
+  pdl_launch_dependents();
+  const int group = p.num_heads / p.num_kv_heads, head_tiles = (group + 8 * NT - 1) / (8 * NT);
+  const int entry = blockIdx.x, share = blockIdx.z;
+  const int kv_head = blockIdx.y / head_tiles, head0 = (blockIdx.y - kv_head * head_tiles) * 8 * NT;
+  int token = entry;
+  if (p.entry_starts) {
+    token = p.entry_starts[entry];
+    if (p.entry_starts[entry + 1] - token != 1) return;   // the whole cluster's
+  }
+  const Visible seen(p, p.positions[entry]);
+  const int each = (seen.tiles + 8 * p.shares - 1) / (8 * p.shares) * 8;      // of a block: whole steps of its warps
+  walk<D, NT>(p, shared, seen, entry, token, kv_head, head0, share * each, min((share + 1) * each, seen.tiles));
   cluster_sync_all();
   const int heads_here = min(8 * NT, group - head0);
-  const uint32_t joined_at = smem_addr(joined);
+  const uint32_t joined_at = smem_addr(shared.joined());
   for (int i = share * static_cast<int>(blockDim.x) + threadIdx.x; i < heads_here * (D / 4); i += p.shares * blockDim.x) {
-    const int h = i / (D / 4), column = (i - h * (D / 4)) * 4, head = kv_head * group + head0 + h;
-    float best = -INFINITY, total = 0.0f;
-    for (int c = 0; c < p.shares; ++c) best = fmaxf(best, cluster_load(joined_at + (h * kRow + D) * 4, c));
-    float4 value = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const int h = i / (D / 4), column = (i - h * (D / 4)) * 4;
+    Join join;
+    for (int c = 0; c < p.shares; ++c) join.best = fmaxf(join.best, cluster_load(joined_at + (h * kRow + D) * 4, c));
 #pragma unroll 4
-    for (int c = 0; c < p.shares; ++c) {
-      const float m = cluster_load(joined_at + (h * kRow + D) * 4, c), l = cluster_load(joined_at + (h * kRow + D + 1) * 4, c);
-      const float4 v = cluster_load_4(joined_at + (h * kRow + column) * 4, c);
-      const float w = m == -INFINITY ? 0.0f : exp2f(m - best);    // a share without visible keys
-      total += l * w;
-      value.x += v.x * w;
-      value.y += v.y * w;
-      value.z += v.z * w;
-      value.w += v.w * w;
-    }
-    if (p.sink) total += exp2f((p.sink_values ? p.sink_values[head] * kLog2e : 0.0f) - best);
-    float out[4] = {value.x / total, value.y / total, value.z / total, value.w / total};
-    if (p.gate) {
-      const float* gate = p.gate + static_cast<size_t>(token) * p.gate_stride + (p.gate_per_head ? head : head * D + column);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) out[c] *= 1.0f / (1.0f + expf(-gate[p.gate_per_head ? 0 : c]));
-    }
-    store_four_as<__nv_bfloat16>(p.out + (static_cast<size_t>(token) * p.num_heads + head) * D + column, out[0], out[1], out[2], out[3]);
+    for (int c = 0; c < p.shares; ++c)
+      join.add(cluster_load(joined_at + (h * kRow + D) * 4, c), cluster_load(joined_at + (h * kRow + D + 1) * 4, c),
+               cluster_load_4(joined_at + (h * kRow + column) * 4, c));
+    finish<D>(p, token, kv_head * group + head0 + h, column, join.best, join.total, join.value);
   }
   cluster_sync_all();   // nobody's shared memory goes while others read it
 }
 
+// Many pairs: the keys of all of them, in units of 8 tiles one pair behind the other, are dealt to the launch's blocks in even runs, so
+// that no block waits for another's longer history.  A walk costs as much as kBegin units before its first one (its queries, its first
+// rows' way, joining its warps), so a pair counts that many in front of its own, or a run of short pairs would outlast the others (the
+// batch of 64 with histories of 0 to 4,095 keys: 39 us with most blocks idle for half of it).  A pair that lies in one block's run is
+// finished there; of one that several share, each leaves its part in memory (`parts`: two places a block, the first for a pair
+// that began in an earlier block) and a second kernel joins them.
+constexpr int kBegin = 3;
+__device__ __forceinline__ int units_for(const DecodeParams& p, int position) {
+  const int tiles = Visible(p, position).tiles;
+  return tiles > 0 ? ((tiles + 7) >> 3) + kBegin : 0;
+}
+__device__ __forceinline__ int units_of(const DecodeParams& p, int entry) {
+  if (entry >= p.num_entries || (p.entry_starts && p.entry_starts[entry + 1] - p.entry_starts[entry] != 1)) return 0;
+  return units_for(p, p.positions[entry]);
+}
+constexpr int kRunEntries = 1024;   // entries whose lengths a block holds
+
 template <int D, int NT>
-int launch(const DecodeParams& p, cudaStream_t s) {
-  constexpr int kStageBytes = kWarps * kStages * static_cast<int>(sizeof(Stage<D>)), kSmem = kStageBytes + NT * D / 32 * (512 + 64);
-  static_assert((kWarps + 1) * 8 * NT * (D + 4) * 4 <= kStageBytes, "the partials fit in the stages");
-  const auto kernel = attention_q4_decode_kernel<D, NT>;
-  cudaError_t error = cudaSuccess;      // every device has to be asked
+__global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) attention_q4_runs_kernel(DecodeParams p, float* __restrict__ parts) {
+  constexpr int kRow = D + 4;
+  extern __shared__ __align__(128) uint8_t shared_at[];
+  const Shared<D, NT> shared{shared_at};
+  __shared__ int positions[kRunEntries], ends[kRunEntries];    // ends: units up to and with an entry
+  __shared__ int warp_units[kWarps];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int group = p.num_heads / p.num_kv_heads, head_tiles = (group + 8 * NT - 1) / (8 * NT), pairs = p.num_kv_heads * head_tiles;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int whole = 0;
+  for (int e0 = 0; e0 < p.num_entries; e0 += 32 * kWarps) {
+    const int e = e0 + threadIdx.x;
+    int position = -1;
+    if (e < p.num_entries && !(p.entry_starts && p.entry_starts[e + 1] - p.entry_starts[e] != 1)) position = p.positions[e];
+    int upto = position >= 0 ? units_for(p, position) : 0;
+#pragma unroll
+    for (int offset = 1; offset < 32; offset <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, upto, offset);
+      if (lane >= offset) upto += v;
+    }
+    if (lane == 31) warp_units[warp] = upto;
+    __syncthreads();
+    int total = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) upto += warp_units[w];
+      total += warp_units[w];
+    }
+    if (e < p.num_entries) {
+      positions[e] = position;
+      ends[e] = whole + upto;
+    }
+    whole += total;
+    __syncthreads();
+  }
+  const long long all = static_cast<long long>(whole) * pairs;
+  const long long runs = min(static_cast<long long>(gridDim.x), all);     // each with a unit at least
+  if (blockIdx.x >= runs) return;
+  long long at = all * blockIdx.x / runs;
+  const long long stop = all * (blockIdx.x + 1) / runs;
+  int entry = 0;                                   // in which the run begins: the first that ends behind it
+  for (int high = p.num_entries - 1; entry < high;) {
+    const int middle = (entry + high) >> 1;
+    if (static_cast<long long>(ends[middle]) * pairs > at) high = middle;
+    else entry = middle + 1;
+  }
+  const auto units_at = [&](int e) { return ends[e] - (e > 0 ? ends[e - 1] : 0); };
+  int units = units_at(entry);
+  if (units == 0) return;
+  const int into = static_cast<int>(at - static_cast<long long>(ends[entry] - units) * pairs);
+  int pair = into / units, unit = into - pair * units;
+  while (at < stop && entry < p.num_entries) {
+    const int token = p.entry_starts ? p.entry_starts[entry] : entry;
+    const int kv_head = pair / head_tiles, head0 = (pair - kv_head * head_tiles) * 8 * NT;
+    const int run = static_cast<int>(min(static_cast<long long>(units - unit), stop - at));
+    // the run's own keys: units kBegin and behind
+    const int own = max(unit - kBegin, 0), own_end = unit + run - kBegin;
+    const bool whole_pair = own == 0 && own_end == units - kBegin;
+    if (own_end > 0) {
+      const Visible seen(p, positions[entry]);
+      walk<D, NT>(p, shared, seen, entry, token, kv_head, head0, 8 * own, min(8 * own_end, seen.tiles));
+      __syncthreads();
+      const int heads_here = min(8 * NT, group - head0);
+      const float* joined = shared.joined();
+      if (whole_pair) {
+        for (int i = threadIdx.x; i < heads_here * (D / 4); i += blockDim.x) {
+          const int h = i / (D / 4), column = (i - h * (D / 4)) * 4;
+          finish<D>(p, token, kv_head * group + head0 + h, column, joined[h * kRow + D], joined[h * kRow + D + 1],
+                    *reinterpret_cast<const float4*>(joined + h * kRow + column));
+        }
+      } else {
+        float* part = parts + (2 * static_cast<size_t>(blockIdx.x) + (own > 0 ? 0 : 1)) * (8 * NT * kRow);
+        for (int i = threadIdx.x; i < heads_here * (kRow / 4); i += blockDim.x)
+          reinterpret_cast<float4*>(part)[i] = reinterpret_cast<const float4*>(joined)[i];
+      }
+      __syncthreads();   // the next walk's queries and stages lie where this one's are
+    }
+    at += run;
+    unit = 0;
+    if (at < stop && ++pair == pairs) {
+      pair = 0;
+      do ++entry;
+      while (entry < p.num_entries && (units = units_at(entry)) == 0);
+    }
+  }
+}
+
+// A block per (entry, pair): joins the parts of a pair that several runs share.
+template <int D, int NT>
+__global__ void __launch_bounds__(128) attention_q4_join_kernel(DecodeParams p, const float* __restrict__ parts, int blocks) {
+  constexpr int kRow = D + 4;
+  __shared__ int sums[2][4];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int group = p.num_heads / p.num_kv_heads, head_tiles = (group + 8 * NT - 1) / (8 * NT), pairs = p.num_kv_heads * head_tiles;
+  const int entry = blockIdx.x, pair = blockIdx.y;
+  int ahead = 0, whole = 0;
+#pragma unroll 4
+  for (int e = threadIdx.x; e < p.num_entries; e += 128) {
+    const int units = units_of(p, e);
+    whole += units;
+    if (e < entry) ahead += units;
+  }
+  const int units = units_of(p, entry);
+  ahead = __reduce_add_sync(0xffffffffu, ahead);
+  whole = __reduce_add_sync(0xffffffffu, whole);
+  if ((threadIdx.x & 31) == 0) {
+    sums[0][threadIdx.x >> 5] = ahead;
+    sums[1][threadIdx.x >> 5] = whole;
+  }
+  __syncthreads();
+  if (units == 0) return;
+  ahead = sums[0][0] + sums[0][1] + sums[0][2] + sums[0][3];
+  whole = sums[1][0] + sums[1][1] + sums[1][2] + sums[1][3];
+  const long long all = static_cast<long long>(whole) * pairs, start = static_cast<long long>(ahead) * pairs + static_cast<long long>(pair) * units;
+  const long long last = start + units - 1, runs = min(static_cast<long long>(blocks), all);
+  // the run that holds a unit x: the last one that begins at x or in front of it; the pair's keys begin behind its first kBegin
+  const int first_run = static_cast<int>(((start + kBegin + 1) * runs - 1) / all), last_run = static_cast<int>(((last + 1) * runs - 1) / all);
+  if (first_run == last_run) return;      // finished there
+  const int kv_head = pair / head_tiles, head0 = (pair - kv_head * head_tiles) * 8 * NT, heads_here = min(8 * NT, group - head0);
+  const int token = p.entry_starts ? p.entry_starts[entry] : entry;
+  const auto part_of = [&](int r) { return parts + (2 * static_cast<size_t>(r) + (r == first_run ? 1 : 0)) * (8 * NT * kRow); };
+  for (int i = threadIdx.x; i < heads_here * (D / 4); i += blockDim.x) {
+    const int h = i / (D / 4), column = (i - h * (D / 4)) * 4;
+    Join join;
+    constexpr int kAtOnce = 4;        // parts that are asked for together; the maximum follows them
+    for (int r = first_run; r <= last_run; r += kAtOnce) {
+      float m[kAtOnce], l[kAtOnce];
+      float4 v[kAtOnce];
+#pragma unroll
+      for (int c = 0; c < kAtOnce; ++c) {
+        const float* part = part_of(min(r + c, last_run)) + h * kRow;
+        m[c] = r + c <= last_run ? part[D] : -INFINITY;
+        l[c] = part[D + 1];
+        v[c] = *reinterpret_cast<const float4*>(part + column);
+      }
+      float best = join.best;
+#pragma unroll
+      for (int c = 0; c < kAtOnce; ++c) best = fmaxf(best, m[c]);
+      const Join before = join;
+      join = Join();
+      join.best = best;
+      join.add(before.best, before.total, before.value);
+#pragma unroll
+      for (int c = 0; c < kAtOnce; ++c) join.add(m[c], l[c], v[c]);
+    }
+    finish<D>(p, token, kv_head * group + head0 + h, column, join.best, join.total, join.value);
+  }
+}
+
+template <int D, int NT>
+int launch(const DecodeParams& p, float* parts, int runs, cudaStream_t s) {
+  constexpr int kSmem = Shared<D, NT>::kBytes;
+  const int group = p.num_heads / p.num_kv_heads, head_tiles = (group + 8 * NT - 1) / (8 * NT);
+  if (p.num_kv_heads * head_tiles > 65535) return VIPERA_BAD_SHAPE;
+  if (p.shares == 0) {
+    const auto kernel = attention_q4_runs_kernel<D, NT>;
+    cudaError_t error = cudaSuccess;     // every device has to be asked
+    if (kSmem > 48 * 1024) error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    if (error == cudaSuccess) error = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    if (error != cudaSuccess) return static_cast<int>(error);
+    const int status = vipera_launch(kernel, dim3(runs), 32 * kWarps, kSmem, s, p, parts);
+    if (status != VIPERA_OK) return status;
+    return vipera_launch(attention_q4_join_kernel<D, NT>, dim3(p.num_entries, p.num_kv_heads * head_tiles), 128, 0, s, p, parts, runs);
+  }
+  const auto kernel = attention_q4_cluster_kernel<D, NT>;
+  cudaError_t error = cudaSuccess;
   if (kSmem > 48 * 1024) error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  if (error == cudaSuccess) error = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
   if (error == cudaSuccess && p.shares > 8) error = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (error != cudaSuccess) return static_cast<int>(error);
-  const int group = p.num_heads / p.num_kv_heads, head_tiles = (group + 8 * NT - 1) / (8 * NT);
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(p.num_entries, p.num_kv_heads * head_tiles, p.shares);
   config.blockDim = dim3(32 * kWarps);
@@ -627,15 +848,23 @@ bool on_16_bytes(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) =
 
 VIPERA_API int vipera_attention_q4_params_size() { return static_cast<int>(sizeof(DecodeParams)); }
 
-// Attention of the entries that bring one token (all of them where entry_starts is null); p->shares blocks, a power of two up to
-// 16, share an entry's keys.
-VIPERA_API int vipera_attention_q4_decode(const DecodeParams* given, void* stream) {
+// Floats of scratch for `runs` runs: two parts each, of the query heads that a block has.
+VIPERA_API size_t vipera_attention_q4_parts(int runs, int num_heads, int num_kv_heads, int head_dim) {
+  return static_cast<size_t>(runs) * 2 * (num_heads / num_kv_heads > 8 ? 16 : 8) * (head_dim + 4);
+}
+
+// Attention of the entries that bring one token (all of them where entry_starts is null).  p->shares: the blocks, a power of two up to
+// 16, that share an entry's keys; 0: all entries' keys go to `runs` blocks in even runs, and `parts` holds their parts.
+VIPERA_API int vipera_attention_q4_decode(const DecodeParams* given, float* parts, size_t parts_floats, int runs, void* stream) {
   DecodeParams p = *given;
   if (p.num_entries <= 0) return VIPERA_OK;
   if (p.num_heads <= 0 || p.num_kv_heads <= 0 || p.num_heads % p.num_kv_heads || p.keep_first < 0 || p.page_size <= 0 ||
-      p.page_size % 16 || p.num_heads > 65535 || p.shares <= 0 || p.shares > 16 || (p.shares & (p.shares - 1)) ||
+      p.page_size % 16 || p.num_heads > 65535 || p.shares < 0 || p.shares > 16 || (p.shares & (p.shares - 1)) ||
       (p.head_dim != 64 && p.head_dim != 128))
     return VIPERA_BAD_SHAPE;
+  if (p.shares == 0 && (runs <= 0 || p.num_entries > kRunEntries || !parts || !on_16_bytes(parts) ||
+                        parts_floats < vipera_attention_q4_parts(runs, p.num_heads, p.num_kv_heads, p.head_dim)))
+    return VIPERA_BAD_ARGUMENT;
   if (p.sink_values) p.sink = 1;
   if (!on_16_bytes(p.q) || !on_16_bytes(p.k_codes) || !on_16_bytes(p.v_codes) || !on_16_bytes(p.k_scales) || !on_16_bytes(p.v_scales) ||
       (reinterpret_cast<uintptr_t>(p.out) & 7))
@@ -646,8 +875,8 @@ VIPERA_API int vipera_attention_q4_decode(const DecodeParams* given, void* strea
     for (p.page_shift = 0; (1 << p.page_shift) < p.page_size;) ++p.page_shift;
   const bool wide = p.num_heads / p.num_kv_heads > 8;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (p.head_dim == 128) return wide ? launch<128, 2>(p, s) : launch<128, 1>(p, s);
-  return wide ? launch<64, 2>(p, s) : launch<64, 1>(p, s);
+  if (p.head_dim == 128) return wide ? launch<128, 2>(p, parts, runs, s) : launch<128, 1>(p, parts, runs, s);
+  return wide ? launch<64, 2>(p, parts, runs, s) : launch<64, 1>(p, parts, runs, s);
 }
 
 VIPERA_API int vipera_attention_q4_rows_params_size() { return static_cast<int>(sizeof(RowsParams)); }

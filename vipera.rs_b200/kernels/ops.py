@@ -1242,20 +1242,28 @@ def attention_q4_takes_decode(dtype: torch.dtype, head_dim: int, page_size: int)
     return dtype == torch.bfloat16 and head_dim in MMA_HEAD_DIMS and page_size % 16 == 0
 
 
-# The packed kernel's blocks: three an SM at once, and a walk's time in microseconds: what a block costs beside its keys, and what each 128
-# of them cost where one, two or three blocks share an SM (fitted to launches at batch 1 to 64 and 2,048 to 32,768 keys).
+# The packed kernel's blocks that an SM holds at once, and a walk's time in microseconds: what a block costs beside its keys, and what
+# each 128 of them cost where one, two or three blocks share an SM (fitted to launches at batch 1 to 64 and 2,048 to 32,768 keys).
 Q4_BLOCKS_PER_SM = 3
 Q4_BLOCK_FIXED, Q4_BLOCK_KEYS = 2.2, (0.0, 0.8, 1.25, 1.75)
+# From this many (entry, KV head) pairs on, for each SM, histories of more than this many keys are dealt to the blocks in even runs: 64
+# requests of 0 to 4,095 keys and 4 KV heads 33 us where two blocks a pair take 38, 48 of 8,192 keys and 8 KV heads 109 where one takes
+# 113; histories of 300 and 1,024 keys are better off with a block a pair (30 and 12 us for 38 and 15).
+Q4_RUNS_FROM, Q4_RUNS_KEYS = 1.0, 1024
+Q4_RUNS_ENTRIES = 1024      # kRunEntries in attention_q4.cu
 
 
 @functools.lru_cache(maxsize=4096)
-def q4_shares(num_entries: int, num_head_tiles: int, seen: int, sm_count: int) -> int:
-    """How many blocks share an entry's keys in a step of single tokens over packed pages, `seen` of them at most: the power of two up to
-    16 (a cluster's blocks) that a model of the launch's time likes best, whole waves of blocks and then what is left."""
-    base, slots, best = num_entries * num_head_tiles, Q4_BLOCKS_PER_SM * sm_count, None
+def q4_shares(pairs: int, seen: int, sm_count: int, runs: bool = True) -> int:
+    """How many blocks share the keys of one of `pairs` (entry, KV head) pairs in a step of single tokens over packed pages, `seen` keys at
+    most: the power of two up to 16 (a cluster's blocks) that a model of the launch's time likes best; 0 (where `runs` allows it): all
+    pairs' keys are dealt out in even runs."""
+    if runs and pairs >= Q4_RUNS_FROM * sm_count and seen > Q4_RUNS_KEYS:
+        return 0
+    slots, best = Q4_BLOCKS_PER_SM * sm_count, None
     for shares in (1, 2, 4, 8, 16):
         units = -(-seen // (128 * shares))
-        full, rest = divmod(base * shares, slots)
+        full, rest = divmod(pairs * shares, slots)
         time = full * (Q4_BLOCK_FIXED + units * Q4_BLOCK_KEYS[3])
         if rest:
             time += Q4_BLOCK_FIXED + units * Q4_BLOCK_KEYS[-(-rest // sm_count)]
@@ -1264,17 +1272,22 @@ def q4_shares(num_entries: int, num_head_tiles: int, seen: int, sm_count: int) -
     return best[1]
 
 
-def _attention_q4_decode(q, out, pages, *, positions, block_table, num_heads, num_kv_heads, head_dim, scale, max_keys, entry_starts,
+def _attention_q4_decode(q, out, pages, *, positions, block_table, num_heads, num_kv_heads, head_dim, scale, max_keys, workspace, entry_starts,
                          window, keep_first, sink, sink_values, gate, gate_offset, gate_per_head) -> None:
     fn = _function("attention_q4", "vipera_attention_q4_decode",
-                   [ctypes.POINTER(_DecodeQ4Params), _c_void])
+                   [ctypes.POINTER(_DecodeQ4Params), _c_void, ctypes.c_size_t, _c_int, _c_void])
     _check_struct("attention_q4", "vipera_attention_q4_params_size", _DecodeQ4Params)
     entries = block_table.shape[0]
     here, int32, what = torch.cuda.current_device(), torch.int32, "attention_q4"
     width = block_table.shape[1]
     group = num_heads // num_kv_heads
-    shares = q4_shares(entries, num_kv_heads * -(-group // (8 if group <= 8 else 16)),
-                       min(max_keys, window + keep_first) if window else max_keys, _sm_count_of(here))
+    wide = group > 8            # a block has 8 query heads, or 16
+    shares = q4_shares(entries * num_kv_heads * -(-group // (16 if wide else 8)),
+                       min(max_keys, window + keep_first) if window else max_keys, _sm_count_of(here), entries <= Q4_RUNS_ENTRIES)
+    parts = runs = None
+    if not shares:
+        runs = (2 if wide else Q4_BLOCKS_PER_SM) * _sm_count_of(here)
+        parts = workspace.get("attention.partials", (runs * 2 * (16 if wide else 8) * (head_dim + 4),), torch.float32)
     gate_pointer, gate_stride = (None, 0) if gate is None else _gate_pointer(
         gate, gate_offset, q.shape[0], num_heads * (1 if gate_per_head else head_dim), what)
     p = _DecodeQ4Params(_place(what, q, torch.bfloat16, here), _place(what, out, torch.bfloat16, here), *_place_pages(what, pages, here),
@@ -1283,7 +1296,10 @@ def _attention_q4_decode(q, out, pages, *, positions, block_table, num_heads, nu
                         None if sink_values is None else _place(what, sink_values, torch.float32, here), gate_pointer, gate_stride,
                         1 if gate_per_head else 0, width, pages.k_codes.shape[2], 0, pages.k_codes.shape[0], entries,
                         num_heads, num_kv_heads, head_dim, scale, window, keep_first, 1 if sink else 0, shares, 0)
-    _check(fn(p, _stream_of(here)), "attention_decode")
+    if shares:
+        _check(fn(p, None, 0, 0, _stream_of(here)), "attention_decode")
+    else:
+        _check(fn(p, parts.data_ptr(), parts.numel(), runs, _stream_of(here)), "attention_decode", kernels=2)
 
 
 Q4_ROWS = {(torch.float32, 128): 8, (torch.float32, 64): 16, (torch.bfloat16, 128): 16, (torch.bfloat16, 64): 16}   # (token, head) rows of a block
@@ -1375,7 +1391,7 @@ def attention_q4(q: torch.Tensor, out: torch.Tensor, pages: Q4Pages, *, entry_st
                    gate_per_head=gate_per_head)
     packed = attention_q4_takes_decode(q.dtype, head_dim, page_size)
     if packed and all_single:
-        _attention_q4_decode(q, out, pages, positions=positions, block_table=block_table, max_keys=max_keys,
+        _attention_q4_decode(q, out, pages, positions=positions, block_table=block_table, max_keys=max_keys, workspace=workspace,
                              entry_starts=None, **heads, **endings)
         return
     if attention_q4_takes_rows(q.dtype, head_dim, page_size, count * num_heads, num_heads, 1 if any_single else entries):
@@ -1399,7 +1415,7 @@ def attention_q4(q: torch.Tensor, out: torch.Tensor, pages: Q4Pages, *, entry_st
     attention_prefill(q, out, k_room, v_room, entry_starts=entry_starts, entry_pos0=entry_pos0, block_table=block_table,
                       num_entries=entries, skip_single=apart, **heads, **endings)
     if apart:
-        _attention_q4_decode(q, out, pages, positions=entry_pos0, block_table=block_table, max_keys=max_keys,
+        _attention_q4_decode(q, out, pages, positions=entry_pos0, block_table=block_table, max_keys=max_keys, workspace=workspace,
                              entry_starts=entry_starts, **heads, **endings)
 
 
