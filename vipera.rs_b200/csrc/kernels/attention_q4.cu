@@ -16,8 +16,8 @@
 //            begins at -8 times the sum of the query's channels and which the key's scale multiplies in 32 bits:
 //            s[key, head] = sum_g scale[key, g] (c[key, g, :] . q[head, g, :]).  The products' sums are as exact as if the codes
 //            were 2^10: off by 2^-22 of that.
-//   values   codes become bfloat16 by a shift, a mask and an OR (0x4300 | u is 128 + u, 136 above the code); the weights take the scales, w[key, head, g] = p[key, head] scale[key, g], rounded to bfloat16 a second time (half a
-//            step of the weight, as p itself): 2 products of pairs a group in the place of 16 on the codes; a product with
+//   values   codes become bfloat16 by a shift, a mask and an OR (0x4300 | u is 128 + u, 136 above the code); the weights take the
+//            scales in 32 bits, w[key, head, g] = p[key, head] scale[key, g], and are rounded to bfloat16 once; a product with
 //            ones sums them, and 136 times that sum goes off at the end.
 // A score's accumulators have the keys on their rows, the second product wants them on its inner axis: movmatrix turns the
 // weights' 8 x 8 blocks in registers, so nothing passes through shared memory until the end.
@@ -51,10 +51,6 @@ constexpr int kWarps = 4;
 constexpr int kWarpKeys = 32;   // keys a warp folds at a time: two tiles of 16
 constexpr int kStages = 3;      // such pairs of tiles on their way to shared memory for each warp
 
-__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
-  const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
 // The codes at bits 4 j and 16 + 4 j of a word as two bfloat16, 128 + u each.  `magic` is 0x43004300 from a parameter: a constant
 // would be an instruction's immediate beside the mask's, and two do not fit into one.
 __device__ __forceinline__ uint32_t codes_of(uint32_t word, int j, uint32_t magic) { return ((word >> (4 * j)) & 0x000f000fu) | magic; }
@@ -472,43 +468,38 @@ __device__ __forceinline__ void walk(const DecodeParams& p, const Shared<D, NT> 
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      uint32_t v[4][G / 2], scale[4][G / 2];     // of keys 4 n + t: a unit of 16 bits a group, and a scale
+      uint32_t v[4][G / 2], scale[2][G / 2];     // of keys 4 n + t: a unit of 16 bits a group; the scales of rows g and g + 8
 #pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        load_words<G / 2>(v[n], from.v[i] + v_from + 4 * n * kRowBytes);
-        load_words<G / 2>(scale[n], from.v_scale[i] + (4 * n + t) * (G * 2));
-      }
+      for (int n = 0; n < 4; ++n) load_words<G / 2>(v[n], from.v[i] + v_from + 4 * n * kRowBytes);
+#pragma unroll
+      for (int r = 0; r < 2; ++r) load_words<G / 2>(scale[r], from.v_scale[i] + (row_key + 8 * r) * (G * 2));
       if (!whole) {   // a hidden key's weight is 0, and its scale must not make that NaN
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          if (tile0 + i >= tiles_end || seen.hides(tile0 + i, seen.key_of(tile0 + i) + 4 * n + t)) {
+        for (int r = 0; r < 2; ++r) {
+          if (tile0 + i >= tiles_end || seen.hides(tile0 + i, seen.key_of(tile0 + i) + 8 * r + row_key)) {
 #pragma unroll
-            for (int w = 0; w < G / 2; ++w) scale[n][w] = 0;
+            for (int w = 0; w < G / 2; ++w) scale[r][w] = 0;
           }
         }
       }
-      uint32_t w[NT][2];      // weights of head g: keys t, 4 + t and 8 + t, 12 + t
+      float weight[NT][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float weight[4];
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          weight[c] = exp2_near(s[i][nt][c] - base[nt][c & 1]);
-          sum[nt][c & 1] += weight[c];
+          weight[nt][c] = exp2_near(s[i][nt][c] - base[nt][c & 1]);
+          sum[nt][c & 1] += weight[nt][c];
         }
-        w[nt][0] = turn_8x8(pack_bf16(weight[0], weight[1]));
-        w[nt][1] = turn_8x8(pack_bf16(weight[2], weight[3]));
-      }
 #pragma unroll
       for (int gr = 0; gr < G; ++gr) {
         const uint32_t pick = gr & 1 ? 0x7632u : 0x5410u;
-        uint32_t pairs[2], b[NT][2];
+        uint32_t pairs[2], b[NT][2];      // b: scaled weights of head g, of keys t, 4 + t and of 8 + t, 12 + t
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           pairs[r] = __byte_perm(v[2 * r][gr / 2], v[2 * r + 1][gr / 2], pick);
-          const uint32_t scales = __byte_perm(scale[2 * r][gr / 2], scale[2 * r + 1][gr / 2], pick);
+          const float x = gr & 1 ? high_of(scale[r][gr / 2]) : low_of(scale[r][gr / 2]);
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) b[nt][r] = mul_bf16x2(w[nt][r], scales);
+          for (int nt = 0; nt < NT; ++nt) b[nt][r] = turn_8x8(pack_bf16(weight[nt][2 * r] * x, weight[nt][2 * r + 1] * x));
         }
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
