@@ -74,13 +74,13 @@ def make_pages(num_pages, page_size, kv_heads, d, seed, device="cpu"):
 
 
 def attend(q, k_rows, v_rows, *, counts, history, tables, page_size, num_heads, num_kv_heads, d, scale, window=0, keep_first=0,
-           sink=False, sink_values=None, gate=None, v_steps=None):
+           sink=False, sink_values=None, gate=None, k_steps=None, v_steps=None):
     """(output [tokens, heads, d], parts): `parts` is what errors of the run's arithmetic are multiples of, for each output or head:
     ``spread`` sum_j p_j |v_j| / l, ``steps`` the same with the values' scales in the place of |v|, ``reach`` the largest sum over
-    channels of |q k| scale that a score of the row has, ``flat`` the same with the head's largest |q| in the place of |q|."""
+    channels of |q k| scale that a score of the row has, ``full`` the same with 16 steps of the key's groups in the place of |k|."""
     q = np.asarray(q, dtype=np.float64).reshape(-1, num_heads, d)
     out, spread, steps = np.zeros_like(q), np.zeros_like(q), np.zeros_like(q)
-    reach, flat = np.zeros(q.shape[:2]), np.zeros(q.shape[:2])
+    reach, full = np.zeros(q.shape[:2]), np.zeros(q.shape[:2])
     token = 0
     for e, (count, held) in enumerate(zip(counts, history)):
         for i in range(count):
@@ -102,28 +102,29 @@ def attend(q, k_rows, v_rows, *, counts, history, tables, page_size, num_heads, 
                 if v_steps is not None:
                     steps[token, h] = np.repeat(p @ np.abs(v_steps[page, kv, place]) / total, GROUP)
                 reach[token, h] = (np.abs(k) @ np.abs(q[token, h])).max() * scale
-                flat[token, h] = np.abs(k).sum(-1).max() * np.abs(q[token, h]).max() * scale
+                if k_steps is not None:
+                    full[token, h] = (np.abs(k_steps[page, kv, place]) @ np.abs(q[token, h]).reshape(-1, GROUP).sum(-1)).max() * 16 * scale
             if gate is not None:
                 factor = 1 / (1 + np.exp(-np.asarray(gate[token], dtype=np.float64).reshape(num_heads, -1)))
                 for part in (out, spread, steps):
                     part[token] *= factor
             token += 1
-    return out, dict(spread=spread, steps=steps, reach=reach, flat=flat)
+    return out, dict(spread=spread, steps=steps, reach=reach, full=full)
 
 
 def allowed(out, parts, keys, d, dtype):
     """How far each output may be off.  Scores are sums of d products and weights and sums run over `keys` keys in 32 bits, a product
     or sum off by 2^-24 of its size, on tensor cores by 2^-22: a score by (d + 8) of these times its reach, a weight and the sum by e
     to that, a sum by one for each key.  2^-30 is for outputs next to 0.  In bfloat16 further:
-    a weight is rounded twice at most (itself and times the scale) and the output once, each by half a step, 2^-8;
-    a channel of the query is the sum of two numbers of 8 bits, within 2^-17 of the head's largest, a score within that of `flat`, a
-    weight and the sum (twice) too;
+    a weight (times the scale, where it is taken there) is rounded once and the output once, each by half a step, 2^-8;
+    codes c meet the query as c + 8, below 16, in half precision's smallest numbers, whose products' sums the tensor cores were seen to
+    have off by 2^-16.7 of their terms' sizes: a score by 2^-16 of `full`, a weight and the sum by e to that;
     values are summed as codes + 136 (144 steps at most) with 136 times the weights' sum taken off: of the 2^-20 that a product of
     17 terms may be off, one for each 16 keys that a warp walks (a quarter of its block's) and four to join the parts."""
     unit = 2.0 ** -22
     relative = 2 * (d + 8) * parts["reach"] * unit + 2 * (keys + 16) * unit
     if dtype == torch.bfloat16:
-        relative = relative + 2 * 2.0 ** -17 * parts["flat"]
-        return (parts["spread"] * (2 * 2.0 ** -8 + 2.0 ** -15 + relative[..., None]) + np.abs(out) * 2.0 ** -8
+        relative = relative + 2 * 2.0 ** -16 * parts["full"]
+        return (parts["spread"] * (2.0 ** -8 + 2.0 ** -15 + relative[..., None]) + np.abs(out) * 2.0 ** -8
                 + parts["steps"] * (keys / 64 + 4) * 144 * 2.0 ** -20 + 2.0 ** -30)
     return parts["spread"] * relative[..., None] + 2.0 ** -30

@@ -212,7 +212,7 @@ def _attend(ops, step, dtype, heads, kv_heads, d, seed=0, window=0, keep_first=0
             gate_per_head=False, workspace=None):
     raw = plain.make_pages(step.num_pages, step.page_size, kv_heads, d, seed + 10, DEVICE)
     k_rows, v_rows = plain.rows_of(raw[0], raw[1], True), plain.rows_of(raw[2], raw[3], False)
-    v_steps = raw[3].double().cpu().numpy()
+    k_steps, v_steps = raw[1].double().cpu().numpy(), raw[3].double().cpu().numpy()
     pages = ops.Q4Pages(*raw)
     tables = [list(row) for row in step.tables]
     _hide(step, pages, window, keep_first)
@@ -228,7 +228,7 @@ def _attend(ops, step, dtype, heads, kv_heads, d, seed=0, window=0, keep_first=0
                      gate=gates, gate_offset=4, gate_per_head=gate_per_head, **step.device())
     expected, parts = plain.attend(q.double().numpy(), k_rows, v_rows, counts=step.counts, history=step.history, tables=tables,
                                    page_size=step.page_size, num_heads=heads, num_kv_heads=kv_heads, d=d, scale=scale, window=window,
-                                   keep_first=keep_first, sink=sink, sink_values=sink_values, gate=gate, v_steps=v_steps)
+                                   keep_first=keep_first, sink=sink, sink_values=sink_values, gate=gate, k_steps=k_steps, v_steps=v_steps)
     got = out[:tokens].double().cpu().numpy().reshape(expected.shape)
     keys = max(c + h for c, h in zip(step.counts, step.history))
     limit = plain.allowed(expected, parts, keys, d, dtype)
@@ -445,6 +445,7 @@ def test_a_step_as_it_is_used_eager_captured_and_on_a_stream_of_its_own(ops):
     q = torch.from_numpy(q.reshape(3, -1)).to(torch.bfloat16).double().numpy()
     tables = [list(table_pages[e * 10:e * 10 + 4]) for e in range(3)]
     expected, parts = plain.attend(q, k_rows, v_rows, counts=[1, 1, 1], history=held, tables=tables, page_size=page, num_heads=heads,
-                                   num_kv_heads=kv_heads, d=d, scale=d ** -0.5, v_steps=pages.v_scales.double().cpu().numpy())
+                                   num_kv_heads=kv_heads, d=d, scale=d ** -0.5, k_steps=pages.k_scales.double().cpu().numpy(),
+                                   v_steps=pages.v_scales.double().cpu().numpy())
     limit = plain.allowed(expected, parts, 64, d, torch.bfloat16)
     assert (np.abs(outs[3].double().cpu().numpy().reshape(expected.shape) - expected) <= limit).all()

@@ -788,6 +788,19 @@ __global__ void __launch_bounds__(128) attention_q4_join_kernel(DecodeParams p, 
   }
 }
 
+// Shared memory beyond 48 KB and clusters of 16 blocks are asked for once on every device (a bit each in `asked`).
+template <typename Kernel>
+int ask_once(uint64_t* asked, Kernel kernel, int shared_bytes, bool clusters) {
+  int device = 0;
+  cudaError_t error = cudaGetDevice(&device);
+  if (error == cudaSuccess && device < 64 && (*asked >> device & 1u)) return VIPERA_OK;
+  if (error == cudaSuccess) error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared_bytes);
+  if (error == cudaSuccess && clusters) error = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (error != cudaSuccess) return static_cast<int>(error);
+  if (device < 64) *asked |= 1ull << device;
+  return VIPERA_OK;
+}
+
 template <int D, int NT>
 int launch(const DecodeParams& p, float* parts, int runs, cudaStream_t s) {
   constexpr int kSmem = Shared<D, NT>::kBytes;
@@ -795,20 +808,17 @@ int launch(const DecodeParams& p, float* parts, int runs, cudaStream_t s) {
   if (p.num_kv_heads * head_tiles > 65535) return VIPERA_BAD_SHAPE;
   if (p.shares == 0) {
     const auto kernel = attention_q4_runs_kernel<D, NT>;
-    cudaError_t error = cudaSuccess;     // every device has to be asked
-    if (kSmem > 48 * 1024) error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
-    if (error == cudaSuccess) error = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
-    if (error != cudaSuccess) return static_cast<int>(error);
+    static uint64_t asked = 0;
+    const int ready = ask_once(&asked, kernel, kSmem, false);
+    if (ready != VIPERA_OK) return ready;
     const int status = vipera_launch(kernel, dim3(runs), 32 * kWarps, kSmem, s, p, parts);
     if (status != VIPERA_OK) return status;
     return vipera_launch(attention_q4_join_kernel<D, NT>, dim3(p.num_entries, p.num_kv_heads * head_tiles), 128, 0, s, p, parts, runs);
   }
   const auto kernel = attention_q4_cluster_kernel<D, NT>;
-  cudaError_t error = cudaSuccess;
-  if (kSmem > 48 * 1024) error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
-  if (error == cudaSuccess) error = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
-  if (error == cudaSuccess && p.shares > 8) error = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  if (error != cudaSuccess) return static_cast<int>(error);
+  static uint64_t asked = 0;
+  const int ready = ask_once(&asked, kernel, kSmem, true);
+  if (ready != VIPERA_OK) return ready;
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(p.num_entries, p.num_kv_heads * head_tiles, p.shares);
   config.blockDim = dim3(32 * kWarps);
@@ -823,7 +833,7 @@ int launch(const DecodeParams& p, float* parts, int runs, cudaStream_t s) {
   attributes[1].val.clusterDim.z = static_cast<unsigned>(p.shares);
   config.attrs = attributes;
   config.numAttrs = 2;
-  error = cudaLaunchKernelEx(&config, kernel, p);
+  const cudaError_t error = cudaLaunchKernelEx(&config, kernel, p);
   return error == cudaSuccess ? VIPERA_OK : static_cast<int>(error);
 }
 

@@ -73,23 +73,78 @@ struct StoreParams {
   int num_tokens, num_heads, num_kv_heads, head_dim, rot_dims, style, page_size;
 };
 
-// One thread: eight neighbouring channels of a head of a token; four neighbouring threads: a group.  A group is in one warp
-// because a head has a multiple of four such octets.  VEC: rows start on 16 bytes and the rotation's halves are
-// whole octets, so that an octet and its partner are fetched in pieces of 16 bytes.
-// Every product and sum of the rotation is rounded by itself (no fused multiply-add), so that a key next to a
-// border between two codes falls the same way wherever the rotation is computed in 32 bits.
+// Where a token's rows of a KV head go.
+struct Row {
+  bool write;
+  size_t row;
+};
+__device__ __forceinline__ Row row_of(const StoreParams& p, int slot, int kv_head) {
+  const bool write = slot >= 0 && slot < p.num_slots;
+  const int page = write ? slot / p.page_size : 0, place = write ? slot - page * p.page_size : 0;
+  return Row{write, (static_cast<size_t>(page) * p.num_kv_heads + kv_head) * p.page_size + place};
+}
+
+// An octet of a head on its way: queries to their type, keys and values to codes.  Four neighbouring lanes hold a group of 32 channels and
+// find its ends together; every lane of the warp takes part.
+template <typename T>
+__device__ __forceinline__ void put_octet(const StoreParams& p, const float (&x)[8], int t, int h, int octet, bool live, const Row& to) {
+  const bool is_q = h < p.num_heads, is_v = h >= p.num_heads + p.num_kv_heads;
+  if (live && is_q) {
+    T* q = static_cast<T*>(p.q_out) + (static_cast<size_t>(t) * p.num_heads + h) * p.head_dim + octet * 8;
+    store_four_as<T>(q, x[0], x[1], x[2], x[3]);
+    store_four_as<T>(q + 4, x[4], x[5], x[6], x[7]);
+  }
+  if (!__any_sync(0xffffffffu, live && !is_q && to.write)) return;
+  float high = x[0], low = x[0];
+  bool fine = true;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    high = fmaxf(high, x[i]);
+    low = fminf(low, x[i]);
+    fine = fine && fabsf(x[i]) <= 3.402823466e38f;
+  }
+#pragma unroll
+  for (int offset = 1; offset <= 2; offset <<= 1) {
+    high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, offset));
+    low = fminf(low, __shfl_xor_sync(0xffffffffu, low, offset));
+    fine = __shfl_xor_sync(0xffffffffu, static_cast<int>(fine), offset) && fine;
+  }
+  if (!live || is_q || !to.write) return;
+  const float scale = fine ? q4::round5((high >= -low ? high : low) * -0.125f) : __int_as_float(0x7fffffff);
+  uint32_t code[8];
+  q4::codes_of(x, scale, code);
+  const int groups = p.head_dim / q4::kGroup, g = octet >> 2, quarter = octet & 3;
+  if (quarter == 0) (is_v ? p.v_scales : p.k_scales)[to.row * groups + g] = __float2bfloat16_rn(scale);
+  if (is_v) {
+    uint16_t* units = reinterpret_cast<uint16_t*>(p.v_codes) + to.row * (p.head_dim / 4);
+    units[(2 * quarter) * groups + g] = static_cast<uint16_t>(code[0] | code[1] << 4 | code[2] << 8 | code[3] << 12);
+    units[(2 * quarter + 1) * groups + g] = static_cast<uint16_t>(code[4] | code[5] << 4 | code[6] << 8 | code[7] << 12);
+  } else {
+    reinterpret_cast<uint32_t*>(p.k_codes)[to.row * (p.head_dim >> 3) + quarter * groups + g] =
+        code[0] | code[2] << 4 | code[4] << 8 | code[6] << 12 | (code[1] | code[3] << 4 | code[5] << 8 | code[7] << 12) << 16;
+  }
+}
+
+__device__ __forceinline__ void load_octet(float (&x)[8], const float* from) {
+  *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(from);
+  *reinterpret_cast<float4*>(x + 4) = *reinterpret_cast<const float4*>(from + 4);
+}
+
+// A thread has an octet of a head of a token.  Every product and sum of the rotation is rounded by itself (no fused multiply-add), so that a
+// key next to a border between two codes falls the same way wherever the rotation is computed in 32 bits.  VEC: rows start on 16 bytes
+// and the rotation's halves are whole octets.
+// 2,048 tokens of 28 + 2 x 4 heads of 128: 17 us, bound by instructions (38 MB read, 16 MB written); an octet of both halves a thread, which
+// reads the row and the tables once, takes 19 us, and two or four heads a thread 20 to 21 (fewer threads, longer chains).
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) rope_cache_q4_kernel(StoreParams p) {
   pdl_launch_dependents();
   pdl_wait();
   const int octets = p.head_dim >> 3;
   const int all_heads = p.num_heads + 2 * p.num_kv_heads;
-  const long long items = static_cast<long long>(p.num_tokens) * all_heads * octets;
-  const long long item = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
-  const bool live = item < items;
-  const int per_token = all_heads * octets;
+  const uint32_t item = blockIdx.x * blockDim.x + threadIdx.x, per_token = all_heads * octets;     // the launcher keeps them below 2^31
+  const bool live = item < static_cast<uint32_t>(p.num_tokens) * per_token;
   const int t = live ? static_cast<int>(item / per_token) : 0;
-  const int rest = live ? static_cast<int>(item - static_cast<long long>(t) * per_token) : 0;
+  const int rest = live ? static_cast<int>(item - static_cast<uint32_t>(t) * per_token) : 0;
   const int h = rest / octets, octet = rest - h * octets, c0 = octet * 8;
   const bool is_q = h < p.num_heads, is_v = h >= p.num_heads + p.num_kv_heads;
   const float* head = p.qkv + static_cast<size_t>(t) * p.row_stride + static_cast<size_t>(h) * p.head_dim;
@@ -99,8 +154,7 @@ __global__ void __launch_bounds__(256) rope_cache_q4_kernel(StoreParams p) {
   const size_t table_row = static_cast<size_t>(max(min(position, p.table_rows - 1), 0)) * half;
   float x[8];
   if (VEC) {
-    *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(head + c0);
-    *reinterpret_cast<float4*>(x + 4) = *reinterpret_cast<const float4*>(head + c0 + 4);
+    load_octet(x, head + c0);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = head[c0 + i];
@@ -120,12 +174,9 @@ __global__ void __launch_bounds__(256) rope_cache_q4_kernel(StoreParams p) {
       const bool low = c0 < half;
       const int i0 = low ? c0 : c0 - half, other = low ? c0 + half : c0 - half;
       float y[8], c[8], s[8];
-#pragma unroll
-      for (int i = 0; i < 8; i += 4) {
-        *reinterpret_cast<float4*>(y + i) = *reinterpret_cast<const float4*>(head + other + i);
-        *reinterpret_cast<float4*>(c + i) = *reinterpret_cast<const float4*>(p.cos_table + table_row + i0 + i);
-        *reinterpret_cast<float4*>(s + i) = *reinterpret_cast<const float4*>(p.sin_table + table_row + i0 + i);
-      }
+      load_octet(y, head + other);
+      load_octet(c, p.cos_table + table_row + i0);
+      load_octet(s, p.sin_table + table_row + i0);
 #pragma unroll
       for (int i = 0; i < 8; ++i)
         x[i] = low ? __fsub_rn(__fmul_rn(x[i], c[i]), __fmul_rn(y[i], s[i]))
@@ -144,44 +195,7 @@ __global__ void __launch_bounds__(256) rope_cache_q4_kernel(StoreParams p) {
       }
     }
   }
-  if (live && is_q) {
-    T* to = static_cast<T*>(p.q_out) + (static_cast<size_t>(t) * p.num_heads + h) * p.head_dim + c0;
-    store_four_as<T>(to, x[0], x[1], x[2], x[3]);
-    store_four_as<T>(to + 4, x[4], x[5], x[6], x[7]);
-  }
-  // the group's ends, over the four threads that hold it (all lanes take part)
-  float high = x[0], low = x[0];
-  bool fine = true;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    high = fmaxf(high, x[i]);
-    low = fminf(low, x[i]);
-    fine = fine && fabsf(x[i]) <= 3.402823466e38f;
-  }
-#pragma unroll
-  for (int offset = 1; offset <= 2; offset <<= 1) {
-    high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, offset));
-    low = fminf(low, __shfl_xor_sync(0xffffffffu, low, offset));
-    fine = __shfl_xor_sync(0xffffffffu, static_cast<int>(fine), offset) && fine;
-  }
-  if (!live || is_q || slot < 0 || slot >= p.num_slots) return;
-  const float scale = fine ? q4::round5((high >= -low ? high : low) * -0.125f) : __int_as_float(0x7fffffff);
-  uint32_t code[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) code[i] = q4::code_of(x[i], scale);
-  const int groups = p.head_dim / q4::kGroup, g = octet >> 2, quarter = octet & 3;
-  const int kv_head = h - p.num_heads - (is_v ? p.num_kv_heads : 0);
-  const int page = slot / p.page_size, place = slot - page * p.page_size;
-  const size_t row = (static_cast<size_t>(page) * p.num_kv_heads + kv_head) * p.page_size + place;
-  if (quarter == 0) (is_v ? p.v_scales : p.k_scales)[row * groups + g] = __float2bfloat16_rn(scale);
-  if (is_v) {
-    uint16_t* units = reinterpret_cast<uint16_t*>(p.v_codes) + row * (p.head_dim / 4);
-    units[(2 * quarter) * groups + g] = static_cast<uint16_t>(code[0] | code[1] << 4 | code[2] << 8 | code[3] << 12);
-    units[(2 * quarter + 1) * groups + g] = static_cast<uint16_t>(code[4] | code[5] << 4 | code[6] << 8 | code[7] << 12);
-  } else {
-    reinterpret_cast<uint32_t*>(p.k_codes)[row * octets + quarter * groups + g] =
-        code[0] | code[2] << 4 | code[4] << 8 | code[6] << 12 | (code[1] | code[3] << 4 | code[5] << 8 | code[7] << 12) << 16;
-  }
+  put_octet<T>(p, x, t, h, octet, live, row_of(p, slot, max(h - p.num_heads - (is_v ? p.num_kv_heads : 0), 0)));
 }
 
 // ---------------------------------------------------------------------------------------
@@ -213,9 +227,26 @@ __device__ __forceinline__ Seen seen_by(const ExpandParams& p, int e) {
   return s;
 }
 
-// A unit of work is the keys, or the values, of one page of one entry.  Every block counts the units of all entries for itself
-// (two trips to memory and a scan), then takes every gridDim-th: the load is even however the lengths differ, and
-// the launch needs no count from the host, so that a captured one serves any lengths.
+// Eight channels of a row as numbers.
+__device__ __forceinline__ void key_octet(float (&x)[8], uint32_t w, float scale) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    x[2 * j] = static_cast<float>(static_cast<int>((w >> (4 * j)) & 15u) - 8) * scale;
+    x[2 * j + 1] = static_cast<float>(static_cast<int>((w >> (16 + 4 * j)) & 15u) - 8) * scale;
+  }
+}
+__device__ __forceinline__ void value_octet(float (&x)[8], uint32_t lo, uint32_t hi, float scale) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    x[j] = static_cast<float>(static_cast<int>((lo >> (4 * j)) & 15u) - 8) * scale;
+    x[4 + j] = static_cast<float>(static_cast<int>((hi >> (4 * j)) & 15u) - 8) * scale;
+  }
+}
+
+// A unit of work is one page of one entry.  Every block counts the units of all entries for itself (two trips to memory and a scan),
+// then takes every gridDim-th: the load is even however the lengths differ, and the launch needs no count from the host, so that
+// a captured one serves any lengths.  A thread has an octet of the keys and the same of the values, kAhead rows of them at once.
+constexpr int kAhead = 4;
 template <typename T>
 __global__ void __launch_bounds__(256) expand_q4_kernel(ExpandParams p) {
   __shared__ int ends[kSlab];      // pages up to and with this entry
@@ -263,9 +294,7 @@ __global__ void __launch_bounds__(256) expand_q4_kernel(ExpandParams p) {
       ends[threadIdx.x * 4 + i] = before;
     }
     __syncthreads();
-    for (long long unit = blockIdx.x; unit < 2LL * total; unit += gridDim.x) {
-      const int index = static_cast<int>(unit >> 1);
-      const bool keys = (unit & 1) == 0;
+    for (int index = blockIdx.x; index < total; index += gridDim.x) {
       int low = 0, high = entries - 1;      // the first entry whose end is above index
       while (low < high) {
         const int middle = (low + high) >> 1;
@@ -280,37 +309,39 @@ __global__ void __launch_bounds__(256) expand_q4_kernel(ExpandParams p) {
       const int at = within < kept_pages ? within : first_page + within - kept_pages;
       const int page = p.block_table[static_cast<size_t>(e) * p.table_width + at];
       if (page < 0 || page >= p.num_pages) continue;
-      const uint8_t* codes = keys ? p.k_codes : p.v_codes;
-      const __nv_bfloat16* scales = keys ? p.k_scales : p.v_scales;
-      T* room = static_cast<T*>(keys ? p.k_room : p.v_room);
-      for (int i = threadIdx.x; i < per_unit; i += blockDim.x) {
-        const int head_row = i / octets, octet = i - head_row * octets;
-        const int place = head_row / p.num_kv_heads, kv_head = head_row - place * p.num_kv_heads;
-        const int position = at * p.page_size + place;
-        if (!((position >= s.first && position <= s.last) || position < s.kept)) continue;
-        const size_t row = (static_cast<size_t>(page) * p.num_kv_heads + kv_head) * p.page_size + place;
-        const int g = octet >> 2, quarter = octet & 3;
-        const float scale = __bfloat162float(scales[row * groups + g]);
-        float x[8];
-        if (keys) {
-          const uint32_t w = reinterpret_cast<const uint32_t*>(codes)[row * octets + quarter * groups + g];
+      const size_t page_row = static_cast<size_t>(page) * p.num_kv_heads * p.page_size;
+      for (int i0 = threadIdx.x; i0 < per_unit; i0 += kAhead * blockDim.x) {
+        uint32_t k[kAhead], v_lo[kAhead], v_hi[kAhead];
+        float k_scale[kAhead], v_scale[kAhead];
+        size_t to[kAhead];
+        bool seen[kAhead];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            x[2 * j] = static_cast<float>(static_cast<int>((w >> (4 * j)) & 15u) - 8) * scale;
-            x[2 * j + 1] = static_cast<float>(static_cast<int>((w >> (16 + 4 * j)) & 15u) - 8) * scale;
-          }
-        } else {
-          const uint16_t* units = reinterpret_cast<const uint16_t*>(codes) + row * (p.head_dim / 4);
-          const uint32_t lo = units[(2 * quarter) * groups + g], hi = units[(2 * quarter + 1) * groups + g];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            x[j] = static_cast<float>(static_cast<int>((lo >> (4 * j)) & 15u) - 8) * scale;
-            x[4 + j] = static_cast<float>(static_cast<int>((hi >> (4 * j)) & 15u) - 8) * scale;
-          }
+        for (int c = 0; c < kAhead; ++c) {     // rows of a KV head lie together in the page: (KV head, place, octet)
+          const int i = i0 + c * blockDim.x;
+          const int row_in = i / octets, octet = i - row_in * octets, kv_head = row_in / p.page_size, place = row_in - kv_head * p.page_size;
+          const int position = at * p.page_size + place, g = octet >> 2, quarter = octet & 3;
+          seen[c] = i < per_unit && ((position >= s.first && position <= s.last) || position < s.kept);
+          if (!seen[c]) continue;
+          const size_t row = page_row + row_in;
+          k[c] = reinterpret_cast<const uint32_t*>(p.k_codes)[row * octets + quarter * groups + g];
+          const uint16_t* units = reinterpret_cast<const uint16_t*>(p.v_codes) + row * (p.head_dim / 4);
+          v_lo[c] = units[(2 * quarter) * groups + g];
+          v_hi[c] = units[(2 * quarter + 1) * groups + g];
+          k_scale[c] = __bfloat162float(p.k_scales[row * groups + g]);
+          v_scale[c] = __bfloat162float(p.v_scales[row * groups + g]);
+          to[c] = ((static_cast<size_t>(page) * p.page_size + place) * p.num_kv_heads + kv_head) * p.head_dim + octet * 8;
         }
-        T* to = room + ((static_cast<size_t>(page) * p.page_size + place) * p.num_kv_heads + kv_head) * p.head_dim + octet * 8;
-        store_four_as<T>(to, x[0], x[1], x[2], x[3]);
-        store_four_as<T>(to + 4, x[4], x[5], x[6], x[7]);
+#pragma unroll
+        for (int c = 0; c < kAhead; ++c) {
+          if (!seen[c]) continue;
+          float x[8];
+          key_octet(x, k[c], k_scale[c]);
+          store_four_as<T>(static_cast<T*>(p.k_room) + to[c], x[0], x[1], x[2], x[3]);
+          store_four_as<T>(static_cast<T*>(p.k_room) + to[c] + 4, x[4], x[5], x[6], x[7]);
+          value_octet(x, v_lo[c], v_hi[c], v_scale[c]);
+          store_four_as<T>(static_cast<T*>(p.v_room) + to[c], x[0], x[1], x[2], x[3]);
+          store_four_as<T>(static_cast<T*>(p.v_room) + to[c] + 4, x[4], x[5], x[6], x[7]);
+        }
       }
     }
     __syncthreads();
@@ -344,7 +375,7 @@ VIPERA_API int vipera_rope_cache_q4(const StoreParams* p, int dtype, void* strea
                    (p->style != ROPE_NEOX || half == 0 || (half % 8 == 0 && aligned(p->cos_table, 16) && aligned(p->sin_table, 16)));
   const long long items = static_cast<long long>(p->num_tokens) * (p->num_heads + 2 * p->num_kv_heads) * (p->head_dim / 8);
   const long long blocks = (items + 255) / 256;
-  if (blocks > 0x7fffffffLL) return VIPERA_BAD_SHAPE;
+  if (blocks > 0x7fffffLL) return VIPERA_BAD_SHAPE;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const dim3 grid(static_cast<unsigned>(blocks));
   if (dtype == VIPERA_BF16)

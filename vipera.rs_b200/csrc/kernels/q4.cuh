@@ -35,10 +35,26 @@ __device__ __forceinline__ float round5(float x) {
   return __uint_as_float((bits + 0x3FFFFu + ((bits >> 19) & 1u)) & 0xFFF80000u);
 }
 
-// The code (0 .. 15) of x in a group of scale s; a scale of 0 or NaN stands for itself whatever the code.
-__device__ __forceinline__ uint32_t code_of(float x, float s) {
-  const float c = fminf(fmaxf(rintf(__fdiv_rn(x, s)), -8.0f), 7.0f);
-  return (s == 0.0f || s != s) ? 8u : static_cast<uint32_t>(static_cast<int>(c) + 8);
+// The codes (0 .. 15) of eight values in a group of scale s; a scale of 0 or NaN stands for itself whatever the code.  A product with 1 / s
+// is near the quotient, and what is left of x beside that code's step, exact in 32 bits (x and the step are within a factor of two), says
+// whether the next code is nearer, or as near and even.  Scales whose reciprocal is not a number divide.
+__device__ __forceinline__ void codes_of(const float (&x)[8], float s, uint32_t (&code)[8]) {
+  const bool none = s == 0.0f || s != s, tiny = fabsf(s) < 0x1p-120f;
+  const float inverse = tiny ? 0.0f : __frcp_rn(s), half = 0.5f * fabsf(s);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float c;
+    if (tiny) {
+      c = none ? 0.0f : rintf(__fdiv_rn(x[i], s));
+    } else {
+      c = rintf(x[i] * inverse);
+      const float left = fmaf(-c, s, x[i]), away = copysignf(1.0f, left * s);
+      const bool odd = static_cast<int>(c) & 1;
+      if (fabsf(left) > half || (fabsf(left) == half && odd)) c += away;
+    }
+    c = fminf(fmaxf(c, -8.0f), 7.0f);
+    code[i] = none ? 8u : static_cast<uint32_t>(static_cast<int>(c) + 8);
+  }
 }
 
 }  // namespace q4

@@ -1101,6 +1101,15 @@ class _RowsQ4Params(ctypes.Structure):
                 ("keep_first", _c_int), ("chunk", _c_int), ("num_splits", _c_int)]
 
 
+# argument types of the launchers (a parameter block is handed over by reference)
+_MAPS_ARGS = [ctypes.POINTER(_MapsParams), _c_void]
+_STORE_Q4_ARGS = [ctypes.POINTER(_StoreQ4Params), _c_int, _c_void]
+_EXPAND_Q4_ARGS = [ctypes.POINTER(_ExpandQ4Params), _c_int, _c_int, _c_void]
+_DECODE_Q4_ARGS = [ctypes.POINTER(_DecodeQ4Params), _c_void, ctypes.c_size_t, _c_int, _c_void]
+_ROWS_Q4_ARGS = [ctypes.POINTER(_RowsQ4Params), _c_void, _c_int, _c_int, _c_void, _c_int, _c_void, _c_void, ctypes.c_longlong, _c_int,
+                 _c_void, ctypes.c_size_t, _c_void]
+
+
 def _place(what: str, tensor: torch.Tensor, dtype: torch.dtype, here: int) -> int:
     """The address of a contiguous tensor of `dtype` on device `here`, the current one, whose stream the launch goes to."""
     if tensor.dtype is not dtype or not tensor.is_contiguous() or tensor.get_device() != here:
@@ -1156,7 +1165,7 @@ def step_maps(entry_starts: torch.Tensor, entry_pos0: torch.Tensor, *, page_size
     left out) and, where given, per token its ``positions``, its ``token_entry`` and its ``slots``: page * page_size + place in
     the page, -1 where the entry holds no page for it.  Without ``pages`` the block table is read instead.  Tokens behind the last
     entry's are left as they were."""
-    fn = _function("cache_q4", "vipera_step_maps", [ctypes.POINTER(_MapsParams), _c_void])
+    fn = _function("cache_q4", "vipera_step_maps", _MAPS_ARGS)
     _check_struct("cache_q4", "vipera_step_maps_params_size", _MapsParams)
     entries = entry_pos0.numel()
     if entry_starts.numel() != entries + 1 or block_table.dim() != 2 or block_table.shape[0] != entries:
@@ -1184,7 +1193,7 @@ def rope_cache_q4(qkv: torch.Tensor, q_out: torch.Tensor, pages: Q4Pages, *, num
     page_size + place, from step_maps; a slot that is negative or outside the pool is not written).  Two tokens of a step do not
     share a slot.  ``slots=None`` writes q alone.  Positions lie inside the tables.  Every product and sum of the rotation is
     rounded by itself in 32 bits."""
-    fn = _function("cache_q4", "vipera_rope_cache_q4", [ctypes.POINTER(_StoreQ4Params), _c_int, _c_void])
+    fn = _function("cache_q4", "vipera_rope_cache_q4", _STORE_Q4_ARGS)
     _check_struct("cache_q4", "vipera_rope_cache_q4_params_size", _StoreQ4Params)
     page_size = _check_q4_pages("rope_cache_q4", pages, num_kv_heads, head_dim)
     rot_dims = head_dim if rot_dims is None else int(rot_dims)
@@ -1218,7 +1227,7 @@ def expand_q4(pages: Q4Pages, k_room: torch.Tensor, v_room: torch.Tensor, *, ent
     [pages, page_size, kv_heads, d] (bfloat16, which holds every row exactly, or float32), so that the block tables serve both.
     Other rows of the rooms stay as they are.  ``window`` and ``keep_first`` as for attention; ``skip_single`` leaves entries of one
     token out."""
-    fn = _function("cache_q4", "vipera_expand_q4", [ctypes.POINTER(_ExpandQ4Params), _c_int, _c_int, _c_void])
+    fn = _function("cache_q4", "vipera_expand_q4", _EXPAND_Q4_ARGS)
     _check_struct("cache_q4", "vipera_expand_q4_params_size", _ExpandQ4Params)
     if k_room.dim() != 4 or v_room.shape != k_room.shape or v_room.dtype != k_room.dtype:
         raise InvalidArgumentError("expand_q4: the rooms are [pages, page_size, kv_heads, d], of one type")
@@ -1274,8 +1283,7 @@ def q4_shares(pairs: int, seen: int, sm_count: int, runs: bool = True) -> int:
 
 def _attention_q4_decode(q, out, pages, *, positions, block_table, num_heads, num_kv_heads, head_dim, scale, max_keys, workspace, entry_starts,
                          window, keep_first, sink, sink_values, gate, gate_offset, gate_per_head) -> None:
-    fn = _function("attention_q4", "vipera_attention_q4_decode",
-                   [ctypes.POINTER(_DecodeQ4Params), _c_void, ctypes.c_size_t, _c_int, _c_void])
+    fn = _function("attention_q4", "vipera_attention_q4_decode", _DECODE_Q4_ARGS)
     _check_struct("attention_q4", "vipera_attention_q4_params_size", _DecodeQ4Params)
     entries = block_table.shape[0]
     here, int32, what = torch.cuda.current_device(), torch.int32, "attention_q4"
@@ -1332,9 +1340,7 @@ def q4_rows_splits(tiles: int, max_keys: int, sm_count: int):
 
 def _attention_q4_rows(q, out, pages, *, entry_starts, entry_pos0, positions, block_table, num_heads, num_kv_heads, head_dim, scale,
                        max_keys, workspace, window, keep_first, sink, sink_values, gate, gate_offset, gate_per_head) -> None:
-    fn = _function("attention_q4", "vipera_attention_q4_rows",
-                   [ctypes.POINTER(_RowsQ4Params), _c_void, _c_int, _c_int, _c_void, _c_int, _c_void, _c_void, ctypes.c_longlong, _c_int,
-                    _c_void, ctypes.c_size_t, _c_void])
+    fn = _function("attention_q4", "vipera_attention_q4_rows", _ROWS_Q4_ARGS)
     _check_struct("attention_q4", "vipera_attention_q4_rows_params_size", _RowsQ4Params)
     here, int32, what = torch.cuda.current_device(), torch.int32, "attention_q4"
     count, entries, dtype = q.shape[0], entry_pos0.numel(), q.dtype
