@@ -92,9 +92,25 @@ def test_rope_cache_q4_refuses_shapes_and_sizes_it_does_not_take(entry_points):
             ops.rope_cache_q4(bad_qkv, bad_q, _pages(ops), **good)
     with pytest.raises(UnsupportedError):
         ops.rope_cache_q4(torch.zeros(3, 8 * 48), torch.zeros(3, 4 * 48), _pages(ops), **{**good, "head_dim": 48})
+    huge = ops.Q4Pages(*[t[:1].expand(2 ** 27, *t.shape[1:]) for t in _pages(ops)])      # 2^31 slots
+    with pytest.raises(UnsupportedError):
+        ops.rope_cache_q4(qkv, q, huge, **good)
     bad = _pages(ops)._replace(v_scales=torch.zeros(3, 2, 16, 4, dtype=torch.bfloat16))
     with pytest.raises(InvalidArgumentError):
         ops.rope_cache_q4(qkv, q, bad, **good)
+
+
+def test_tensors_elsewhere_of_another_type_or_in_pieces_are_refused(entry_points):
+    from vipera_rs_b200.errors import InternalError, InvalidArgumentError
+
+    ops = entry_points
+    table = torch.zeros(1, 4, dtype=torch.int32)
+    with pytest.raises(InternalError):            # on the host
+        ops.step_maps(_int(0, 1), _int(0), page_size=16, block_table=table)
+    with pytest.raises(InvalidArgumentError):     # 64-bit lengths
+        ops.step_maps(_int(0, 1).long(), _int(0), page_size=16, block_table=table)
+    with pytest.raises(InvalidArgumentError):     # every second number of a tensor
+        ops.step_maps(torch.zeros(4, dtype=torch.int32)[::2], _int(0), page_size=16, block_table=table)
 
 
 def test_expand_q4_refuses_rooms_of_another_cache(entry_points):
@@ -148,6 +164,8 @@ def test_the_memory_plan_counts_packed_pages_and_one_slots_room():
     # A's two layers are alike: the room is one layer's pages, and one page more
     spec = _spec(helpers.CONFIGS["A"])
     assert planner.room_bytes(spec, 256, 3, 2) == planner.cache_bytes(spec, 256, 3, 2) // 2 + 16 * 2 * 2 * 64 * 2
+    # 32-bit steps keep (outputs, maximum, sum) of every token and head
+    assert planner.room_bytes(spec, 256, 3, 4) == 2 * planner.room_bytes(spec, 256, 3, 2) + planner.PLANNED_STEP_TOKENS * 4 * (64 + 2) * 4
 
 
 def test_models_whose_mixers_need_the_runs_type_refuse_4_bits():
@@ -183,7 +201,7 @@ def test_keys_are_shared_by_a_clusters_blocks_and_cut_into_whole_walks():
     for tiles in (1, 3, 8, 64, 300, 12000):
         for keys in (1, 128, 129, 2049, 40000, 10**6):
             shares = ops.q4_shares(tiles, keys, 148)
-            assert (shares == 0) == (tiles >= 148 and keys > 1024)       # in even runs where there are many and long ones
+            assert (shares == 0) == (tiles >= 16 and tiles * -(-keys // 128) >= 8 * 444)      # in even runs where there is much to read
             assert shares in (0, 1, 2, 4, 8, 16) and (shares < 2 or keys > 64 * shares)    # no more than there are walks for, but for one
             chunk, splits = ops.q4_rows_splits(tiles, keys, 148)
             assert chunk % 64 == 0 and 0 < splits <= 64 and chunk * (splits - 1) < keys <= chunk * splits
@@ -203,3 +221,23 @@ def test_page_lists_are_the_requests_pages_one_behind_the_other():
         assert starts.tolist()[0] == 0 and starts.tolist()[-1] == len(pages)
         for row, (first, last) in enumerate(zip(starts[:-1], starts[1:])):
             assert table[row].tolist() == pages[first:last].tolist() + [-1] * (8 - (last - first))
+
+
+def test_the_command_line_plans_packed_pages(tmp_path, capsys):
+    import json
+
+    import helpers
+    from nobupel_cases import MIXED
+    from vipera_rs_b200 import cli
+
+    for raw, code in ((helpers.CONFIGS["A"], 0), (MIXED, 2)):
+        (tmp_path / "config.json").write_text(json.dumps(raw))
+        plans = []
+        for flags in ([], ["--kv-type", "q4"]):
+            assert cli.main(["plan", str(tmp_path), "--ctx", "64", "--batch", "2", "--json", *flags]) == (code if flags else 0)
+            plans.append(capsys.readouterr())
+        if code:
+            assert plans[1].err.startswith("vipera: unsupported:")
+        else:
+            run, packed = (json.loads(p.out) for p in plans)
+            assert packed["kv_bytes"] * 32 == run["kv_bytes"] * 9

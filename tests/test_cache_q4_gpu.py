@@ -242,8 +242,8 @@ def _attend(ops, step, dtype, heads, kv_heads, d, seed=0, window=0, keep_first=0
 def deal(ops, request, monkeypatch):
     """How single tokens' keys are shared: by the blocks of a cluster, or dealt out in even runs as where requests are many."""
     ops.q4_shares.cache_clear()
-    monkeypatch.setattr(ops, "Q4_RUNS_FROM", 0.0 if request.param == "runs" else 1e9)
-    monkeypatch.setattr(ops, "Q4_RUNS_KEYS", 0)
+    monkeypatch.setattr(ops, "Q4_RUNS_UNITS", 0 if request.param == "runs" else 1e9)
+    monkeypatch.setattr(ops, "Q4_RUNS_PAIRS", 0)
     yield request.param
     ops.q4_shares.cache_clear()
 
@@ -314,9 +314,49 @@ def test_single_tokens_beside_portions_in_either_deal(ops, deal, monkeypatch):
 
 def test_many_requests_take_the_even_runs(ops):
     ops.q4_shares.cache_clear()
-    assert ops.q4_shares(180, 1200, ops._sm_count_of(0)) == 0
+    assert ops.q4_shares(180, 3000, ops._sm_count_of(0)) == 0
     rng = np.random.default_rng(12)
-    _attend(ops, Step([1] * 90, [int(x) for x in rng.integers(0, 300, 89)] + [1199], 16), torch.bfloat16, 4, 2, 64)
+    _attend(ops, Step([1] * 90, [int(x) for x in rng.integers(0, 300, 89)] + [2999], 16), torch.bfloat16, 4, 2, 64)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_entries_without_tokens_take_no_part(ops, form, dtype):
+    _attend(ops, Step([0, 3, 0, 1, 0, 20, 0], [5, 40, 0, 33, 100, 0, 1], 16), dtype, 4, 2, 64)
+
+
+@pytest.mark.parametrize("counts", [[1, 1], [3, 2]])
+def test_a_query_that_is_not_finite_shows_in_its_own_head(ops, deal, counts):
+    """NaN and infinities in one head of one token: that head's outputs are NaN, all others those of the same step without."""
+    step = Step(counts, [70, 20], 16)
+    tokens, heads, d = sum(counts), 6, 64
+    pages = ops.Q4Pages(*plain.make_pages(step.num_pages, 16, 2, d, 3, DEVICE))
+    q = torch.randn(tokens, heads * d, device=DEVICE).to(torch.bfloat16)
+    outs = []
+    for bad in (None, float("nan"), float("inf")):
+        x, out = q.clone(), torch.zeros_like(q)
+        if bad is not None:
+            x[1, 2 * d + 5] = bad
+        ops.attention_q4(x, out, pages, num_heads=heads, num_kv_heads=2, head_dim=d, scale=0.125, workspace=_workspace(), **step.device())
+        outs.append(out.view(tokens, heads, d))
+    for out in outs[1:]:
+        assert out[1, 2].isnan().all()
+        keep = torch.ones(tokens, heads, dtype=torch.bool, device=DEVICE)
+        keep[1, 2] = False
+        assert torch.equal(out[keep], outs[0][keep])
+
+
+def test_queries_of_any_size_keep_their_bits(ops, deal):
+    """Queries times a power of two and the scale divided by it: the same outputs, from numbers near the smallest to near the largest."""
+    step = Step([1, 1], [90, 17], 16)
+    pages = ops.Q4Pages(*plain.make_pages(step.num_pages, 16, 1, 128, 3, DEVICE))
+    q = torch.randn(2, 4 * 128, device=DEVICE).to(torch.bfloat16)
+    outs = []
+    for up in (0, -80, 80, 20):
+        out = torch.zeros_like(q)
+        ops.attention_q4(q * 2.0 ** up, out, pages, num_heads=4, num_kv_heads=1, head_dim=128, scale=128 ** -0.5 * 2.0 ** -up,
+                         workspace=_workspace(), **step.device())
+        outs.append(out)
+    assert all(torch.equal(out, outs[0]) for out in outs[1:])
 
 
 def test_a_long_history_in_many_splits(ops, deal):

@@ -44,6 +44,7 @@ struct DecodeParams {
   int table_width, page_size, page_shift, num_pages, num_entries, num_heads, num_kv_heads, head_dim;
   float scale;
   int window, keep_first, sink, shares;
+  int settled;                    // positions, tables and earlier steps' rows are complete before the kernel ahead of this one begins
   uint32_t magic;                 // set by the launcher
 };
 
@@ -210,7 +211,7 @@ struct Shared {
 // heads' outputs, maxima and sums in `joined`, to be read behind a barrier.
 template <int D, int NT>
 __device__ __forceinline__ void walk(const DecodeParams& p, const Shared<D, NT> shared, const Visible seen, int entry, int token, int kv_head,
-                                     int head0, int tile_begin, int tiles_end) {
+                                     int head0, int tile_begin, int tiles_end, bool waited = true) {
   constexpr int G = D / 32, kRowBytes = D / 2, kChunks = kRowBytes / 16;
   constexpr int kRow = D + 4;
   uint4* queries = shared.queries();
@@ -292,8 +293,19 @@ __device__ __forceinline__ void walk(const DecodeParams& p, const Shared<D, NT> 
     cp_async_commit();
   };
 
+  // Rows of earlier steps may come before the kernel ahead has ended; the query's own row, and the queries, only then.  The kernel behind
+  // may start from there on and not before: the decode step of one request is 1.32 ms so and 1.46 where it may start at once (its
+  // blocks then take the places that this kernel's clusters wait for).
+  if (!waited && tiles_end == seen.tiles) {
+    pdl_wait();
+    pdl_launch_dependents();
+  }
 #pragma unroll
   for (int j = 0; j < kStages - 1; ++j) fetch(j);
+  if (!waited && tiles_end != seen.tiles) {
+    pdl_wait();
+    pdl_launch_dependents();
+  }
 
   // --- the queries in half precision: lane (g, t) has channels 32 group + 8 t .. + 7 of head 8 nt + g ---
   // in shared memory, a piece of 16 bytes a lane: neighbouring channels, the second and fourth pair a 16th; and, for heads 2 t and 2 t + 1,
@@ -590,8 +602,10 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) attention_q4_clu
   constexpr int kRow = D + 4;
   extern __shared__ __align__(128) uint8_t shared_at[];
   const Shared<D, NT> shared{shared_at};
-  pdl_wait();
-  pdl_launch_dependents();
+  if (!p.settled) {
+    pdl_wait();
+    pdl_launch_dependents();
+  }
   const int group = p.num_heads / p.num_kv_heads, head_tiles = (group + 8 * NT - 1) / (8 * NT);
   const int entry = blockIdx.x, share = blockIdx.z;
   const int kv_head = blockIdx.y / head_tiles, head0 = (blockIdx.y - kv_head * head_tiles) * 8 * NT;
@@ -602,7 +616,7 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) attention_q4_clu
   }
   const Visible seen(p, p.positions[entry]);
   const int each = (seen.tiles + 8 * p.shares - 1) / (8 * p.shares) * 8;      // of a block: whole steps of its warps
-  walk<D, NT>(p, shared, seen, entry, token, kv_head, head0, share * each, min((share + 1) * each, seen.tiles));
+  walk<D, NT>(p, shared, seen, entry, token, kv_head, head0, min(share * each, seen.tiles), min((share + 1) * each, seen.tiles), !p.settled);
   cluster_sync_all();
   const int heads_here = min(8 * NT, group - head0);
   const uint32_t joined_at = smem_addr(shared.joined());
@@ -725,7 +739,7 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) attention_q4_run
   }
 }
 
-// A block per (entry, pair): joins the parts of a pair that several runs share.
+// Two blocks an (entry, pair): they join the parts of a pair that several runs share.
 template <int D, int NT>
 __global__ void __launch_bounds__(128) attention_q4_join_kernel(DecodeParams p, const float* __restrict__ parts, int blocks) {
   constexpr int kRow = D + 4;
@@ -760,10 +774,10 @@ __global__ void __launch_bounds__(128) attention_q4_join_kernel(DecodeParams p, 
   const int kv_head = pair / head_tiles, head0 = (pair - kv_head * head_tiles) * 8 * NT, heads_here = min(8 * NT, group - head0);
   const int token = p.entry_starts ? p.entry_starts[entry] : entry;
   const auto part_of = [&](int r) { return parts + (2 * static_cast<size_t>(r) + (r == first_run ? 1 : 0)) * (8 * NT * kRow); };
-  for (int i = threadIdx.x; i < heads_here * (D / 4); i += blockDim.x) {
+  for (int i = blockIdx.z * 128 + threadIdx.x; i < heads_here * (D / 4); i += 256) {
     const int h = i / (D / 4), column = (i - h * (D / 4)) * 4;
     Join join;
-    constexpr int kAtOnce = 4;        // parts that are asked for together; the maximum follows them
+    constexpr int kAtOnce = 8;        // parts that are asked for together; the maximum follows them
     for (int r = first_run; r <= last_run; r += kAtOnce) {
       float m[kAtOnce], l[kAtOnce];
       float4 v[kAtOnce];
@@ -813,7 +827,7 @@ int launch(const DecodeParams& p, float* parts, int runs, cudaStream_t s) {
     if (ready != VIPERA_OK) return ready;
     const int status = vipera_launch(kernel, dim3(runs), 32 * kWarps, kSmem, s, p, parts);
     if (status != VIPERA_OK) return status;
-    return vipera_launch(attention_q4_join_kernel<D, NT>, dim3(p.num_entries, p.num_kv_heads * head_tiles), 128, 0, s, p, parts, runs);
+    return vipera_launch(attention_q4_join_kernel<D, NT>, dim3(p.num_entries, p.num_kv_heads * head_tiles, 2), 128, 0, s, p, parts, runs);
   }
   const auto kernel = attention_q4_cluster_kernel<D, NT>;
   static uint64_t asked = 0;

@@ -21,9 +21,9 @@ struct MapsParams {
 
 // Block (x, e): its share of entry e's table row and of its tokens.  What bounds it is the latency of two trips to
 // memory (lengths, then pages) behind the launch, not bytes, so an entry's lengths are asked for at once and nothing
-// is searched: a token's entry is the block's.
+// is searched: a token's entry is the block's.  It does not let the kernel behind it start early: kernels of a step read positions and
+// tables before their own wait, and must find them written.
 __global__ void __launch_bounds__(256) step_maps_kernel(MapsParams p) {
-  pdl_launch_dependents();
   pdl_wait();
   const int e = blockIdx.y;
   const int begin = max(p.entry_starts[e], 0), end = min(p.entry_starts[e + 1], p.num_tokens);
@@ -52,6 +52,7 @@ __global__ void __launch_bounds__(256) step_maps_kernel(MapsParams p) {
       p.slots[t] = page < 0 ? -1 : page * p.page_size + place;
     }
   }
+  __threadfence();
 }
 
 // ---------------------------------------------------------------------------------------

@@ -1090,7 +1090,7 @@ class _DecodeQ4Params(ctypes.Structure):
                 ("sink_values", _c_void), ("gate", _c_void), ("gate_stride", ctypes.c_longlong), ("gate_per_head", _c_int),
                 ("table_width", _c_int), ("page_size", _c_int), ("page_shift", _c_int), ("num_pages", _c_int), ("num_entries", _c_int), ("num_heads", _c_int),
                 ("num_kv_heads", _c_int), ("head_dim", _c_int), ("scale", _c_float), ("window", _c_int), ("keep_first", _c_int),
-                ("sink", _c_int), ("shares", _c_int), ("magic", ctypes.c_uint)]
+                ("sink", _c_int), ("shares", _c_int), ("settled", _c_int), ("magic", ctypes.c_uint)]
 
 
 class _RowsQ4Params(ctypes.Structure):
@@ -1209,6 +1209,8 @@ def rope_cache_q4(qkv: torch.Tensor, q_out: torch.Tensor, pages: Q4Pages, *, num
         if cos is None or sin is None or cos.dim() != 2 or cos.shape[1] != rot_dims // 2 or sin.shape != cos.shape or not cos.shape[0]:
             raise InvalidArgumentError("rope_cache_q4: cos/sin tables of width rot_dims/2 are needed")
         table_rows = cos.shape[0]
+    if pages.k_codes.shape[0] * page_size > 0x7fffffff or count * (num_heads + 2 * num_kv_heads) * (head_dim // 8) > 0x7fffffff:
+        raise UnsupportedError("rope_cache_q4: a pool has fewer than 2^31 slots, a step fewer than 2^31 pieces of 8 channels")
     here, int32, what = torch.cuda.current_device(), torch.int32, "rope_cache_q4"
     if qkv.dtype is not torch.float32 or qkv.get_device() != here:     # its rows may lie apart
         raise InvalidArgumentError("rope_cache_q4: qkv must be float32 on the current CUDA device")
@@ -1255,10 +1257,11 @@ def attention_q4_takes_decode(dtype: torch.dtype, head_dim: int, page_size: int)
 # each 128 of them cost where one, two or three blocks share an SM (fitted to launches at batch 1 to 64 and 2,048 to 32,768 keys).
 Q4_BLOCKS_PER_SM = 3
 Q4_BLOCK_FIXED, Q4_BLOCK_KEYS = 2.2, (0.0, 0.8, 1.25, 1.75)
-# From this many (entry, KV head) pairs on, for each SM, histories of more than this many keys are dealt to the blocks in even runs: 64
-# requests of 0 to 4,095 keys and 4 KV heads 33 us where two blocks a pair take 38, 48 of 8,192 keys and 8 KV heads 109 where one takes
-# 113; histories of 300 and 1,024 keys are better off with a block a pair (30 and 12 us for 38 and 15).
-Q4_RUNS_FROM, Q4_RUNS_KEYS = 1.0, 1024
+# Where a block would have this many times 128 keys were all histories the longest, and there are some pairs to join, the keys of all
+# pairs are dealt to the blocks in even runs: 64 requests of 0 to 4,095 keys and 4 KV heads take 34 us where two blocks a pair take 39, 48 of
+# 8,192 keys and 8 KV heads 112 for 116, two of 16,000 beside fourteen of 1,000 22 for 28; shorter walks do not pay for the second
+# launch (64 requests of 2,048 keys and 2 KV heads 23 us for 21).
+Q4_RUNS_UNITS, Q4_RUNS_PAIRS = 8, 16
 Q4_RUNS_ENTRIES = 1024      # kRunEntries in attention_q4.cu
 
 
@@ -1267,9 +1270,9 @@ def q4_shares(pairs: int, seen: int, sm_count: int, runs: bool = True) -> int:
     """How many blocks share the keys of one of `pairs` (entry, KV head) pairs in a step of single tokens over packed pages, `seen` keys at
     most: the power of two up to 16 (a cluster's blocks) that a model of the launch's time likes best; 0 (where `runs` allows it): all
     pairs' keys are dealt out in even runs."""
-    if runs and pairs >= Q4_RUNS_FROM * sm_count and seen > Q4_RUNS_KEYS:
-        return 0
     slots, best = Q4_BLOCKS_PER_SM * sm_count, None
+    if runs and pairs >= Q4_RUNS_PAIRS and pairs * -(-seen // 128) >= Q4_RUNS_UNITS * slots:
+        return 0
     for shares in (1, 2, 4, 8, 16):
         units = -(-seen // (128 * shares))
         full, rest = divmod(pairs * shares, slots)
@@ -1281,7 +1284,7 @@ def q4_shares(pairs: int, seen: int, sm_count: int, runs: bool = True) -> int:
     return best[1]
 
 
-def _attention_q4_decode(q, out, pages, *, positions, block_table, num_heads, num_kv_heads, head_dim, scale, max_keys, workspace, entry_starts,
+def _attention_q4_decode(q, out, pages, *, positions, block_table, num_heads, num_kv_heads, head_dim, scale, max_keys, workspace, settled, entry_starts,
                          window, keep_first, sink, sink_values, gate, gate_offset, gate_per_head) -> None:
     fn = _function("attention_q4", "vipera_attention_q4_decode", _DECODE_Q4_ARGS)
     _check_struct("attention_q4", "vipera_attention_q4_params_size", _DecodeQ4Params)
@@ -1303,7 +1306,7 @@ def _attention_q4_decode(q, out, pages, *, positions, block_table, num_heads, nu
                         None if entry_starts is None else _place(what, entry_starts, int32, here),
                         None if sink_values is None else _place(what, sink_values, torch.float32, here), gate_pointer, gate_stride,
                         1 if gate_per_head else 0, width, pages.k_codes.shape[2], 0, pages.k_codes.shape[0], entries,
-                        num_heads, num_kv_heads, head_dim, scale, window, keep_first, 1 if sink else 0, shares, 0)
+                        num_heads, num_kv_heads, head_dim, scale, window, keep_first, 1 if sink else 0, shares, 1 if settled else 0, 0)
     if shares:
         _check(fn(p, None, 0, 0, _stream_of(here)), "attention_decode")
     else:
@@ -1363,11 +1366,14 @@ def attention_q4(q: torch.Tensor, out: torch.Tensor, pages: Q4Pages, *, entry_st
                  positions: torch.Tensor, token_entry: torch.Tensor, block_table: torch.Tensor, num_heads: int, num_kv_heads: int,
                  head_dim: int, scale: float, max_keys: int, all_single: bool, any_single: bool, workspace, window: int = 0,
                  keep_first: int = 0, sink: bool = False, sink_values: Optional[torch.Tensor] = None,
-                 gate: Optional[torch.Tensor] = None, gate_offset: int = 0, gate_per_head: bool = False, longest: int = 0) -> None:
+                 gate: Optional[torch.Tensor] = None, gate_offset: int = 0, gate_per_head: bool = False, longest: int = 0,
+                 settled: bool = False) -> None:
     """Causal grouped-query attention of every token of a step over its request's pages of 4 bits; q and out [tokens, heads * d],
     bfloat16 or float32, the step described as for the other attentions.  ``max_keys``: no request sees more; ``all_single``: every
     entry brings one token; ``any_single``: some entry may.  ``window``, ``keep_first``, ``sink``, ``sink_values`` and the gate as
-    for ``attention``, ``longest`` too.  ``workspace.get(name, shape, dtype)`` gives rooms that the call may use until it is
+    for ``attention``, ``longest`` too.  ``settled``: positions, tables and the rows of earlier steps were complete before the kernel ahead of
+    this call was launched (as in a step whose description the host copied), so that they may be read while that kernel still runs.
+    ``workspace.get(name, shape, dtype)`` gives rooms that the call may use until it is
     done on its stream.
 
     With heads of 64 or 128 values and pages of a multiple of 16 tokens, single tokens, short portions and all of a 32-bit step are
@@ -1397,7 +1403,7 @@ def attention_q4(q: torch.Tensor, out: torch.Tensor, pages: Q4Pages, *, entry_st
                    gate_per_head=gate_per_head)
     packed = attention_q4_takes_decode(q.dtype, head_dim, page_size)
     if packed and all_single:
-        _attention_q4_decode(q, out, pages, positions=positions, block_table=block_table, max_keys=max_keys, workspace=workspace,
+        _attention_q4_decode(q, out, pages, positions=positions, block_table=block_table, max_keys=max_keys, workspace=workspace, settled=settled,
                              entry_starts=None, **heads, **endings)
         return
     if attention_q4_takes_rows(q.dtype, head_dim, page_size, count * num_heads, num_heads, 1 if any_single else entries):
@@ -1421,7 +1427,7 @@ def attention_q4(q: torch.Tensor, out: torch.Tensor, pages: Q4Pages, *, entry_st
     attention_prefill(q, out, k_room, v_room, entry_starts=entry_starts, entry_pos0=entry_pos0, block_table=block_table,
                       num_entries=entries, skip_single=apart, **heads, **endings)
     if apart:
-        _attention_q4_decode(q, out, pages, positions=entry_pos0, block_table=block_table, max_keys=max_keys, workspace=workspace,
+        _attention_q4_decode(q, out, pages, positions=entry_pos0, block_table=block_table, max_keys=max_keys, workspace=workspace, settled=settled,
                              entry_starts=entry_starts, **heads, **endings)
 
 

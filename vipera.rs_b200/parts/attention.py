@@ -431,7 +431,7 @@ class GQAttention(Mixer):
                          scale=self.scale, max_keys=max(ctx.max_kv_len, 1), all_single=ctx.all_single, any_single=ctx.any_single,
                          workspace=ctx.workspace, window=self.window or 0, keep_first=self.keep_first, sink=self.sink,
                          sink_values=self.sink_values, gate=qkv if self.gated else None, gate_offset=self.gate_offset,
-                         gate_per_head=self.gate_per_head, longest=longest)
+                         gate_per_head=self.gate_per_head, longest=longest, settled=True)
         return self._output(ctx, mixed, residual)
 
     def _attend(self, ctx, q, mixed, cache, table, gate=None):
