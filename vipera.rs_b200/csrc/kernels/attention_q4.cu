@@ -442,8 +442,9 @@ __device__ __forceinline__ void walk(const DecodeParams& p, const Shared<D, NT> 
           }
         }
     }
-    // Weights are taken against a maximum that follows when a score is 2^8 above it, so that most steps need no word among the
-    // eight lanes that hold a head's keys.
+    // Only a step that raises some head's maximum needs a word among the eight lanes that hold a head's keys.  The maximum follows at once
+    // (a threshold of 2^8 would save one such step in three): the weight of the key that a head looks at most is then 1, and is
+    // not rounded, which halves the error where few keys count.
     float high[NT][2];
     bool grown = false;
 #pragma unroll
@@ -451,7 +452,7 @@ __device__ __forceinline__ void walk(const DecodeParams& p, const Shared<D, NT> 
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         high[nt][c] = fmaxf(fmaxf(s[0][nt][c], s[0][nt][2 + c]), fmaxf(s[1][nt][c], s[1][nt][2 + c]));
-        grown = grown || high[nt][c] > most[nt][c] + 8.0f;
+        grown = grown || high[nt][c] > most[nt][c];
       }
     if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll

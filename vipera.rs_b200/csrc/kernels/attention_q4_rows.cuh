@@ -201,7 +201,7 @@ __global__ void __launch_bounds__(32 * kWarps) attention_q4_rows_kernel(RowsPara
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         high[nt][c] = fmaxf(s[nt][c], s[nt][2 + c]);
-        grown = grown || high[nt][c] > most[nt][c] + 8.0f;
+        grown = grown || high[nt][c] > most[nt][c];
       }
     }
     if (__any_sync(0xffffffffu, grown)) {
