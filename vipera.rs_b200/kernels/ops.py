@@ -1110,24 +1110,32 @@ _ROWS_Q4_ARGS = [ctypes.POINTER(_RowsQ4Params), _c_void, _c_int, _c_int, _c_void
                  _c_void, ctypes.c_size_t, _c_void]
 
 
-def _place(what: str, tensor: torch.Tensor, dtype: torch.dtype, here: int) -> int:
-    """The address of a contiguous tensor of `dtype` on device `here`, the current one, whose stream the launch goes to."""
-    if tensor.dtype is not dtype or not tensor.is_contiguous() or tensor.get_device() != here:
-        if tensor.dtype is not dtype:
-            raise InvalidArgumentError(f"{what}: a tensor is {tensor.dtype} in the place of {dtype}")
-        if not tensor.is_contiguous():
-            raise InvalidArgumentError(f"{what}: tensors must be contiguous")
-        if not tensor.is_cuda:
-            raise InternalError(f"{what}: a tensor is not on a CUDA device; this engine has no CPU path")
-        raise InvalidArgumentError(f"{what}: a tensor is on {tensor.device}, the current device is cuda:{here}")
-    return tensor.data_ptr()
+def _refuse_place(what: str, tensor: torch.Tensor, dtype: torch.dtype, here: int) -> None:
+    if tensor.dtype is not dtype:
+        raise InvalidArgumentError(f"{what}: a tensor is {tensor.dtype} in the place of {dtype}")
+    if not tensor.is_contiguous():
+        raise InvalidArgumentError(f"{what}: tensors must be contiguous")
+    if not tensor.is_cuda:
+        raise InternalError(f"{what}: a tensor is not on a CUDA device; this engine has no CPU path")
+    raise InvalidArgumentError(f"{what}: a tensor is on {tensor.device}, the current device is cuda:{here}")
 
 
-def _place_pages(what: str, pages: Q4Pages, here: int):
+def _places(what: str, dtype: torch.dtype, here: int, *tensors) -> list:
+    """The addresses of contiguous tensors of `dtype` on device `here`, the current one, whose stream the launch goes to (None for None)."""
+    out = []
+    for tensor in tensors:
+        if tensor is None:
+            out.append(None)
+            continue
+        if tensor.dtype is not dtype or tensor.get_device() != here or not tensor.is_contiguous():
+            _refuse_place(what, tensor, dtype, here)
+        out.append(tensor.data_ptr())
+    return out
+
+
+def _place_pages(what: str, pages: Q4Pages, here: int) -> list:
     """The addresses of the pages' parts: codes of keys and values, scales of keys and values."""
-    k_codes, k_scales, v_codes, v_scales = pages
-    return (_place(what, k_codes, torch.uint8, here), _place(what, v_codes, torch.uint8, here),
-            _place(what, k_scales, torch.bfloat16, here), _place(what, v_scales, torch.bfloat16, here))
+    return _places(what, torch.uint8, here, pages[0], pages[2]) + _places(what, torch.bfloat16, here, pages[1], pages[3])
 
 
 @functools.lru_cache(maxsize=None)
@@ -1179,9 +1187,8 @@ def step_maps(entry_starts: torch.Tensor, entry_pos0: torch.Tensor, *, page_size
     if counts:
         raise InvalidArgumentError("step_maps: positions, token_entry and slots hold one number for each token")
     here, int32, what = torch.cuda.current_device(), torch.int32, "step_maps"
-    at = [None if t is None else _place(what, t, int32, here)
-          for t in (entry_starts, entry_pos0, page_starts, pages, block_table, positions, token_entry, slots)]
-    p = _MapsParams(*at, entries, tokens, 0 if pages is None else pages.numel(), block_table.shape[1], page_size)
+    p = _MapsParams(*_places(what, int32, here, entry_starts, entry_pos0, page_starts, pages, block_table, positions, token_entry, slots),
+                    entries, tokens, 0 if pages is None else pages.numel(), block_table.shape[1], page_size)
     _check(fn(p, _stream_of(here)), what)
 
 
@@ -1214,12 +1221,11 @@ def rope_cache_q4(qkv: torch.Tensor, q_out: torch.Tensor, pages: Q4Pages, *, num
     here, int32, what = torch.cuda.current_device(), torch.int32, "rope_cache_q4"
     if qkv.dtype is not torch.float32 or qkv.get_device() != here:     # its rows may lie apart
         raise InvalidArgumentError("rope_cache_q4: qkv must be float32 on the current CUDA device")
-    k_codes, v_codes, k_scales, v_scales = _place_pages(what, pages, here)
-    cos_at, sin_at = (_place(what, cos, torch.float32, here), _place(what, sin, torch.float32, here)) if table_rows else (None, None)
-    p = _StoreQ4Params(qkv.data_ptr(), qkv.stride(0), _place(what, q_out, q_out.dtype, here), k_codes, v_codes, k_scales, v_scales,
-                       _place(what, positions, int32, here), cos_at, sin_at, None if slots is None else _place(what, slots, int32, here),
-                       0 if slots is None else pages.k_codes.shape[0] * page_size, table_rows, count, num_heads, num_kv_heads, head_dim,
-                       rot_dims, style, page_size)
+    positions_at, slots_at = _places(what, int32, here, positions, slots)
+    cos_at, sin_at = _places(what, torch.float32, here, cos, sin) if table_rows else (None, None)
+    p = _StoreQ4Params(qkv.data_ptr(), qkv.stride(0), *_places(what, q_out.dtype, here, q_out), *_place_pages(what, pages, here),
+                       positions_at, cos_at, sin_at, slots_at, 0 if slots is None else pages.k_codes.shape[0] * page_size, table_rows, count,
+                       num_heads, num_kv_heads, head_dim, rot_dims, style, page_size)
     _check(fn(p, dtype_code(q_out.dtype), _stream_of(here)), "rope_cache")
 
 
@@ -1241,10 +1247,9 @@ def expand_q4(pages: Q4Pages, k_room: torch.Tensor, v_room: torch.Tensor, *, ent
         raise InvalidArgumentError("expand_q4: entry_starts has one item more than entry_pos0, the block table a row for each entry")
     here, int32, what = torch.cuda.current_device(), torch.int32, "expand_q4"
     width = block_table.shape[1]
-    p = _ExpandQ4Params(*_place_pages(what, pages, here), _place(what, k_room, k_room.dtype, here), _place(what, v_room, k_room.dtype, here),
-                        _place(what, entry_starts, int32, here), _place(what, entry_pos0, int32, here),
-                        _place(what, block_table, int32, here), width, page_size, entries, num_pages, num_kv_heads,
-                        head_dim, max(int(window or 0), 0), int(keep_first or 0), 1 if skip_single else 0)
+    p = _ExpandQ4Params(*_place_pages(what, pages, here), *_places(what, k_room.dtype, here, k_room, v_room),
+                        *_places(what, int32, here, entry_starts, entry_pos0, block_table), width, page_size, entries, num_pages,
+                        num_kv_heads, head_dim, max(int(window or 0), 0), int(keep_first or 0), 1 if skip_single else 0)
     _check(fn(p, dtype_code(k_room.dtype), min(4 * _sm_count_of(here), max(1, 2 * entries * width)), _stream_of(here)), what)
 
 
@@ -1301,10 +1306,9 @@ def _attention_q4_decode(q, out, pages, *, positions, block_table, num_heads, nu
         parts = workspace.get("attention.partials", (runs * 2 * (16 if wide else 8) * (head_dim + 4),), torch.float32)
     gate_pointer, gate_stride = (None, 0) if gate is None else _gate_pointer(
         gate, gate_offset, q.shape[0], num_heads * (1 if gate_per_head else head_dim), what)
-    p = _DecodeQ4Params(_place(what, q, torch.bfloat16, here), _place(what, out, torch.bfloat16, here), *_place_pages(what, pages, here),
-                        _place(what, positions, int32, here), _place(what, block_table, int32, here),
-                        None if entry_starts is None else _place(what, entry_starts, int32, here),
-                        None if sink_values is None else _place(what, sink_values, torch.float32, here), gate_pointer, gate_stride,
+    sinks, = _places(what, torch.float32, here, sink_values)
+    p = _DecodeQ4Params(*_places(what, torch.bfloat16, here, q, out), *_place_pages(what, pages, here),
+                        *_places(what, int32, here, positions, block_table, entry_starts), sinks, gate_pointer, gate_stride,
                         1 if gate_per_head else 0, width, pages.k_codes.shape[2], 0, pages.k_codes.shape[0], entries,
                         num_heads, num_kv_heads, head_dim, scale, window, keep_first, 1 if sink else 0, shares, 1 if settled else 0, 0)
     if shares:
@@ -1353,12 +1357,13 @@ def _attention_q4_rows(q, out, pages, *, entry_starts, entry_pos0, positions, bl
         count, num_heads, head_dim, splits + (1 if keep_first else 0)),), torch.float32)
     gate_pointer, gate_stride = (None, 0) if gate is None else _gate_pointer(
         gate, gate_offset, count, num_heads * (1 if gate_per_head else head_dim), what)
-    p = _RowsQ4Params(_place(what, q, dtype, here), *_place_pages(what, pages, here), _place(what, entry_starts, int32, here),
-                      _place(what, entry_pos0, int32, here), _place(what, block_table, int32, here), None, None, block_table.shape[1],
+    q_at, out_at = _places(what, dtype, here, q, out)
+    starts_at, pos0_at, table_at, positions_at = _places(what, int32, here, entry_starts, entry_pos0, block_table, positions)
+    sinks, = _places(what, torch.float32, here, sink_values)
+    p = _RowsQ4Params(q_at, *_place_pages(what, pages, here), starts_at, pos0_at, table_at, None, None, block_table.shape[1],
                       pages.k_codes.shape[2], pages.k_codes.shape[0], entries, count, num_heads, num_kv_heads, scale, window, keep_first,
                       chunk, splits)
-    _check(fn(p, _place(what, out, dtype, here), dtype_code(dtype), head_dim, _place(what, positions, int32, here), 1 if sink else 0,
-              None if sink_values is None else _place(what, sink_values, torch.float32, here), gate_pointer, gate_stride,
+    _check(fn(p, out_at, dtype_code(dtype), head_dim, positions_at, 1 if sink else 0, sinks, gate_pointer, gate_stride,
               1 if gate_per_head else 0, scratch.data_ptr(), scratch.numel(), _stream_of(here)), "attention", kernels=2)
 
 
