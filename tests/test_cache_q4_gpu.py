@@ -359,6 +359,44 @@ def test_queries_of_any_size_keep_their_bits(ops, deal):
     assert all(torch.equal(out, outs[0]) for out in outs[1:])
 
 
+def _off(tensor):
+    """The same numbers a place further on: contiguous, and not where rows of 16 bytes begin."""
+    room = torch.zeros(tensor.numel() + 1, dtype=tensor.dtype, device=DEVICE)
+    room[1:] = tensor.reshape(-1)
+    return room[1:].view(tensor.shape)
+
+
+def test_tensors_that_do_not_begin_on_16_bytes_are_refused(ops):
+    """Before a launch: the kernels move pieces of 16 bytes."""
+    from vipera_rs_b200.errors import InternalError
+
+    step = Step([1, 1], [20, 3], 16)
+    pages = ops.Q4Pages(*plain.make_pages(step.num_pages, 16, 1, 64, 3, DEVICE))
+    q, qkv = torch.zeros(2, 2 * 64, dtype=torch.bfloat16, device=DEVICE), torch.zeros(2, 4 * 64, device=DEVICE)
+    rooms = [torch.zeros(step.num_pages, 16, 1, 64, dtype=torch.bfloat16, device=DEVICE) for _ in range(2)]
+    described = step.device()
+    lengths = {name: described[name] for name in ("entry_starts", "entry_pos0", "block_table")}
+    stores = dict(num_heads=2, num_kv_heads=1, head_dim=64, positions=described["positions"], cos=None, sin=None, style=ops.ROPE_NONE,
+                  slots=_int(step.slots))
+    attends = dict(num_heads=2, num_kv_heads=1, head_dim=64, scale=0.125, workspace=_workspace(), **described)
+    off_codes = pages._replace(k_codes=_off(pages.k_codes))
+    calls = [lambda: ops.rope_cache_q4(qkv, _off(q), pages, **stores), lambda: ops.rope_cache_q4(qkv, q, off_codes, **stores),
+             lambda: ops.expand_q4(pages, _off(rooms[0]), rooms[1], **lengths), lambda: ops.expand_q4(off_codes, *rooms, **lengths),
+             lambda: ops.attention_q4(_off(q), q.clone(), pages, **attends), lambda: ops.attention_q4(q, _off(q), pages, **attends),
+             lambda: ops.attention_q4(q, q.clone(), off_codes, **attends),
+             lambda: ops.attention_q4(q, q.clone(), pages._replace(v_scales=_off(pages.v_scales)), **attends),
+             lambda: ops.attention_q4(q.float(), q.float(), off_codes, **attends)]
+    for call in calls:
+        with pytest.raises(InternalError, match="bad argument"):
+            call()
+    # a row that begins anywhere is read value by value
+    out, far = torch.zeros_like(q), torch.zeros_like(q)
+    qkv.normal_()
+    ops.rope_cache_q4(qkv, out, pages, **stores)
+    ops.rope_cache_q4(_off(qkv), far, pages, **stores)
+    assert torch.equal(out, far)
+
+
 def test_a_long_history_in_many_splits(ops, deal):
     """Thousands of keys, the longest beside a short one, of single tokens and of portions."""
     _attend(ops, Step([1, 1], [9000, 5], 16), torch.bfloat16, 2, 1, 64)

@@ -605,6 +605,7 @@ struct Join {
 };
 
 // Few (entry, KV head) pairs: the blocks of a cluster share the keys of one, each a part as large, and join their parts.
+// One entry of 2,048 keys, 12 heads of 128 on 2, sixteen blocks a pair: 7.8 us, the latency of a start (2), one walk and two cluster barriers.
 template <int D, int NT>
 __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) attention_q4_cluster_kernel(DecodeParams p) {
   constexpr int kRow = D + 4;
@@ -747,7 +748,8 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) attention_q4_run
   }
 }
 
-// Two blocks an (entry, pair): they join the parts of a pair that several runs share.
+// Two blocks an (entry, pair): they join the parts of a pair that several runs share.  4 us for 48 entries of 8 pairs, two trips to memory (the
+// lengths, the parts) behind a launch.
 template <int D, int NT>
 __global__ void __launch_bounds__(128) attention_q4_join_kernel(DecodeParams p, const float* __restrict__ parts, int blocks) {
   constexpr int kRow = D + 4;
