@@ -266,14 +266,22 @@ def test_windows_kept_keys_and_sinks(ops, deal, window, keep_first, sink, d):
     _attend(ops, Step([1, 1, 1], [300, 39, 0], 16, seed=window), torch.bfloat16, 8, 2, d, window=window, keep_first=keep_first, sink=sink)
 
 
-@pytest.fixture(params=["packed", "expanded"])
+@pytest.fixture(params=["packed", "tensor", "cut", "expanded"])
 def form(ops, request, monkeypatch):
-    """Which way bfloat16 portions take: over the packed pages, or over rows that are expanded first."""
-    if request.param == "expanded":
-        monkeypatch.setattr(ops, "Q4_ROWS_FIRST", 0)
+    """Which way bfloat16 portions take: the kernel of any number of rows, the tensor cores' with its keys in one piece or in several, or rows
+    that are expanded first."""
+    if request.param != "packed":
+        monkeypatch.setattr(ops, "Q4_ROWS_WORK", 0)
         assert not ops.attention_q4_takes_rows(torch.bfloat16, 64, 16, 2, 2, 1)
+        if request.param == "expanded":
+            monkeypatch.setattr(ops, "attention_q4_takes_portions", lambda *sizes: False)
+        else:
+            assert ops.attention_q4_takes_portions(torch.bfloat16, 64, 16)
+            rows, keys = (128, 128) if request.param == "cut" else (256, 1 << 20)
+            monkeypatch.setattr(ops, "q4_portion_plan", lambda tokens, heads, kv_heads, d, seen, *rest: (rows, keys, -(-seen // keys)))
     else:
-        assert ops.attention_q4_takes_rows(torch.bfloat16, 64, 16, 60 * 8, 8, 1)
+        monkeypatch.setattr(ops, "Q4_ROWS_WORK", 1e12)
+        monkeypatch.setattr(ops, "Q4_ROWS_PORTIONS", 1 << 20)
     return request.param
 
 
@@ -307,7 +315,7 @@ def test_portions_with_windows_and_kept_keys(ops, form, dtype, window, keep_firs
 
 def test_single_tokens_beside_portions_in_either_deal(ops, deal, monkeypatch):
     """The entries of one token of a mixed step, the others skipped: none of them first, some last, several in a row."""
-    monkeypatch.setattr(ops, "Q4_ROWS_FIRST", 0)
+    monkeypatch.setattr(ops, "Q4_ROWS_WORK", 0)
     _attend(ops, Step([5, 1, 1, 40, 1, 3, 1], [9, 300, 0, 0, 77, 20, 500], 16), torch.bfloat16, 6, 2, 64)
     _attend(ops, Step([1, 20, 2], [130, 10, 0], 16), torch.bfloat16, 4, 2, 128, window=50, keep_first=7)
 
@@ -527,3 +535,104 @@ def test_a_step_as_it_is_used_eager_captured_and_on_a_stream_of_its_own(ops):
                                    v_steps=pages.v_scales.double().cpu().numpy())
     limit = plain.allowed(expected, parts, 64, d, torch.bfloat16)
     assert (np.abs(outs[3].double().cpu().numpy().reshape(expected.shape) - expected) <= limit).all()
+
+
+def _portions(step, pages, q, ops, heads, kv_heads, d, scale=0.1, **more):
+    out = torch.zeros_like(q)
+    ops.attention_q4(q, out, pages, num_heads=heads, num_kv_heads=kv_heads, head_dim=d, scale=scale, workspace=_workspace(), **step.device(), **more)
+    return out
+
+
+@pytest.mark.parametrize("heads, kv_heads, d", [(7, 1, 128), (14, 2, 64), (3, 3, 128), (40, 1, 64)])
+@pytest.mark.parametrize("counts, history, window", [([300], [0], 0), ([130, 2, 37], [0, 700, 251], 0), ([200, 64], [120, 1000], 150)])
+def test_long_portions_on_the_tensor_cores(ops, form, heads, kv_heads, d, counts, history, window):
+    """Several tiles of rows and of keys, tiles that begin inside a token's heads, buffers used again and again."""
+    if form == "packed":
+        pytest.skip("the kernel of few rows")
+    _attend(ops, Step(counts, history, 16, seed=d), torch.bfloat16, heads, kv_heads, d, window=window)
+
+
+@pytest.mark.parametrize("keep_first", [0, 5])
+@pytest.mark.parametrize("d", [64, 128])
+def test_values_that_are_not_finite_show_in_the_rows_that_see_them(ops, form, keep_first, d):
+    """One group of one value: the group's outputs of the rows whose keys it is among are NaN, all others those of the same step without."""
+    heads, kv_heads, key = 6, 2, 141
+    step = Step([90, 3], [100, 60], 16)
+    window = 30 if keep_first else 0
+    raw = plain.make_pages(step.num_pages, 16, kv_heads, d, 3, DEVICE)
+    pages = ops.Q4Pages(*raw)
+    q = torch.randn(93, heads * d, device=DEVICE).to(torch.bfloat16)
+    more = dict(window=window, keep_first=keep_first)
+    without = _portions(step, pages, q, ops, heads, kv_heads, d, **more).view(93, heads, d)
+    raw[3][step.tables[0][key // 16], 1, key % 16, 1] = float("nan")
+    with_one = _portions(step, pages, q, ops, heads, kv_heads, d, **more).view(93, heads, d)
+    sees = [i < 90 and key <= 100 + i and (not window or key > 100 + i - window) for i in range(93)]
+    assert 0 < sum(sees) < 93
+    if form == "expanded":      # rows of one tile of the flash kernel share what they do not see
+        assert with_one[sees, 3:, 32:64].isnan().all()
+        return
+    bad = torch.zeros(93, heads, d, dtype=torch.bool, device=DEVICE)
+    bad[sees, 3:, 32:64] = True
+    assert with_one[bad].isnan().all()
+    assert torch.equal(with_one[~bad], without[~bad])
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_steps_near_the_largest_number(ops, form, d):
+    """Scales whose multiples leave the type: only their codes' own are asked for."""
+    step = Step([40], [30], 16)
+    raw = plain.make_pages(step.num_pages, 16, 1, d, 3, DEVICE)
+    pages = ops.Q4Pages(*raw)
+    q = torch.randn(40, 2 * d, device=DEVICE).to(torch.bfloat16)
+    usual = _portions(step, pages, q, ops, 2, 1, d)
+    raw[3].mul_(2.0 ** 117)
+    huge = _portions(step, pages, q, ops, 2, 1, d)
+    assert huge.isfinite().all() and raw[3].abs().max() > 2.0 ** 117
+    assert torch.equal(huge.float() * 2.0 ** -117, usual.float())
+    raw[3].mul_(2.0 ** -117)
+    raw[1].mul_(2.0 ** 117)
+    assert raw[1].abs().max() > 2.0 ** 117
+    assert torch.equal(_portions(step, pages, q, ops, 2, 1, d, scale=0.1 * 2.0 ** -117), usual)
+
+
+def test_the_tensor_cores_kernel_in_a_captured_step_on_another_stream(ops, monkeypatch):
+    monkeypatch.setattr(ops, "Q4_ROWS_WORK", 0)
+    step = Step([200, 1, 60], [30, 500, 900], 16)
+    pages = ops.Q4Pages(*plain.make_pages(step.num_pages, 16, 2, 128, 3, DEVICE))
+    q = torch.randn(261, 8 * 128, device=DEVICE).to(torch.bfloat16)
+    described, room, out = step.device(), _workspace(), torch.zeros_like(q)
+    run = lambda: ops.attention_q4(q, out, pages, num_heads=8, num_kv_heads=2, head_dim=128, scale=0.09, workspace=room, **described)
+    run()
+    first = out.clone()
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=stream):
+        run()
+    for scale in (1.0, 0.5):
+        q.mul_(scale)
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        if scale == 1.0:
+            assert torch.equal(out, first)
+    run()
+    last = out.clone()
+    out.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, last) and not torch.equal(out, first)
+    assert int(ops.kernel_status_word(q.device)[0]) == 0
+
+
+def test_keys_that_are_not_finite_show_in_the_rows_that_see_them(ops, form):
+    heads, d, key = 4, 64, 77
+    step = Step([60], [40], 16)
+    raw = plain.make_pages(step.num_pages, 16, 2, d, 3, DEVICE)
+    pages = ops.Q4Pages(*raw)
+    q = torch.randn(60, heads * d, device=DEVICE).to(torch.bfloat16)
+    without = _portions(step, pages, q, ops, heads, 2, d).view(60, heads, d)
+    raw[1][step.tables[0][key // 16], 1, key % 16, 0] = float("nan")
+    with_one = _portions(step, pages, q, ops, heads, 2, d).view(60, heads, d)
+    sees = torch.arange(60, device=DEVICE) + 40 >= key
+    assert with_one[sees, 2:].isnan().all()
+    assert torch.equal(with_one[~sees], without[~sees]) and torch.equal(with_one[:, :2], without[:, :2])

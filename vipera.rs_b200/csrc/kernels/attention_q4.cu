@@ -621,7 +621,10 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) attention_q4_clu
   int token = entry;
   if (p.entry_starts) {
     token = p.entry_starts[entry];
-    if (p.entry_starts[entry + 1] - token != 1) return;   // the whole cluster's
+    if (p.entry_starts[entry + 1] - token != 1) {   // the whole cluster's; a grid without an entry must not end before the kernels ahead
+      if (p.settled && entry == 0) pdl_wait();
+      return;
+    }
   }
   const Visible seen(p, p.positions[entry]);
   const int each = (seen.tiles + 8 * p.shares - 1) / (8 * p.shares) * 8;      // of a block: whole steps of its warps

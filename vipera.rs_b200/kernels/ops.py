@@ -1101,11 +1101,22 @@ class _RowsQ4Params(ctypes.Structure):
                 ("keep_first", _c_int), ("chunk", _c_int), ("num_splits", _c_int)]
 
 
+class _PortionsQ4Params(ctypes.Structure):
+    _fields_ = [("q", _c_void), ("out", _c_void), ("k_codes", _c_void), ("v_codes", _c_void), ("k_scales", _c_void), ("v_scales", _c_void),
+                ("entry_starts", _c_void), ("entry_pos0", _c_void), ("block_table", _c_void), ("sink_values", _c_void), ("gate", _c_void),
+                ("gate_stride", ctypes.c_longlong), ("partial_ml", _c_void), ("partial_out", _c_void), ("status", _c_void),
+                ("gate_per_head", _c_int), ("sink", _c_int), ("table_width", _c_int), ("page_size", _c_int), ("num_pages", _c_int),
+                ("num_entries", _c_int), ("num_tokens", _c_int), ("num_heads", _c_int), ("num_kv_heads", _c_int), ("head_dim", _c_int),
+                ("scale", _c_float), ("window", _c_int), ("keep_first", _c_int), ("chunk", _c_int), ("num_splits", _c_int),
+                ("skip_single", _c_int), ("block_rows", _c_int)]
+
+
 # argument types of the launchers (a parameter block is handed over by reference)
 _MAPS_ARGS = [ctypes.POINTER(_MapsParams), _c_void]
 _STORE_Q4_ARGS = [ctypes.POINTER(_StoreQ4Params), _c_int, _c_void]
 _EXPAND_Q4_ARGS = [ctypes.POINTER(_ExpandQ4Params), _c_int, _c_int, _c_void]
 _DECODE_Q4_ARGS = [ctypes.POINTER(_DecodeQ4Params), _c_void, ctypes.c_size_t, _c_int, _c_void]
+_PORTIONS_Q4_ARGS = [ctypes.POINTER(_PortionsQ4Params), _c_void, _c_void, ctypes.c_size_t, _c_void]
 _ROWS_Q4_ARGS = [ctypes.POINTER(_RowsQ4Params), _c_void, _c_int, _c_int, _c_void, _c_int, _c_void, _c_void, ctypes.c_longlong, _c_int,
                  _c_void, ctypes.c_size_t, _c_void]
 
@@ -1320,20 +1331,19 @@ def _attention_q4_decode(q, out, pages, *, positions, block_table, num_heads, nu
 Q4_ROWS = {(torch.float32, 128): 8, (torch.float32, 64): 16, (torch.bfloat16, 128): 16, (torch.bfloat16, 64): 16}   # (token, head) rows of a block
 
 
-# bfloat16 portions of few (token, head) rows read the packed pages; more of them pay for rows that are expanded once and read by the
-# flash kernel, whose blocks of 128 tokens and a head walk a whole history each.  Fitted to both forms timed at 28, 12 and 14 heads (the
-# latter of 64), 1 and 8 requests, 2 to 256 tokens each behind 0 to 20,000: one request of 64 tokens and 28 heads behind 4,000
-# keys takes 66 and 86 microseconds, of 128 tokens 115 and 63; eight of 16 behind 4,000 keys 121 and 199, of 64 342 and 199.
-Q4_ROWS_FIRST, Q4_ROWS_MORE, Q4_ROWS_HALF = 1800, 15, 1.4
+# bfloat16 portions of little work (rows times keys) and few requests are shared by the blocks of the kernel of any number of rows; the
+# tensor cores' kernel has a longer start and more behind it.  12 heads of 128, one request: 64 tokens behind 500 take 20 and 24
+# microseconds, 128 tokens 27 and 27, 16 behind 4,000 22 and 22, 64 41 and 33; eight requests of 4 behind 500 18 and 18, of 64 51 and 25.
+Q4_ROWS_WORK, Q4_ROWS_HALF, Q4_ROWS_PORTIONS = 1e6, 1.4, 2
 
 
-def attention_q4_takes_rows(dtype: torch.dtype, head_dim: int, page_size: int, rows: int, heads: int, portions: int) -> bool:
-    """Whether a step of `rows` (token, head) rows, portions of `portions` requests, reads the packed pages: 32-bit steps always do (where
-    the heads and pages are those the kernel is built for), bfloat16 ones with few rows."""
+def attention_q4_takes_rows(dtype: torch.dtype, head_dim: int, page_size: int, rows: int, max_keys: int, portions: int) -> bool:
+    """Whether a step of `rows` (token, head) rows, portions of `portions` requests, is the kernel's of any number of rows: 32-bit steps
+    always are (where the heads and pages are those the kernel is built for), bfloat16 ones with little to do."""
     if head_dim not in MMA_HEAD_DIMS or page_size % 16:
         return False
-    most = (Q4_ROWS_FIRST + Q4_ROWS_MORE * heads * (portions - 1)) * (Q4_ROWS_HALF if head_dim == 64 else 1.0)
-    return dtype == torch.float32 or (Q4_ROWS_FIRST > 0 and rows <= most)
+    most = Q4_ROWS_WORK * (Q4_ROWS_HALF if head_dim == 64 else 1.0)
+    return dtype == torch.float32 or (portions <= Q4_ROWS_PORTIONS and rows * max_keys <= most)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -1365,6 +1375,66 @@ def _attention_q4_rows(q, out, pages, *, entry_starts, entry_pos0, positions, bl
                       chunk, splits)
     _check(fn(p, out_at, dtype_code(dtype), head_dim, positions_at, 1 if sink else 0, sinks, gate_pointer, gate_stride,
               1 if gate_per_head else 0, scratch.data_ptr(), scratch.numel(), _stream_of(here)), "attention", kernels=2)
+
+
+def attention_q4_takes_portions(dtype: torch.dtype, head_dim: int, page_size: int) -> bool:
+    """Whether the tensor cores' kernel unpacks a step's pages itself."""
+    return (dtype == torch.bfloat16 and head_dim in TC_ATTENTION_HEAD_DIMS and page_size % 16 == 0 and
+            os.environ.get("VIPERA_ATTENTION_TC", "1") != "0")
+
+
+# The tensor cores' kernel in microseconds: a block's start and ending, 128 keys of a block of two tiles of rows and of one, a part of a row to be
+# written and joined, the joining launch; by head size (fitted to launches of 12, 14 and 28 heads, 1 and 4 requests of 8 to 2,048 tokens
+# behind 0 to 8,000).
+Q4_PORTION_TIMES = {128: (10.0, 2.45, 2.15, 0.00063, 6.0), 64: (9.0, 2.15, 1.72, 0.0004, 5.0)}
+Q4_PORTION_CUTS = (1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48)
+
+
+@functools.lru_cache(maxsize=4096)
+def q4_portion_plan(tokens: int, num_heads: int, num_kv_heads: int, head_dim: int, max_keys: int, window: int, sm_count: int):
+    """How the tensor cores' kernel cuts a step: (rows of a block, keys of a cut, cuts), the choice that a model of the launch's time likes
+    best.  A block of 256 rows unpacks a history once for two tiles of rows, blocks of 128 are twice as many; histories are cut where blocks
+    are few.  28 heads of 128, 2,048 tokens: 57 us with 256 rows and 82 with 128; 12 heads 53 and 45; 28 heads, 100 tokens behind 8,000: 166
+    and 137 in one piece, 45 in cuts of 1,024 keys; 512 tokens behind 8,000 176 and 145, 123 in cuts of 2,048 (of 256 rows, 168 of 128)."""
+    fixed, two, one, part, joining = Q4_PORTION_TIMES[head_dim]
+    seen = min(max_keys, window + tokens) if window else max_keys
+    cuts = Q4_PORTION_CUTS if 2 * seen >= max_keys else (1,)
+    mean = seen - min(seen, tokens) / 2           # as if all tokens were one request's
+    best = None
+    for rows, each in ((256, two), (128, one)):
+        blocks = num_kv_heads * -(-tokens * (num_heads // num_kv_heads) // rows)
+        for count in cuts:
+            chunk = 128 * -(-max_keys // (128 * count))
+            if count > 1 and chunk < 256:
+                break
+            time = max(fixed + min(chunk, seen) / 128 * each, blocks * (mean / 128 * each + fixed * max(1.0, count * mean / seen)) / sm_count)
+            if count > 1:
+                time += joining + tokens * num_heads * count * part
+            if best is None or time < best[0] - 1e-9:
+                best = (time, rows, chunk)
+    return best[1], best[2], -(-max_keys // best[2])
+
+
+def _attention_q4_portions(q, out, pages, *, entry_starts, entry_pos0, positions, block_table, num_heads, num_kv_heads, head_dim, scale,
+                           max_keys, workspace, window, keep_first, sink, sink_values, gate, gate_offset, gate_per_head, skip_single) -> None:
+    fn = _function("attention_q4_tc", "vipera_attention_q4_portions", _PORTIONS_Q4_ARGS)
+    _check_struct("attention_q4_tc", "vipera_attention_q4_portions_params_size", _PortionsQ4Params)
+    here, int32, what = torch.cuda.current_device(), torch.int32, "attention_q4"
+    count, entries = q.shape[0], entry_pos0.numel()
+    rows, chunk, splits = q4_portion_plan(count, num_heads, num_kv_heads, head_dim, max_keys, window, _sm_count_of(here))
+    places, scratch = splits + (1 if keep_first else 0), None
+    if places > 1:
+        scratch = workspace.get("attention.partials", (attention_decode_scratch_floats(count, num_heads, head_dim, places),), torch.float32)
+    gate_pointer, gate_stride = (None, 0) if gate is None else _gate_pointer(
+        gate, gate_offset, count, num_heads * (1 if gate_per_head else head_dim), what)
+    sinks, = _places(what, torch.float32, here, sink_values)
+    starts_at, pos0_at, table_at, positions_at = _places(what, int32, here, entry_starts, entry_pos0, block_table, positions)
+    p = _PortionsQ4Params(*_places(what, torch.bfloat16, here, q, out), *_place_pages(what, pages, here), starts_at, pos0_at, table_at, sinks,
+                          gate_pointer, gate_stride, None, None, kernel_status_word(q.device).data_ptr(), 1 if gate_per_head else 0,
+                          1 if sink else 0, block_table.shape[1], pages.k_codes.shape[2], pages.k_codes.shape[0], entries, count, num_heads,
+                          num_kv_heads, head_dim, scale, window, keep_first, chunk, splits, 1 if skip_single else 0, rows)
+    _check(fn(p, positions_at, None if scratch is None else scratch.data_ptr(), 0 if scratch is None else scratch.numel(), _stream_of(here)),
+           "attention", kernels=2 if places > 1 else 1)
 
 
 def attention_q4(q: torch.Tensor, out: torch.Tensor, pages: Q4Pages, *, entry_starts: torch.Tensor, entry_pos0: torch.Tensor,
@@ -1411,9 +1481,17 @@ def attention_q4(q: torch.Tensor, out: torch.Tensor, pages: Q4Pages, *, entry_st
         _attention_q4_decode(q, out, pages, positions=positions, block_table=block_table, max_keys=max_keys, workspace=workspace, settled=settled,
                              entry_starts=None, **heads, **endings)
         return
-    if attention_q4_takes_rows(q.dtype, head_dim, page_size, count * num_heads, num_heads, 1 if any_single else entries):
+    if attention_q4_takes_rows(q.dtype, head_dim, page_size, count * num_heads, max_keys, 1 if any_single else entries):
         _attention_q4_rows(q, out, pages, entry_starts=entry_starts, entry_pos0=entry_pos0, positions=positions, block_table=block_table,
                            max_keys=max_keys, workspace=workspace, **heads, **endings)
+        return
+    if attention_q4_takes_portions(q.dtype, head_dim, page_size):
+        apart = any_single      # single tokens beside portions are the other kernel's
+        _attention_q4_portions(q, out, pages, entry_starts=entry_starts, entry_pos0=entry_pos0, positions=positions, block_table=block_table,
+                               max_keys=max_keys, workspace=workspace, skip_single=apart, **heads, **endings)
+        if apart:
+            _attention_q4_decode(q, out, pages, positions=entry_pos0, block_table=block_table, max_keys=max_keys, workspace=workspace,
+                                 settled=settled, entry_starts=entry_starts, **heads, **endings)
         return
     # what the flash kernels know of endings decides whether portions are theirs (see parts/attention.py)
     extended = sink_values is not None or gate is not None

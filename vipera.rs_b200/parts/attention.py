@@ -60,7 +60,7 @@ class GQAttention(Mixer):
     buffer they are in).  Pages of 4 bits (a ``PagedQ4View``) are taken where ``_takes_four_bits`` says: keys and values of one
     size of whole groups of 32, windows, kept first keys, sinks, gates and every position encoding among the options."""
 
-    kernels = ("rope_cache", "attention", "attention_mma", "attention_tc", "cache_q4", "attention_q4")
+    kernels = ("rope_cache", "attention", "attention_mma", "attention_tc", "cache_q4", "attention_q4", "attention_q4_tc")
     takes_lazy_input = True
     leaves_rows = True   # forward(ctx, h, None, ...) returns (rows [tokens, hidden] float32, 1)
     # With mixed head weights: steps of this many tokens and more that bring portions run every
@@ -243,7 +243,7 @@ class GQAttention(Mixer):
         if self._takes_four_bits(self.params):
             own.append("cache_q4")
             if self.dtype == torch.bfloat16 and self.head_dim in ops.MMA_HEAD_DIMS:
-                own.append("attention_q4")
+                own += ["attention_q4", "attention_q4_tc"]
         if self.talk is not None:
             own.append("attention_talk")
             if self.dtype == torch.bfloat16 and self.head_dim in ops.MMA_HEAD_DIMS and self.value_dim == self.head_dim:
