@@ -161,11 +161,11 @@ def test_the_memory_plan_counts_packed_pages_and_one_slots_room():
         assert packed["kv_bytes"] * 32 == run["kv_bytes"] * 9 and packed["kv_bytes_per_token"] * 32 == run["kv_bytes_per_token"] * 9
         room = packed["workspace_bytes"] - run["workspace_bytes"]
         assert room == planner.room_bytes(spec, 256, 3, 2) > 0
-    # A's two layers are alike: the room is one layer's pages, and one page more
-    spec = _spec(helpers.CONFIGS["A"])
-    assert planner.room_bytes(spec, 256, 3, 2) == planner.cache_bytes(spec, 256, 3, 2) // 2 + 16 * 2 * 2 * 64 * 2
-    # 32-bit steps keep (outputs, maximum, sum) of every token and head
-    assert planner.room_bytes(spec, 256, 3, 4) == 2 * planner.room_bytes(spec, 256, 3, 2) + planner.PLANNED_STEP_TOKENS * 4 * (64 + 2) * 4
+    # (outputs, maximum, sum) of every token and head of a step; A's heads of 64 are read packed
+    spec, parts = _spec(helpers.CONFIGS["A"]), planner.PLANNED_STEP_TOKENS * 4 * (64 + 2) * 4
+    assert planner.room_bytes(spec, 256, 3, 2) == planner.room_bytes(spec, 256, 3, 4) == parts
+    # in pages that the kernels do not read, one layer's of the two alike, and one page more
+    assert planner.room_bytes(spec, 256, 3, 2, page_size=8) == planner.cache_bytes(spec, 256, 3, 2) // 2 + 8 * 2 * 2 * 64 * 2 + parts
 
 
 def test_models_whose_mixers_need_the_runs_type_refuse_4_bits():
@@ -241,3 +241,26 @@ def test_the_command_line_plans_packed_pages(tmp_path, capsys):
         else:
             run, packed = (json.loads(p.out) for p in plans)
             assert packed["kv_bytes"] * 32 == run["kv_bytes"] * 9
+
+
+def test_how_the_tensor_cores_kernel_is_cut(entry_points):
+    """Whole cuts of 128 keys that cover what is seen, few enough for their places, one where a window leaves little of a history."""
+    ops = entry_points
+    rng = np.random.default_rng(3)
+    for _ in range(300):
+        d, kv_heads, group = int(rng.choice([64, 128])), int(rng.integers(1, 9)), int(rng.integers(1, 17))
+        tokens = int(2 ** rng.uniform(0, 13))
+        seen = tokens + int(2 ** rng.uniform(0, 17))
+        window = int(rng.choice([0, 0, 500]))
+        rows, keys, cuts = ops.q4_portion_plan(tokens, kv_heads * group, kv_heads, d, seen, window, 148)
+        assert rows in (128, 256) and keys % 128 == 0 and 1 <= cuts <= 127 and (cuts - 1) * keys < seen <= cuts * keys
+        assert cuts == 1 or keys >= 256
+        if window and 2 * (window + tokens) < seen:
+            assert cuts == 1
+    # blocks enough for the device: two tiles of rows each, in one piece; few rows behind a long history: in many
+    assert ops.q4_portion_plan(2048, 28, 4, 128, 2048, 0, 148) == (256, 2048, 1)
+    assert ops.q4_portion_plan(8, 28, 4, 128, 20008, 0, 148)[2] >= 8
+    assert not ops.attention_q4_takes_portions(torch.float32, 128, 16) and not ops.attention_q4_takes_portions(torch.bfloat16, 96, 16)
+    assert not ops.attention_q4_takes_portions(torch.bfloat16, 128, 24)
+    assert ops.attention_q4_takes_rows(torch.float32, 128, 16, 10 ** 6, 10 ** 6, 50) and not ops.attention_q4_takes_rows(torch.float32, 96, 16, 1, 1, 1)
+    assert ops.attention_q4_takes_rows(torch.bfloat16, 128, 16, 60, 500, 1) and not ops.attention_q4_takes_rows(torch.bfloat16, 128, 16, 60, 500, 3)

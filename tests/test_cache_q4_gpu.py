@@ -636,3 +636,20 @@ def test_keys_that_are_not_finite_show_in_the_rows_that_see_them(ops, form):
     sees = torch.arange(60, device=DEVICE) + 40 >= key
     assert with_one[sees, 2:].isnan().all()
     assert torch.equal(with_one[~sees], without[~sees]) and torch.equal(with_one[:, :2], without[:, :2])
+
+
+@pytest.mark.parametrize("settled", [False, True])
+def test_a_step_that_was_said_to_hold_single_tokens_and_does_not(ops, monkeypatch, settled):
+    """The single tokens' kernel finds nothing to do; what follows must still see the portions' outputs."""
+    monkeypatch.setattr(ops, "Q4_ROWS_WORK", 0)
+    step = Step([150, 70], [900, 0], 16)
+    pages = ops.Q4Pages(*plain.make_pages(step.num_pages, 16, 2, 128, 3, DEVICE))
+    q = torch.randn(220, 8 * 128, device=DEVICE).to(torch.bfloat16)
+    described = dict(step.device(), any_single=True)
+    outs = []
+    for said in (False, True):
+        out = torch.zeros_like(q)
+        ops.attention_q4(q, out, pages, num_heads=8, num_kv_heads=2, head_dim=128, scale=0.09, workspace=_workspace(), settled=settled,
+                         **dict(described, any_single=said))
+        outs.append(out.clone())
+    assert torch.equal(outs[0], outs[1]) and outs[0].abs().amax() > 0

@@ -7,8 +7,8 @@
 // as their sums; bfloat16 steps round a weight once.  The query's parts lie in shared memory.
 //
 // What bounds it: issuing, and for short steps the latency of one walk.  Rows times keys go by at 1.7e5 a microsecond with heads of
-// 128 in bfloat16, so that the flash kernel behind an expansion wins beyond a size (ops.attention_q4_takes_rows has the rule and both sides'
-// times).  384 rows of 32 bits over 96 to 2,113 keys: 15 us and 6 for the parts' ending, from a cold cache.
+// 128 in bfloat16, so that the tensor cores' kernel (attention_q4_tc.cu) wins beyond a size (ops.attention_q4_takes_rows has the rule and
+// both sides' times).  384 rows of 32 bits over 96 to 2,113 keys: 15 us and 6 for the parts' ending, from a cold cache.
 #pragma once
 
 namespace {

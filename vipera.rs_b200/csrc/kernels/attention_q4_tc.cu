@@ -3,25 +3,35 @@
 //
 // A block is 256 of the (token, query head) rows of one request and KV head, two tiles of 128, and a split of the keys; both tiles use
 // every 128 keys and values that the block unpacks.  (A tile of 128 tokens of one head would unpack a history group times as often, and
-// a portion of a few tokens would leave its rows empty: 18 tokens of 7 heads fill one tile.)
+// a portion of a few tokens would leave its rows empty: 18 tokens of 7 heads fill one tile.)  A chain of work goes with each: softmax warps,
+// scores and output in tensor memory, an issuing warp.  Scores are computed 64 keys at a time into two places in turn, so that a chain's
+// products run while it computes the weights of the 64 before.  Where a block has one tile of rows, both chains work at it, each at every
+// second 64 keys, and join their outputs at the end.
 //
 //   unpacking  four warps, a thread a key: the next 128 rows' codes are asked for while these become bfloat16 numbers, exactly: u of a
 //              code moved to the top of the fraction under 0x4180 is 16 + u, and (16 + u) s - 24 s = (u - 8) s in one rounding,
 //              which rounds nothing.  Shared rows are 128 bytes with the 16-byte pieces swizzled; a value's
 //              channels lie in the order in which its word holds them (a channel of group g beside the same one of group g + 1),
 //              which orders the output's columns and is undone when they leave.
-//   scores     S = Q K^T, tcgen05.mma 128 x 128 x d for each tile.
-//   softmax    a thread a row: two passes over the 128 scores (the largest; weights and their sum, in 32 bits).  The maximum
-//              follows when it has grown by 2^8, so that the outputs are rarely rescaled.  Weights go back to tensor memory as bfloat16,
-//              over the scores, and are the left operand from there: shared memory, whose rate bounds products of two shared
+//   scores     S = Q K^T, tcgen05.mma 128 x 64 x d.
+//   softmax    a thread a row: the largest of 64 scores, then weights and their sum, in 32 bits.  The maximum follows when it has
+//              grown by 2^8, so that the outputs are rarely rescaled.  Weights go back to tensor memory as bfloat16, over the
+//              scores, and are the left operand from there: shared memory, whose rate bounds products of two shared
 //              operands of 128 rows, then feeds this product's right one alone.
-//   output     O += P V, 128 x d x 128 in tensor memory.  S, S, O and O of 128 columns are all of it.
+//   output     O += P V, 128 x d x 64 in tensor memory.  S, S, O and O of 128 columns are all of it.
 //
 // A block whose rows are all there is (one split) writes them; else maxima, sums and outputs go to `partial_ml` and `partial_out`, and a second
 // kernel joins them (kept first keys are a split of their own, as in attention_q4_rows.cuh).  Rows that hold no visible key of the block
 // are zeros and are never read.  A value's group that is not finite is held as zeros, and its key is noted for the softmax, which makes the
 // outputs NaN of the rows that see it and of no other.  Every wait is bounded: one that runs out leaves an error in the
 // status word, and every role runs to its end.
+//
+// What bounds it.  2,048 tokens of 28 heads of 128 on 4: 55 us from a cold cache, 544 TFLOP/s (a third of the measured rate; expanding and the
+// flash kernel take 72).  A block takes 5 us to its first scores and 2.5 to its ending, and 4,200 clocks for 128 keys of its 256 rows: the
+// exponentials alone are 2,048 (16 a clock), the products 2,048 to 2,560, and both chains' softmax warps and the unpacking ones share the
+// issue slots, of which that takes 2,700.  Without the rows' loads 51 us, without the exponentials 55, without both 47.  Scores of 128 keys
+// at once, weights and products one behind the other, took 6,000 clocks, with the products of both tiles from one warp in turn 4,700; rows asked for
+// a whole tile ahead 4 % longer (registers).  A lone block's 128 keys of 128 rows take 2 us: the unpacking warps' loads and work.
 #include "attention_combine.cuh"
 #include "q4.cuh"
 #include "tcgen05.cuh"
@@ -63,9 +73,10 @@ struct Job {
 };
 
 struct Shared {
-  uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2][2], p_full[2][2], pv_done[2][2];      // the last three by tile and half
+  uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2][2], p_full[2][2], pv_done[2][2];      // the last three by chain and buffer
   uint4 bad_any[4];                // of the last four tiles of keys: those with a group of values that is not finite
   uint32_t bad[4][4][4];           // [tile & 3][group][32 keys]
+  float4 told[2][kTileRows];       // a pair's chains: maximum, sum and noted groups of every row
   uint32_t tmem;
   int abort_flag;
   Job job;
@@ -321,12 +332,14 @@ __global__ void __launch_bounds__(kThreads, 1) attention_q4_portions_kernel(cons
   }
   const int first_tile = begin / kKeys, num_tiles = (end + kKeys - 1) / kKeys - first_tile;
   const int steps = (end - first_tile * kKeys + 63) / 64;       // of 64 keys
-  const int tiles_here = job.rows > kTileRows ? 2 : 1;
+  // One tile of rows only: both chains (softmax warps, scores, output, issuing warp) work at it, on every first and every second 64 keys.
+  const bool pair = job.rows <= kTileRows;
+  const auto steps_of = [&](int chain) { return !pair ? steps : (steps + 1 - chain) / 2; };
 
   if (warp < kSoftmaxWarps) {
     // ---------------- a thread a row ----------------
-    const int tile = warp >> 2, row = threadIdx.x & (kTileRows - 1), r = tile * kTileRows + row;
-    if (tile < tiles_here) {
+    const int chain = warp >> 2, tile = pair ? 0 : chain, row = threadIdx.x & (kTileRows - 1), r = tile * kTileRows + row, own_steps = steps_of(chain);
+    {
       const int used = min(r, job.rows - 1);        // rows behind the last compute what nobody reads
       const int token = job.token0 + (job.row0 + used) / group, head = kv_head * group + (job.row0 + used) % group;
       const int position = job.pos0 + (job.row0 + used) / group;
@@ -335,14 +348,16 @@ __global__ void __launch_bounds__(kThreads, 1) attention_q4_portions_kernel(cons
       // a warp's 32 rows, neighbouring lanes side by side in one row, all asked for before the first is stored
       const long long row_at = (static_cast<long long>(token) * p.num_heads + head) * D;
       const int warp_row = (warp & 3) * 32, piece_of = lane % kPieces, row_of = lane / kPieces;
-      uint4 asked[kPieces];
+      if (tile == chain) {
+        uint4 asked[kPieces];
 #pragma unroll
-      for (int i = 0; i < kPieces; ++i)
-        asked[i] = *reinterpret_cast<const uint4*>(p.q + __shfl_sync(0xffffffffu, row_at, i * (32 / kPieces) + row_of) + 8 * piece_of);
+        for (int i = 0; i < kPieces; ++i)
+          asked[i] = *reinterpret_cast<const uint4*>(p.q + __shfl_sync(0xffffffffu, row_at, i * (32 / kPieces) + row_of) + 8 * piece_of);
 #pragma unroll
-      for (int i = 0; i < kPieces; ++i) *reinterpret_cast<uint4*>(q_tile + piece_at(warp_row + i * (32 / kPieces) + row_of, piece_of)) = asked[i];
-      tcgen05::fence_async();
-      tcgen05::bar_arrive(&sh->q_full[tile]);
+        for (int i = 0; i < kPieces; ++i) *reinterpret_cast<uint4*>(q_tile + piece_at(warp_row + i * (32 / kPieces) + row_of, piece_of)) = asked[i];
+        tcgen05::fence_async();
+        tcgen05::bar_arrive(&sh->q_full[tile]);
+      }
       // what the row sees here, and what every row of the tile sees
       const int tile_last = min(tile * kTileRows + kTileRows, job.rows) - 1;
       const int tile_low_position = job.pos0 + (job.row0 + tile * kTileRows) / group, tile_high_position = job.pos0 + (job.row0 + tile_last) / group;
@@ -355,14 +370,14 @@ __global__ void __launch_bounds__(kThreads, 1) attention_q4_portions_kernel(cons
       }
       const float scale_log2 = p.scale * kLog2e;
       const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-      const uint32_t s_at = lanes + tile * 128, o_at = lanes + 256 + tile * 128;
+      const uint32_t s_at = lanes + chain * 128, o_at = lanes + 256 + chain * 128;
       float row_max = -INFINITY, row_sum = 0.0f;
       uint32_t bad_groups = 0;
-      for (int i = 0; i < steps; ++i) {
-        const int half = i & 1, key0 = first_tile * kKeys + 64 * i;
-        const uint32_t turn = (i >> 1) & 1, scores_at = s_at + 64 * half;
+      for (int n = 0; n < own_steps; ++n) {
+        const int i = pair ? 2 * n + chain : n, half = i & 1, key0 = first_tile * kKeys + 64 * i, buffer = n & 1;
+        const uint32_t scores_at = s_at + 64 * buffer;
         const bool edge = key0 < all_first || key0 + 63 > all_last;
-        wait(&sh->s_full[tile][half], turn, abort_flag, p.status);
+        wait(&sh->s_full[chain][buffer], (n >> 1) & 1, abort_flag, p.status);
         tcgen05::fence_after();
         uint32_t s[64];
         tensor_load_32(scores_at, s);
@@ -392,8 +407,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_q4_portions_kernel(cons
         const float shrink = new_max == row_max ? 1.0f : exp2_of(row_max - new_max);
         row_max = new_max;
         row_sum *= shrink;
-        if (i > 0 && __any_sync(0xffffffffu, shrink != 1.0f)) {
-          wait(&sh->pv_done[tile][half ^ 1], ((i - 1) >> 1) & 1, abort_flag, p.status);
+        if (n > 0 && __any_sync(0xffffffffu, shrink != 1.0f)) {
+          wait(&sh->pv_done[chain][buffer ^ 1], ((n - 1) >> 1) & 1, abort_flag, p.status);
           tcgen05::fence_after();
 #pragma unroll 1
           for (int c = 0; c < D; c += 16) {
@@ -422,26 +437,54 @@ __global__ void __launch_bounds__(kThreads, 1) attention_q4_portions_kernel(cons
         row_sum += sum_of_pair(sum[0]) + sum_of_pair(sum[1]);
         tensor_store_wait();
         tcgen05::fence_before();
-        tcgen05::bar_arrive(&sh->p_full[tile][half]);
+        tcgen05::bar_arrive(&sh->p_full[chain][buffer]);
       }
-      wait(&sh->pv_done[tile][(steps - 1) & 1], ((steps - 1) >> 1) & 1, abort_flag, p.status);
+      if (own_steps > 0) wait(&sh->pv_done[chain][(own_steps - 1) & 1], ((own_steps - 1) >> 1) & 1, abort_flag, p.status);
       tcgen05::fence_after();
+      // A pair's chains join: each has the rows' other half of the keys, and writes half of the columns.
+      float factor = own_steps > 0 ? 1.0f : 0.0f, other_factor = 0.0f;
+      const bool other_too = pair && steps_of(chain ^ 1) > 0;
+      const auto meet = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 3)) : "memory"); };
+      if (pair) {
+        sh->told[chain][row] = make_float4(row_max, row_sum, __uint_as_float(bad_groups), 0.0f);
+        tcgen05::fence_before();
+        meet();
+        tcgen05::fence_after();
+        const float4 other = sh->told[chain ^ 1][row];
+        const float best = fmaxf(row_max, other.x);
+        factor = row_max == -INFINITY ? 0.0f : exp2_of(row_max - best);
+        other_factor = other.x == -INFINITY ? 0.0f : exp2_of(other.x - best);
+        row_sum = (own_steps > 0 ? row_sum * factor : 0.0f) + (other_too ? other.y * other_factor : 0.0f);
+        row_max = best;
+        bad_groups |= __float_as_uint(other.z);
+      }
       const bool whole = p.partial_ml == nullptr;
       const size_t place = (static_cast<size_t>(token) * p.num_heads + head) * (p.num_splits + (p.keep_first > 0 ? 1 : 0)) + split;
-      float factor = 1.0f;
       if (whole) {
         if (p.sink) row_sum += exp2f((p.sink_values ? p.sink_values[head] * kLog2e : 0.0f) - row_max);
-        factor = 1.0f / row_sum;
-        if (p.gate && p.gate_per_head) factor *= 1.0f / (1.0f + __expf(-p.gate[static_cast<size_t>(token) * p.gate_stride + head]));
-      } else if (r < job.rows && !*abort_flag) {
+        float inverse = 1.0f / row_sum;
+        if (p.gate && p.gate_per_head) inverse *= 1.0f / (1.0f + __expf(-p.gate[static_cast<size_t>(token) * p.gate_stride + head]));
+        factor *= inverse;
+        other_factor *= inverse;
+      } else if (r < job.rows && tile == chain && !*abort_flag) {
         *reinterpret_cast<float2*>(p.partial_ml + 2 * place) = make_float2(row_max, row_sum);
       }
       const float* gate = p.gate && !p.gate_per_head ? p.gate + static_cast<size_t>(token) * p.gate_stride + static_cast<size_t>(head) * D : nullptr;
+      const uint32_t other_at = lanes + 256 + (chain ^ 1) * 128;
 #pragma unroll 1
-      for (int a = 0; a < D / 32; ++a) {
+      for (int a = pair ? chain * (D / 64) : 0; a < (pair ? (chain + 1) * (D / 64) : D / 32); ++a) {
         uint32_t o[32];
-        tensor_load_32(o_at + 32 * a, o);
+        if (own_steps > 0) tensor_load_32(o_at + 32 * a, o);
         tensor_load_wait();
+#pragma unroll
+        for (int k = 0; k < 32; ++k) o[k] = own_steps > 0 ? __float_as_uint(__uint_as_float(o[k]) * factor) : 0u;
+        if (other_too) {
+          uint32_t more[32];
+          tensor_load_32(other_at + 32 * a, more);
+          tensor_load_wait();
+#pragma unroll
+          for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(fmaf(__uint_as_float(more[k]), other_factor, __uint_as_float(o[k])));
+        }
 #pragma unroll
         for (int part = 0; part < 4; ++part) {     // eight neighbouring channels
           const int g = D == 128 ? part : part >> 1, piece = D == 128 ? 4 * part + a : 4 * (part >> 1) + 2 * a + (part & 1);
@@ -449,7 +492,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_q4_portions_kernel(cons
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const int word = D == 128 ? 2 * (i / 4) + g / 2 : 2 * (part & 1) + i / 4;
-            x[i] = __uint_as_float(o[8 * word + 2 * (i & 3) + (g & 1)]) * factor;
+            x[i] = __uint_as_float(o[8 * word + 2 * (i & 3) + (g & 1)]);
             if (bad_groups >> g & 1) x[i] = __int_as_float(0x7fffffff);
           }
           if (whole) {
@@ -470,16 +513,19 @@ __global__ void __launch_bounds__(kThreads, 1) attention_q4_portions_kernel(cons
         }
       }
       if (whole) {
-        __syncwarp();
+        if (pair) meet();
+        else __syncwarp();
         const bool failed = *abort_flag;
         uint4 done[kPieces];
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i) done[i] = *reinterpret_cast<const uint4*>(q_tile + piece_at(warp_row + i * (32 / kPieces) + row_of, piece_of));
+        for (int i = 0; i < kPieces; ++i)
+          if (!pair || i / (kPieces / 2) == chain) done[i] = *reinterpret_cast<const uint4*>(q_tile + piece_at(warp_row + i * (32 / kPieces) + row_of, piece_of));
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
           const int from = i * (32 / kPieces) + row_of;
           const long long at = __shfl_sync(0xffffffffu, row_at, from);
-          if (tile * kTileRows + warp_row + from < job.rows && !failed) *reinterpret_cast<uint4*>(p.out + at + 8 * piece_of) = done[i];
+          if ((!pair || i / (kPieces / 2) == chain) && tile * kTileRows + warp_row + from < job.rows && !failed)
+            *reinterpret_cast<uint4*>(p.out + at + 8 * piece_of) = done[i];
         }
       }
     }
@@ -574,48 +620,42 @@ __global__ void __launch_bounds__(kThreads, 1) attention_q4_portions_kernel(cons
       page = page_of(j + 2);
     }
   } else if (warp < kIssueWarp + 2) {
-    // ---------------- products of one tile of rows ----------------
-    const int tile = warp - kIssueWarp;
+    // ---------------- products of one chain ----------------
+    const int chain = warp - kIssueWarp, tile = pair ? 0 : chain, own_steps = steps_of(chain);
     constexpr uint32_t kTypes = (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(kTileRows >> 4) << 24);
     constexpr uint32_t kScores = kTypes | (static_cast<uint32_t>(64 >> 3) << 17);
     constexpr uint32_t kOutput = kTypes | (static_cast<uint32_t>(D >> 3) << 17) | (1u << 16);      // the right operand's inner axis runs down its rows
-    if (tile < tiles_here) {
-      const uint32_t q_at = shared_address(q_tiles + tile * kTile), s_at = tmem + tile * 128, o_at = tmem + 256 + tile * 128;
+    if (own_steps > 0) {
+      const uint32_t q_at = shared_address(q_tiles + tile * kTile), s_at = tmem + chain * 128, o_at = tmem + 256 + chain * 128;
       wait(&sh->q_full[tile], 0, abort_flag, p.status);
-      auto scores = [&](int i) {
-        const int j = i >> 1, half = i & 1, stage = j & 1;
+      auto scores = [&](int n) {
+        const int i = pair ? 2 * n + chain : n, j = i >> 1, half = i & 1, stage = j & 1, buffer = n & 1;
         const uint32_t k_at = shared_address(k_tiles + stage * kTile) + half * 64 * 128;
-        if (half == 0) wait(&sh->k_full[stage], (j >> 1) & 1, abort_flag, p.status);
-        if (j > 0) wait(&sh->pv_done[tile][half], (j - 1) & 1, abort_flag, p.status);     // the weights lie where these scores go
+        if (pair || half == 0) wait(&sh->k_full[stage], (j >> 1) & 1, abort_flag, p.status);
+        if (n >= 2) wait(&sh->pv_done[chain][buffer], ((n >> 1) - 1) & 1, abort_flag, p.status);     // the weights lie where these scores go
         tcgen05::fence_after();
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) {
           const uint32_t offset = static_cast<uint32_t>((ks >> 2) * kHalfBytes + (ks & 3) * 32);
-          tcgen05::mma_shared(s_at + 64 * half, operand_along(q_at + offset), operand_along(k_at + offset), kScores, ks > 0 ? 1u : 0u);
+          tcgen05::mma_shared(s_at + 64 * buffer, operand_along(q_at + offset), operand_along(k_at + offset), kScores, ks > 0 ? 1u : 0u);
         }
-        tcgen05::commit(&sh->s_full[tile][half]);
-        if (half == 1 || i == steps - 1) {
-          tcgen05::commit(&sh->k_empty[stage]);
-          if (tiles_here == 1) tcgen05::commit(&sh->k_empty[stage]);      // for the tile that is not there
-        }
+        tcgen05::commit(&sh->s_full[chain][buffer]);
+        if (pair || half == 1 || i == steps - 1) tcgen05::commit(&sh->k_empty[stage]);
       };
       scores(0);
-      if (steps > 1) scores(1);
-      for (int i = 0; i < steps; ++i) {
-        const int j = i >> 1, half = i & 1, stage = j & 1;
+      if (own_steps > 1) scores(1);
+      for (int n = 0; n < own_steps; ++n) {
+        const int i = pair ? 2 * n + chain : n, j = i >> 1, half = i & 1, stage = j & 1, buffer = n & 1;
         const uint32_t v_at = shared_address(v_tiles + stage * kTile) + half * 64 * 128;
-        if (half == 0) wait(&sh->v_full[stage], (j >> 1) & 1, abort_flag, p.status);
-        wait(&sh->p_full[tile][half], j & 1, abort_flag, p.status);
+        if (pair || half == 0) wait(&sh->v_full[stage], (j >> 1) & 1, abort_flag, p.status);
+        wait(&sh->p_full[chain][buffer], (n >> 1) & 1, abort_flag, p.status);
         tcgen05::fence_after();
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks)
-          mma_tensor(o_at, s_at + 64 * half + ks * 8, operand_down(v_at + ks * 2048), kOutput, (i > 0 || ks > 0) ? 1u : 0u);
-        tcgen05::commit(&sh->pv_done[tile][half]);
-        if (half == 1 || i == steps - 1) {
-          tcgen05::commit(&sh->v_empty[stage]);
-          if (tiles_here == 1) tcgen05::commit(&sh->v_empty[stage]);
-        }
-        if (i + 2 < steps) scores(i + 2);
+          mma_tensor(o_at, s_at + 64 * buffer + ks * 8, operand_down(v_at + ks * 2048), kOutput, (n > 0 || ks > 0) ? 1u : 0u);
+        tcgen05::commit(&sh->pv_done[chain][buffer]);
+        if (pair || half == 1 || i == steps - 1) tcgen05::commit(&sh->v_empty[stage]);
+        if (n + 2 < own_steps) scores(n + 2);
       }
     }
     tcgen05::fence_before();

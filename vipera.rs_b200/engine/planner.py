@@ -86,15 +86,14 @@ def kv_bytes_per_token(spec: ModelSpec, element_bytes: int, kv_type: Optional[st
 
 
 def room_bytes(spec: ModelSpec, ctx: int, batch: int, element_bytes: int, page_size: int = 16) -> int:
-    """What attention over pages of 4 bits expands a layer's rows to where it does not read them packed: one cache slot's pages in the
-    run's type, of the group where they are the largest (layers share the room); in 32-bit runs also the parts of a step's outputs."""
+    """What attention over pages of 4 bits needs beside them: the parts of a step's outputs, and, where it does not read them packed (heads
+    other than 64 and 128, pages not of a multiple of 16 tokens), a room to expand a layer's rows to: one cache slot's pages in the run's
+    type, of the group where they are the largest (layers share the room)."""
     groups, _ = plan_groups(spec_cache_requests(spec))
-    room = max((batch * _group_tokens(group, ctx, page_size) + page_size) * group.bytes_per_token(element_bytes) // len(group.slots)
-               for group in groups)
-    if element_bytes == 4:
-        parts = [part.params for layer in spec.layers for part in layer.parts.values()]
-        room += PLANNED_STEP_TOKENS * 4 * max(int(p.get("num_heads", 0)) * (int(p.get("head_dim", 0)) + 2) for p in parts)
-    return room
+    room = max([(batch * _group_tokens(group, ctx, page_size) + page_size) * group.bytes_per_token(element_bytes) // len(group.slots)
+                for group in groups if group.head_dim not in (64, 128) or page_size % 16] or [0])
+    parts = [part.params for layer in spec.layers for part in layer.parts.values()]
+    return room + PLANNED_STEP_TOKENS * 4 * max(int(p.get("num_heads", 0)) * (int(p.get("head_dim", 0)) + 2) for p in parts)
 
 
 def workspace_bytes(spec: ModelSpec, batch: int, element_bytes: int, tokens: int = PLANNED_STEP_TOKENS) -> int:

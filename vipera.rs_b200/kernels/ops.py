@@ -1386,7 +1386,7 @@ def attention_q4_takes_portions(dtype: torch.dtype, head_dim: int, page_size: in
 # The tensor cores' kernel in microseconds: a block's start and ending, 128 keys of a block of two tiles of rows and of one, a part of a row to be
 # written and joined, the joining launch; by head size (fitted to launches of 12, 14 and 28 heads, 1 and 4 requests of 8 to 2,048 tokens
 # behind 0 to 8,000).
-Q4_PORTION_TIMES = {128: (10.0, 2.45, 2.15, 0.00063, 6.0), 64: (9.0, 2.15, 1.72, 0.0004, 5.0)}
+Q4_PORTION_TIMES = {128: (10.0, 2.45, 1.95, 0.00063, 6.0), 64: (9.0, 2.15, 1.5, 0.0004, 5.0)}
 Q4_PORTION_CUTS = (1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48)
 
 
@@ -1394,8 +1394,8 @@ Q4_PORTION_CUTS = (1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48)
 def q4_portion_plan(tokens: int, num_heads: int, num_kv_heads: int, head_dim: int, max_keys: int, window: int, sm_count: int):
     """How the tensor cores' kernel cuts a step: (rows of a block, keys of a cut, cuts), the choice that a model of the launch's time likes
     best.  A block of 256 rows unpacks a history once for two tiles of rows, blocks of 128 are twice as many; histories are cut where blocks
-    are few.  28 heads of 128, 2,048 tokens: 57 us with 256 rows and 82 with 128; 12 heads 53 and 45; 28 heads, 100 tokens behind 8,000: 166
-    and 137 in one piece, 45 in cuts of 1,024 keys; 512 tokens behind 8,000 176 and 145, 123 in cuts of 2,048 (of 256 rows, 168 of 128)."""
+    are few.  28 heads of 128, 2,048 tokens: 57 us with 256 rows and 82 with 128; 12 heads 54 and 43; 28 heads, 64 tokens behind 8,000: 158
+    and 129 in one piece, 45 and 39 in cuts of 1,024 keys; 256 tokens behind 8,000 164 and 131, 66 and 90 in cuts of 2,048."""
     fixed, two, one, part, joining = Q4_PORTION_TIMES[head_dim]
     seen = min(max_keys, window + tokens) if window else max_keys
     cuts = Q4_PORTION_CUTS if 2 * seen >= max_keys else (1,)
@@ -1451,9 +1451,10 @@ def attention_q4(q: torch.Tensor, out: torch.Tensor, pages: Q4Pages, *, entry_st
     ``workspace.get(name, shape, dtype)`` gives rooms that the call may use until it is
     done on its stream.
 
-    With heads of 64 or 128 values and pages of a multiple of 16 tokens, single tokens, short portions and all of a 32-bit step are
-    attended over the packed pages.  Elsewhere the rows that the step sees are expanded to the run's type first (a room as large as one
-    layer's pages in that type) and the kernels for such pages attend."""
+    With heads of 64 or 128 values and pages of a multiple of 16 tokens every kernel reads the packed pages: the single tokens' one, that of
+    any number of rows (32-bit steps, short portions), the tensor cores' (other portions).  Elsewhere, and with VIPERA_ATTENTION_TC=0, the
+    rows that the step sees are expanded to the run's type first (a room as large as one layer's pages in that type) and the kernels for
+    such pages attend."""
     page_size = _check_q4_pages("attention_q4", pages, num_kv_heads, head_dim)
     count, entries = q.shape[0], entry_pos0.numel()
     if num_kv_heads <= 0 or num_heads % num_kv_heads or tuple(q.shape) != (count, num_heads * head_dim) or out.shape != q.shape \
