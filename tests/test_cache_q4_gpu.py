@@ -653,3 +653,46 @@ def test_a_step_that_was_said_to_hold_single_tokens_and_does_not(ops, monkeypatc
                          **dict(described, any_single=said))
         outs.append(out.clone())
     assert torch.equal(outs[0], outs[1]) and outs[0].abs().amax() > 0
+
+
+def test_mixed_steps_behind_their_writes_in_a_graph(ops, monkeypatch):
+    """Write, portions, single tokens, again and again without a pause: the single tokens' kernel starts while the portions' one runs, and
+    finds the step's own rows and queries."""
+    monkeypatch.setattr(ops, "Q4_ROWS_WORK", 0)
+    heads, kv_heads, d, steps = 8, 2, 128, 6
+    step = Step([300, 1, 1, 40, 1], [100, 700, 0, 30, 1500], 16)
+    tokens = sum(step.counts)
+    monkeypatch.setattr(ops, "q4_portion_plan", lambda *a: (128, 1 << 20, 1))
+    described, slots, room = step.device(), _int(step.slots), _workspace()
+    qkv = torch.randn(steps, tokens, (heads + 2 * kv_heads) * d, device=DEVICE)
+    start = plain.make_pages(step.num_pages, 16, kv_heads, d, 3, DEVICE)
+
+    def run(pause):
+        pages = ops.Q4Pages(*[t.clone() for t in start])
+        q, outs = (torch.zeros(steps, tokens, heads * d, dtype=torch.bfloat16, device=DEVICE) for _ in range(2))
+
+        def all_steps():
+            for i in range(steps):
+                ops.rope_cache_q4(qkv[i], q[i], pages, num_heads=heads, num_kv_heads=kv_heads, head_dim=d, positions=described["positions"],
+                                  cos=None, sin=None, style=ops.ROPE_NONE, slots=slots)
+                pause()
+                ops.attention_q4(q[i], outs[i], pages, num_heads=heads, num_kv_heads=kv_heads, head_dim=d, scale=0.09, workspace=room, **described)
+                pause()
+        return all_steps, outs
+
+    slow, expected = run(torch.cuda.synchronize)
+    slow()
+    fast, outs = run(lambda: None)
+    fast()
+    torch.cuda.synchronize()
+    assert torch.equal(outs, expected)
+    again, outs = run(lambda: None)
+    again()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        again()
+    for _ in range(3):
+        outs.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs, expected)

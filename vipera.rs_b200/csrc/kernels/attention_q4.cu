@@ -51,7 +51,9 @@ struct DecodeParams {
   int table_width, page_size, page_shift, num_pages, num_entries, num_heads, num_kv_heads, head_dim;
   float scale;
   int window, keep_first, sink, shares;
-  int settled;                    // positions, tables and earlier steps' rows are complete before the kernel ahead of this one begins
+  // 1: positions, tables and earlier steps' rows are complete before the kernel ahead of this one begins.  2: that kernel, of the same step's
+  // portions, lets this one begin once all that went before itself is complete, and shares nothing with it: this one waits for it at its end.
+  int settled;
   uint32_t magic;                 // set by the launcher
 };
 
@@ -611,7 +613,7 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) attention_q4_clu
   constexpr int kRow = D + 4;
   extern __shared__ __align__(128) uint8_t shared_at[];
   const Shared<D, NT> shared{shared_at};
-  if (!p.settled) {
+  if (p.settled == 0) {
     pdl_wait();
     pdl_launch_dependents();
   }
@@ -628,7 +630,7 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) attention_q4_clu
   }
   const Visible seen(p, p.positions[entry]);
   const int each = (seen.tiles + 8 * p.shares - 1) / (8 * p.shares) * 8;      // of a block: whole steps of its warps
-  walk<D, NT>(p, shared, seen, entry, token, kv_head, head0, min(share * each, seen.tiles), min((share + 1) * each, seen.tiles), !p.settled);
+  walk<D, NT>(p, shared, seen, entry, token, kv_head, head0, min(share * each, seen.tiles), min((share + 1) * each, seen.tiles), p.settled != 1);
   cluster_sync_all();
   const int heads_here = min(8 * NT, group - head0);
   const uint32_t joined_at = smem_addr(shared.joined());
@@ -643,6 +645,10 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) attention_q4_clu
     finish<D>(p, token, kv_head * group + head0 + h, column, join.best, join.total, join.value);
   }
   cluster_sync_all();   // nobody's shared memory goes while others read it
+  if (p.settled == 2) {
+    pdl_wait();
+    pdl_launch_dependents();
+  }
 }
 
 // Many pairs: the keys of all of them, in units of 8 tiles one pair behind the other, are dealt to the launch's blocks in even runs, so
@@ -669,8 +675,11 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) attention_q4_run
   const Shared<D, NT> shared{shared_at};
   __shared__ int positions[kRunEntries], ends[kRunEntries];    // ends: units up to and with an entry
   __shared__ int warp_units[kWarps];
-  pdl_wait();
-  pdl_launch_dependents();
+  if (p.settled != 2) {
+    pdl_wait();
+    pdl_launch_dependents();
+  }
+  const bool last = p.settled == 2 && blockIdx.x == 0;      // a grid that found nothing to do must not end before the kernels ahead
   const int group = p.num_heads / p.num_kv_heads, head_tiles = (group + 8 * NT - 1) / (8 * NT), pairs = p.num_kv_heads * head_tiles;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int whole = 0;
@@ -701,7 +710,10 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) attention_q4_run
   }
   const long long all = static_cast<long long>(whole) * pairs;
   const long long runs = min(static_cast<long long>(gridDim.x), all);     // each with a unit at least
-  if (blockIdx.x >= runs) return;
+  if (blockIdx.x >= runs) {
+    if (last) pdl_wait();
+    return;
+  }
   long long at = all * blockIdx.x / runs;
   const long long stop = all * (blockIdx.x + 1) / runs;
   int entry = 0;                                   // in which the run begins: the first that ends behind it
@@ -712,7 +724,10 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) attention_q4_run
   }
   const auto units_at = [&](int e) { return ends[e] - (e > 0 ? ends[e - 1] : 0); };
   int units = units_at(entry);
-  if (units == 0) return;
+  if (units == 0) {
+    if (last) pdl_wait();
+    return;
+  }
   const int into = static_cast<int>(at - static_cast<long long>(ends[entry] - units) * pairs);
   int pair = into / units, unit = into - pair * units;
   while (at < stop && entry < p.num_entries) {
@@ -748,6 +763,10 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) attention_q4_run
       do ++entry;
       while (entry < p.num_entries && (units = units_at(entry)) == 0);
     }
+  }
+  if (p.settled == 2) {
+    pdl_wait();
+    pdl_launch_dependents();
   }
 }
 

@@ -317,7 +317,6 @@ __global__ void __launch_bounds__(kThreads, 1) attention_q4_portions_kernel(cons
   tcgen05::fence_after();
   const uint32_t tmem = sh->tmem;
   const Job job = sh->job;
-  pdl_launch_dependents();     // not before every block has its tensor memory: a kernel behind this one that took it would wait for this one's end
   // visible keys of the block's rows in this split: those from `begin` up to `end`
   const bool kept_split = split == p.num_splits;
   const int low_position = job.pos0 + job.row0 / group, high_position = job.pos0 + (job.row0 + job.rows - 1) / group;
@@ -345,6 +344,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_q4_portions_kernel(cons
       const int position = job.pos0 + (job.row0 + used) / group;
       uint8_t* q_tile = q_tiles + tile * kTile;
       pdl_wait();
+      // The kernel behind may start from here on: not before every block has its tensor memory (one that took it would wait for this one's end),
+      // and with what went before this kernel complete, so that the step's single tokens, which share nothing with the portions, need
+      // not wait for them (DecodeParams::settled in attention_q4.cu).
+      pdl_launch_dependents();
       // a warp's 32 rows, neighbouring lanes side by side in one row, all asked for before the first is stored
       const long long row_at = (static_cast<long long>(token) * p.num_heads + head) * D;
       const int warp_row = (warp & 3) * 32, piece_of = lane % kPieces, row_of = lane / kPieces;

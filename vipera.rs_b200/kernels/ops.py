@@ -1321,7 +1321,7 @@ def _attention_q4_decode(q, out, pages, *, positions, block_table, num_heads, nu
     p = _DecodeQ4Params(*_places(what, torch.bfloat16, here, q, out), *_place_pages(what, pages, here),
                         *_places(what, int32, here, positions, block_table, entry_starts), sinks, gate_pointer, gate_stride,
                         1 if gate_per_head else 0, width, pages.k_codes.shape[2], 0, pages.k_codes.shape[0], entries,
-                        num_heads, num_kv_heads, head_dim, scale, window, keep_first, 1 if sink else 0, shares, 1 if settled else 0, 0)
+                        num_heads, num_kv_heads, head_dim, scale, window, keep_first, 1 if sink else 0, shares, int(settled), 0)
     if shares:
         _check(fn(p, None, 0, 0, _stream_of(here)), "attention_decode")
     else:
@@ -1416,7 +1416,8 @@ def q4_portion_plan(tokens: int, num_heads: int, num_kv_heads: int, head_dim: in
 
 
 def _attention_q4_portions(q, out, pages, *, entry_starts, entry_pos0, positions, block_table, num_heads, num_kv_heads, head_dim, scale,
-                           max_keys, workspace, window, keep_first, sink, sink_values, gate, gate_offset, gate_per_head, skip_single) -> None:
+                           max_keys, workspace, window, keep_first, sink, sink_values, gate, gate_offset, gate_per_head, skip_single) -> int:
+    """Launches what the plan says and returns how many kernels those were."""
     fn = _function("attention_q4_tc", "vipera_attention_q4_portions", _PORTIONS_Q4_ARGS)
     _check_struct("attention_q4_tc", "vipera_attention_q4_portions_params_size", _PortionsQ4Params)
     here, int32, what = torch.cuda.current_device(), torch.int32, "attention_q4"
@@ -1435,6 +1436,7 @@ def _attention_q4_portions(q, out, pages, *, entry_starts, entry_pos0, positions
                           num_kv_heads, head_dim, scale, window, keep_first, chunk, splits, 1 if skip_single else 0, rows)
     _check(fn(p, positions_at, None if scratch is None else scratch.data_ptr(), 0 if scratch is None else scratch.numel(), _stream_of(here)),
            "attention", kernels=2 if places > 1 else 1)
+    return 2 if places > 1 else 1
 
 
 def attention_q4(q: torch.Tensor, out: torch.Tensor, pages: Q4Pages, *, entry_starts: torch.Tensor, entry_pos0: torch.Tensor,
@@ -1488,11 +1490,12 @@ def attention_q4(q: torch.Tensor, out: torch.Tensor, pages: Q4Pages, *, entry_st
         return
     if attention_q4_takes_portions(q.dtype, head_dim, page_size):
         apart = any_single      # single tokens beside portions are the other kernel's
-        _attention_q4_portions(q, out, pages, entry_starts=entry_starts, entry_pos0=entry_pos0, positions=positions, block_table=block_table,
-                               max_keys=max_keys, workspace=workspace, skip_single=apart, **heads, **endings)
-        if apart:
+        kernels = _attention_q4_portions(q, out, pages, entry_starts=entry_starts, entry_pos0=entry_pos0, positions=positions,
+                                         block_table=block_table, max_keys=max_keys, workspace=workspace, skip_single=apart, **heads,
+                                         **endings)
+        if apart:       # right behind the portions' kernel they need not wait for it (behind a joining one, which writes their rows, they do)
             _attention_q4_decode(q, out, pages, positions=entry_pos0, block_table=block_table, max_keys=max_keys, workspace=workspace,
-                                 settled=settled, entry_starts=entry_starts, **heads, **endings)
+                                 settled=2 if kernels == 1 else settled, entry_starts=entry_starts, **heads, **endings)
         return
     # what the flash kernels know of endings decides whether portions are theirs (see parts/attention.py)
     extended = sink_values is not None or gate is not None
