@@ -52,7 +52,8 @@ struct DecodeParams {
   float scale;
   int window, keep_first, sink, shares;
   // 1: positions, tables and earlier steps' rows are complete before the kernel ahead of this one begins.  2: that kernel, of the same step's
-  // portions, lets this one begin once all that went before itself is complete, and shares nothing with it: this one waits for it at its end.
+  // portions, lets this one begin once all that went before itself is complete, and shares nothing with it: this one waits for it at its end
+  // (portions of 512, 200 and 37 tokens beside 16 single ones behind 2,048: 57 us for 74).
   int settled;
   uint32_t magic;                 // set by the launcher
 };

@@ -26,12 +26,13 @@
 // outputs NaN of the rows that see it and of no other.  Every wait is bounded: one that runs out leaves an error in the
 // status word, and every role runs to its end.
 //
-// What bounds it.  2,048 tokens of 28 heads of 128 on 4: 55 us from a cold cache, 544 TFLOP/s (a third of the measured rate; expanding and the
-// flash kernel take 72).  A block takes 5 us to its first scores and 2.5 to its ending, and 4,200 clocks for 128 keys of its 256 rows: the
-// exponentials alone are 2,048 (16 a clock), the products 2,048 to 2,560, and both chains' softmax warps and the unpacking ones share the
-// issue slots, of which that takes 2,700.  Without the rows' loads 51 us, without the exponentials 55, without both 47.  Scores of 128 keys
+// What bounds it.  2,048 tokens of 28 heads of 128 on 4: 49 us, 57 from a cold cache, 617 and 525 TFLOP/s (of 1,661 measured; expanding and the
+// flash kernel take 69 and 73).  A block takes 5 us to its first scores and 2.5 to its ending, and 4,200 clocks for 128 keys of its 256
+// rows: the exponentials alone are 2,048 (16 a clock), the tensor cores are busy for 2,700 (products of 64 columns cost as much as of 128),
+// and both chains' softmax warps and the unpacking ones share the issue slots, of which they take 2,700.  Without the rows' loads 51 us, without the exponentials 55, without both 47.  Scores of 128 keys
 // at once, weights and products one behind the other, took 6,000 clocks, with the products of both tiles from one warp in turn 4,700; rows asked for
-// a whole tile ahead 4 % longer (registers).  A lone block's 128 keys of 128 rows take 2 us: the unpacking warps' loads and work.
+// a whole tile ahead 4 % longer (registers), eight unpacking warps 7 % longer there and 10 % shorter where blocks have one tile.  A lone
+// block's 128 keys of 128 rows take 2 us: the unpacking warps' loads and work.
 #include "attention_combine.cuh"
 #include "q4.cuh"
 #include "tcgen05.cuh"

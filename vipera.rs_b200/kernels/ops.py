@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import os
+import struct
 from typing import NamedTuple, Optional
 
 import torch
@@ -1111,13 +1112,25 @@ class _PortionsQ4Params(ctypes.Structure):
                 ("skip_single", _c_int), ("block_rows", _c_int)]
 
 
-# argument types of the launchers (a parameter block is handed over by reference)
-_MAPS_ARGS = [ctypes.POINTER(_MapsParams), _c_void]
-_STORE_Q4_ARGS = [ctypes.POINTER(_StoreQ4Params), _c_int, _c_void]
-_EXPAND_Q4_ARGS = [ctypes.POINTER(_ExpandQ4Params), _c_int, _c_int, _c_void]
-_DECODE_Q4_ARGS = [ctypes.POINTER(_DecodeQ4Params), _c_void, ctypes.c_size_t, _c_int, _c_void]
-_PORTIONS_Q4_ARGS = [ctypes.POINTER(_PortionsQ4Params), _c_void, _c_void, ctypes.c_size_t, _c_void]
-_ROWS_Q4_ARGS = [ctypes.POINTER(_RowsQ4Params), _c_void, _c_int, _c_int, _c_void, _c_int, _c_void, _c_void, ctypes.c_longlong, _c_int,
+def _packer(block):
+    """Packs a parameter block's fields, in their order, as its bytes (a third of what building the structure takes)."""
+    code = {_c_void: "P", _c_int: "i", _c_float: "f", ctypes.c_longlong: "q", ctypes.c_uint: "I"}
+    packed = struct.Struct("@" + "".join(code[kind] for _, kind in block._fields_) + "0q")
+    if packed.size != ctypes.sizeof(block):
+        raise InternalError(f"{block.__name__}: {packed.size} bytes packed, {ctypes.sizeof(block)} in the structure")
+    return packed.pack
+
+
+_pack_maps, _pack_store_q4, _pack_expand_q4, _pack_decode_q4, _pack_rows_q4, _pack_portions_q4 = (
+    _packer(block) for block in (_MapsParams, _StoreQ4Params, _ExpandQ4Params, _DecodeQ4Params, _RowsQ4Params, _PortionsQ4Params))
+
+# argument types of the launchers (a parameter block is handed over as its bytes)
+_MAPS_ARGS = [ctypes.c_char_p, _c_void]
+_STORE_Q4_ARGS = [ctypes.c_char_p, _c_int, _c_void]
+_EXPAND_Q4_ARGS = [ctypes.c_char_p, _c_int, _c_int, _c_void]
+_DECODE_Q4_ARGS = [ctypes.c_char_p, _c_void, ctypes.c_size_t, _c_int, _c_void]
+_PORTIONS_Q4_ARGS = [ctypes.c_char_p, _c_void, _c_void, ctypes.c_size_t, _c_void]
+_ROWS_Q4_ARGS = [ctypes.c_char_p, _c_void, _c_int, _c_int, _c_void, _c_int, _c_void, _c_void, ctypes.c_longlong, _c_int,
                  _c_void, ctypes.c_size_t, _c_void]
 
 
@@ -1132,11 +1145,11 @@ def _refuse_place(what: str, tensor: torch.Tensor, dtype: torch.dtype, here: int
 
 
 def _places(what: str, dtype: torch.dtype, here: int, *tensors) -> list:
-    """The addresses of contiguous tensors of `dtype` on device `here`, the current one, whose stream the launch goes to (None for None)."""
+    """The addresses of contiguous tensors of `dtype` on device `here`, the current one, whose stream the launch goes to (0 for None)."""
     out = []
     for tensor in tensors:
         if tensor is None:
-            out.append(None)
+            out.append(0)
             continue
         if tensor.dtype is not dtype or tensor.get_device() != here or not tensor.is_contiguous():
             _refuse_place(what, tensor, dtype, here)
@@ -1167,8 +1180,8 @@ def _check_q4_pages(what: str, pages: Q4Pages, num_kv_heads: int, head_dim: int)
         raise UnsupportedError(f"{what}: heads of 4 bits have a multiple of {Q4_GROUP} channels up to 256, not {head_dim}")
     k_codes, k_scales, v_codes, v_scales = pages
     shape, groups = k_codes.shape, k_scales.shape
-    if len(shape) != 4 or len(groups) != 4 or shape[1] != num_kv_heads or shape[3] * 2 != head_dim or v_codes.shape != shape \
-            or groups[3] * Q4_GROUP != head_dim or groups[:3] != shape[:3] or v_scales.shape != groups:
+    if len(shape) != 4 or shape[1] != num_kv_heads or shape[3] * 2 != head_dim or v_codes.shape != shape \
+            or groups != (shape[0], num_kv_heads, shape[2], head_dim // Q4_GROUP) or v_scales.shape != groups:
         raise InvalidArgumentError(f"{what}: pages of 4 bits are codes [pages, kv_heads, page_size, d / 2] and scales "
                                    "[pages, kv_heads, page_size, d / 32]")
     return shape[2]
@@ -1198,7 +1211,7 @@ def step_maps(entry_starts: torch.Tensor, entry_pos0: torch.Tensor, *, page_size
     if counts:
         raise InvalidArgumentError("step_maps: positions, token_entry and slots hold one number for each token")
     here, int32, what = torch.cuda.current_device(), torch.int32, "step_maps"
-    p = _MapsParams(*_places(what, int32, here, entry_starts, entry_pos0, page_starts, pages, block_table, positions, token_entry, slots),
+    p = _pack_maps(*_places(what, int32, here, entry_starts, entry_pos0, page_starts, pages, block_table, positions, token_entry, slots),
                     entries, tokens, 0 if pages is None else pages.numel(), block_table.shape[1], page_size)
     _check(fn(p, _stream_of(here)), what)
 
@@ -1233,8 +1246,8 @@ def rope_cache_q4(qkv: torch.Tensor, q_out: torch.Tensor, pages: Q4Pages, *, num
     if qkv.dtype is not torch.float32 or qkv.get_device() != here:     # its rows may lie apart
         raise InvalidArgumentError("rope_cache_q4: qkv must be float32 on the current CUDA device")
     positions_at, slots_at = _places(what, int32, here, positions, slots)
-    cos_at, sin_at = _places(what, torch.float32, here, cos, sin) if table_rows else (None, None)
-    p = _StoreQ4Params(qkv.data_ptr(), qkv.stride(0), *_places(what, q_out.dtype, here, q_out), *_place_pages(what, pages, here),
+    cos_at, sin_at = _places(what, torch.float32, here, cos, sin) if table_rows else (0, 0)
+    p = _pack_store_q4(qkv.data_ptr(), qkv.stride(0), *_places(what, q_out.dtype, here, q_out), *_place_pages(what, pages, here),
                        positions_at, cos_at, sin_at, slots_at, 0 if slots is None else pages.k_codes.shape[0] * page_size, table_rows, count,
                        num_heads, num_kv_heads, head_dim, rot_dims, style, page_size)
     _check(fn(p, dtype_code(q_out.dtype), _stream_of(here)), "rope_cache")
@@ -1258,7 +1271,7 @@ def expand_q4(pages: Q4Pages, k_room: torch.Tensor, v_room: torch.Tensor, *, ent
         raise InvalidArgumentError("expand_q4: entry_starts has one item more than entry_pos0, the block table a row for each entry")
     here, int32, what = torch.cuda.current_device(), torch.int32, "expand_q4"
     width = block_table.shape[1]
-    p = _ExpandQ4Params(*_place_pages(what, pages, here), *_places(what, k_room.dtype, here, k_room, v_room),
+    p = _pack_expand_q4(*_place_pages(what, pages, here), *_places(what, k_room.dtype, here, k_room, v_room),
                         *_places(what, int32, here, entry_starts, entry_pos0, block_table), width, page_size, entries, num_pages,
                         num_kv_heads, head_dim, max(int(window or 0), 0), int(keep_first or 0), 1 if skip_single else 0)
     _check(fn(p, dtype_code(k_room.dtype), min(4 * _sm_count_of(here), max(1, 2 * entries * width)), _stream_of(here)), what)
@@ -1300,7 +1313,7 @@ def q4_shares(pairs: int, seen: int, sm_count: int, runs: bool = True) -> int:
     return best[1]
 
 
-def _attention_q4_decode(q, out, pages, *, positions, block_table, num_heads, num_kv_heads, head_dim, scale, max_keys, workspace, settled, entry_starts,
+def _attention_q4_decode(q, out, pages, positions, block_table, num_heads, num_kv_heads, head_dim, scale, max_keys, workspace, settled, entry_starts,
                          window, keep_first, sink, sink_values, gate, gate_offset, gate_per_head) -> None:
     fn = _function("attention_q4", "vipera_attention_q4_decode", _DECODE_Q4_ARGS)
     _check_struct("attention_q4", "vipera_attention_q4_params_size", _DecodeQ4Params)
@@ -1315,10 +1328,10 @@ def _attention_q4_decode(q, out, pages, *, positions, block_table, num_heads, nu
     if not shares:
         runs = (2 if wide else Q4_BLOCKS_PER_SM) * _sm_count_of(here)
         parts = workspace.get("attention.partials", (runs * 2 * (16 if wide else 8) * (head_dim + 4),), torch.float32)
-    gate_pointer, gate_stride = (None, 0) if gate is None else _gate_pointer(
+    gate_pointer, gate_stride = (0, 0) if gate is None else _gate_pointer(
         gate, gate_offset, q.shape[0], num_heads * (1 if gate_per_head else head_dim), what)
     sinks, = _places(what, torch.float32, here, sink_values)
-    p = _DecodeQ4Params(*_places(what, torch.bfloat16, here, q, out), *_place_pages(what, pages, here),
+    p = _pack_decode_q4(*_places(what, torch.bfloat16, here, q, out), *_place_pages(what, pages, here),
                         *_places(what, int32, here, positions, block_table, entry_starts), sinks, gate_pointer, gate_stride,
                         1 if gate_per_head else 0, width, pages.k_codes.shape[2], 0, pages.k_codes.shape[0], entries,
                         num_heads, num_kv_heads, head_dim, scale, window, keep_first, 1 if sink else 0, shares, int(settled), 0)
@@ -1365,12 +1378,12 @@ def _attention_q4_rows(q, out, pages, *, entry_starts, entry_pos0, positions, bl
     chunk, splits = q4_rows_splits(num_kv_heads * -(-count * (num_heads // num_kv_heads) // rows), max_keys, _sm_count_of(here))
     scratch = workspace.get("attention.partials", (attention_decode_scratch_floats(
         count, num_heads, head_dim, splits + (1 if keep_first else 0)),), torch.float32)
-    gate_pointer, gate_stride = (None, 0) if gate is None else _gate_pointer(
+    gate_pointer, gate_stride = (0, 0) if gate is None else _gate_pointer(
         gate, gate_offset, count, num_heads * (1 if gate_per_head else head_dim), what)
     q_at, out_at = _places(what, dtype, here, q, out)
     starts_at, pos0_at, table_at, positions_at = _places(what, int32, here, entry_starts, entry_pos0, block_table, positions)
     sinks, = _places(what, torch.float32, here, sink_values)
-    p = _RowsQ4Params(q_at, *_place_pages(what, pages, here), starts_at, pos0_at, table_at, None, None, block_table.shape[1],
+    p = _pack_rows_q4(q_at, *_place_pages(what, pages, here), starts_at, pos0_at, table_at, 0, 0, block_table.shape[1],
                       pages.k_codes.shape[2], pages.k_codes.shape[0], entries, count, num_heads, num_kv_heads, scale, window, keep_first,
                       chunk, splits)
     _check(fn(p, out_at, dtype_code(dtype), head_dim, positions_at, 1 if sink else 0, sinks, gate_pointer, gate_stride,
@@ -1426,12 +1439,12 @@ def _attention_q4_portions(q, out, pages, *, entry_starts, entry_pos0, positions
     places, scratch = splits + (1 if keep_first else 0), None
     if places > 1:
         scratch = workspace.get("attention.partials", (attention_decode_scratch_floats(count, num_heads, head_dim, places),), torch.float32)
-    gate_pointer, gate_stride = (None, 0) if gate is None else _gate_pointer(
+    gate_pointer, gate_stride = (0, 0) if gate is None else _gate_pointer(
         gate, gate_offset, count, num_heads * (1 if gate_per_head else head_dim), what)
     sinks, = _places(what, torch.float32, here, sink_values)
     starts_at, pos0_at, table_at, positions_at = _places(what, int32, here, entry_starts, entry_pos0, block_table, positions)
-    p = _PortionsQ4Params(*_places(what, torch.bfloat16, here, q, out), *_place_pages(what, pages, here), starts_at, pos0_at, table_at, sinks,
-                          gate_pointer, gate_stride, None, None, kernel_status_word(q.device).data_ptr(), 1 if gate_per_head else 0,
+    p = _pack_portions_q4(*_places(what, torch.bfloat16, here, q, out), *_place_pages(what, pages, here), starts_at, pos0_at, table_at, sinks,
+                          gate_pointer, gate_stride, 0, 0, kernel_status_word(q.device).data_ptr(), 1 if gate_per_head else 0,
                           1 if sink else 0, block_table.shape[1], pages.k_codes.shape[2], pages.k_codes.shape[0], entries, count, num_heads,
                           num_kv_heads, head_dim, scale, window, keep_first, chunk, splits, 1 if skip_single else 0, rows)
     _check(fn(p, positions_at, None if scratch is None else scratch.data_ptr(), 0 if scratch is None else scratch.numel(), _stream_of(here)),
@@ -1459,8 +1472,8 @@ def attention_q4(q: torch.Tensor, out: torch.Tensor, pages: Q4Pages, *, entry_st
     such pages attend."""
     page_size = _check_q4_pages("attention_q4", pages, num_kv_heads, head_dim)
     count, entries = q.shape[0], entry_pos0.numel()
-    if num_kv_heads <= 0 or num_heads % num_kv_heads or tuple(q.shape) != (count, num_heads * head_dim) or out.shape != q.shape \
-            or out.dtype != q.dtype:
+    if num_kv_heads <= 0 or num_heads % num_kv_heads or q.shape != (count, num_heads * head_dim) or out.shape != q.shape \
+            or out.dtype is not q.dtype:
         raise InvalidArgumentError("attention_q4: q and out must be [tokens, heads * d] of one dtype, heads a multiple of KV heads")
     if entry_starts.numel() != entries + 1 or block_table.dim() != 2 or block_table.shape[0] != entries \
             or positions.numel() < count or token_entry.numel() < count or (all_single and entries != count):
@@ -1470,20 +1483,20 @@ def attention_q4(q: torch.Tensor, out: torch.Tensor, pages: Q4Pages, *, entry_st
     if not 0 < max_keys <= block_table.shape[1] * page_size:
         raise InvalidArgumentError("attention_q4: the block tables reach as far as max_keys says")
     window = int(window or 0)
-    if window < 0 or keep_first < 0:
+    if not (0 <= window <= 0x7fffffff and 0 <= keep_first <= 0x7fffffff):
         raise InvalidArgumentError("attention_q4: a window and its kept first keys are counts")
     if count == 0:
         return
     dtype_code(q.dtype)
     keep_first = int(keep_first) if window else 0
+    packed = attention_q4_takes_decode(q.dtype, head_dim, page_size)
+    if packed and all_single:       # (the shortest launches: nothing is made for them that they do not need)
+        _attention_q4_decode(q, out, pages, positions, block_table, num_heads, num_kv_heads, head_dim, scale, max_keys, workspace, settled, None,
+                             window, keep_first, sink, sink_values, gate, gate_offset, gate_per_head)
+        return
     heads = dict(num_heads=num_heads, num_kv_heads=num_kv_heads, head_dim=head_dim, scale=scale, window=window)
     endings = dict(keep_first=keep_first, sink=sink, sink_values=sink_values, gate=gate, gate_offset=gate_offset,
                    gate_per_head=gate_per_head)
-    packed = attention_q4_takes_decode(q.dtype, head_dim, page_size)
-    if packed and all_single:
-        _attention_q4_decode(q, out, pages, positions=positions, block_table=block_table, max_keys=max_keys, workspace=workspace, settled=settled,
-                             entry_starts=None, **heads, **endings)
-        return
     if attention_q4_takes_rows(q.dtype, head_dim, page_size, count * num_heads, max_keys, 1 if any_single else entries):
         _attention_q4_rows(q, out, pages, entry_starts=entry_starts, entry_pos0=entry_pos0, positions=positions, block_table=block_table,
                            max_keys=max_keys, workspace=workspace, **heads, **endings)
