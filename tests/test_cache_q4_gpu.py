@@ -696,3 +696,22 @@ def test_mixed_steps_behind_their_writes_in_a_graph(ops, monkeypatch):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(outs, expected)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rows_behind_the_last_request_stay_as_they_are(ops, form, dtype):
+    """A padded step: more rows of q and out than the requests bring."""
+    heads, d = 4, 64
+    step = Step([30, 2], [200, 0], 16)
+    pages = ops.Q4Pages(*plain.make_pages(step.num_pages, 16, 2, d, 3, DEVICE))
+    q = torch.randn(40, heads * d, device=DEVICE).to(dtype)
+    out = torch.full_like(q, 7.0)
+    described = step.device()
+    for name in ("positions", "token_entry"):
+        described[name] = torch.cat([described[name], torch.zeros(8, dtype=torch.int32, device=DEVICE)])
+    run = lambda q, out: ops.attention_q4(q, out, pages, num_heads=heads, num_kv_heads=2, head_dim=d, scale=0.125, workspace=_workspace(), **described)
+    run(q, out)
+    alone = torch.zeros_like(q[:32])
+    run(q[:32].contiguous(), alone)
+    assert torch.equal(out[:32], alone)
+    assert (out[32:] == 7.0).all()

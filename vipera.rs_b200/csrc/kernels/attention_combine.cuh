@@ -1,5 +1,5 @@
-// The second kernel of split-key attention: partial results of an entry's splits become its output rows.  Shared by
-// the kernels over pages of bfloat16 (attention_mma.cu) and over pages of 4 bits (attention_q4.cu).
+// The second kernel of split-key attention: partial results of an entry's splits become its output rows.  For
+// the kernels over pages of bfloat16 (attention_mma.cu); those over pages of 4 bits take the keys a query sees from here.
 //
 // partial layout: [entry][head][place]: max (log2 units), sum, and D unnormalised outputs.
 #pragma once

@@ -28,7 +28,7 @@
 // less than their share when taken out.  More blocks an SM (four of 128 registers), more or fewer stages and rows read
 // straight into registers change nothing; 8-bit operands (e4m3, where a nibble is a number as it stands) cost conversions on this
 // device, 443 instructions; shifts as high halves of products are 9 % slower; codes less their offset before the products 411.
-#include "attention_combine.cuh"
+#include "attention_q4_join.cuh"
 #include "attention_mma.cuh"
 #include "q4.cuh"
 
@@ -154,7 +154,7 @@ __device__ __forceinline__ void merge_warps(const float* merge, int row, int par
     total += merge[(w * ROWS + row) * kRow + D + 1] * m[w];
   }
   if (part == 0) {
-    ml[0] = best == -INFINITY && total != total ? 0.0f : best;   // the combine kernel passes over -inf
+    ml[0] = best == -INFINITY && total != total ? 0.0f : best;   // the joining kernel passes over -inf
     ml[1] = total;
   }
 #pragma unroll
@@ -930,7 +930,7 @@ VIPERA_API int vipera_attention_q4_decode(const DecodeParams* given, float* part
 VIPERA_API int vipera_attention_q4_rows_params_size() { return static_cast<int>(sizeof(RowsParams)); }
 
 // Attention of every token of a step, q of `dtype` and out too: partials per (token, head, place) in `scratch`, then the endings that
-// the combine kernel knows (`positions` [tokens]; sink, sink_values and gate as for the kernel of single tokens).
+// the joining kernel knows (`positions` [tokens]; sink, sink_values and gate as for the kernel of single tokens).
 VIPERA_API int vipera_attention_q4_rows(const RowsParams* given, void* out, int dtype, int head_dim, const int* positions, int sink,
                                         const float* sink_values, const float* gate, long long gate_stride, int gate_per_head,
                                         float* scratch, size_t scratch_floats, void* stream) {
@@ -955,9 +955,8 @@ VIPERA_API int vipera_attention_q4_rows(const RowsParams* given, void* out, int 
   if (wide) status = head_dim == 128 ? launch_rows<128, float, 1>(p, s) : launch_rows<64, float, 2>(p, s);
   else if (dtype == VIPERA_BF16) status = head_dim == 128 ? launch_rows<128, __nv_bfloat16, 2>(p, s) : launch_rows<64, __nv_bfloat16, 2>(p, s);
   if (status != VIPERA_OK) return status;
-  const auto combine = head_dim == 128 ? (wide ? attention_combine_kernel<128, true, true> : attention_combine_kernel<128, true, false>)
-                                       : (wide ? attention_combine_kernel<64, true, true> : attention_combine_kernel<64, true, false>);
-  return vipera_launch(combine, dim3(p.num_tokens, p.num_heads), head_dim, 0, s, p.partial_ml, p.partial_out, p.num_splits,
-                       static_cast<__nv_bfloat16*>(out), p.num_heads, positions, p.window, p.chunk, static_cast<const int*>(nullptr),
-                       p.keep_first, sink, sink_values, gate, gate_stride, gate_per_head);
+  const JoinParams join{p.partial_ml, p.partial_out, out, positions, p.entry_starts + p.num_entries, sink_values, gate, gate_stride, gate_per_head,
+                        sink, p.num_tokens, p.num_heads, p.window, p.keep_first, p.chunk, p.num_splits};
+  if (wide) return head_dim == 128 ? launch_join<128, float>(join, s) : launch_join<64, float>(join, s);
+  return head_dim == 128 ? launch_join<128, __nv_bfloat16>(join, s) : launch_join<64, __nv_bfloat16>(join, s);
 }

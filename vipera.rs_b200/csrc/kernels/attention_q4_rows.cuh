@@ -8,7 +8,7 @@
 //
 // What bounds it: issuing, and for short steps the latency of one walk.  Rows times keys go by at 1.7e5 a microsecond with heads of
 // 128 in bfloat16, so that the tensor cores' kernel (attention_q4_tc.cu) wins beyond a size (ops.attention_q4_takes_rows has the rule and
-// both sides' times).  384 rows of 32 bits over 96 to 2,113 keys: 15 us and 6 for the parts' ending, from a cold cache.
+// both sides' times).  384 rows of 32 bits over 96 to 2,113 keys: 22 us with the joining launch, from a cold cache.
 #pragma once
 
 namespace {
@@ -92,7 +92,7 @@ __global__ void __launch_bounds__(32 * kWarps) attention_q4_rows_kernel(RowsPara
   const int places = p.num_splits + (p.keep_first > 0 ? 1 : 0);
   const int begin = kept_split ? 0 : max(split * p.chunk, first_low / 32 * 32);
   const int end = kept_split ? min(p.keep_first, first_high) : min((split + 1) * p.chunk, last_high + 1);
-  if (begin >= end && !kept_split) return;    // no row's keys are here: the combine kernel does not look (it does for kept keys)
+  if (begin >= end && !kept_split) return;    // no row's keys are here: the joining kernel does not look (it does for kept keys)
 
   for (int i = threadIdx.x; i < NT * G * 32; i += blockDim.x) {     // (row tile, group, lane): eight channels
     const int l = i & 31, gr = i / 32 % G, nt = i / 32 / G, r = row0 + nt * 8 + (l >> 2);

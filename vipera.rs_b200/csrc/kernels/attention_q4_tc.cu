@@ -33,7 +33,7 @@
 // at once, weights and products one behind the other, took 6,000 clocks, with the products of both tiles from one warp in turn 4,700; rows asked for
 // a whole tile ahead 4 % longer (registers), eight unpacking warps 7 % longer there and 10 % shorter where blocks have one tile.  A lone
 // block's 128 keys of 128 rows take 2 us: the unpacking warps' loads and work.
-#include "attention_combine.cuh"
+#include "attention_q4_join.cuh"
 #include "q4.cuh"
 #include "tcgen05.cuh"
 
@@ -671,59 +671,6 @@ __global__ void __launch_bounds__(kThreads, 1) attention_q4_portions_kernel(cons
   }
 }
 
-// A warp a (token, head) row: the parts of the splits that hold keys of it become its output.  The parts of 28,672 rows of 128 in two
-// splits (29 MB) take 12 us, where a block of 128 threads a row takes 60.
-template <int D>
-__global__ void __launch_bounds__(256) attention_q4_portions_join_kernel(const PortionParams p, const int* __restrict__ positions) {
-  constexpr int kOwn = D / 32;
-  pdl_launch_dependents();
-  const long long row = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (row >= static_cast<long long>(p.num_tokens) * p.num_heads) return;
-  const int token = static_cast<int>(row / p.num_heads), head = static_cast<int>(row - static_cast<long long>(token) * p.num_heads);
-  const int position = positions[token], visible = first_visible_key(position, p.window);
-  const int places = p.num_splits + (p.keep_first > 0 ? 1 : 0);
-  const int first = visible / p.chunk, window_last = min(p.num_splits - 1, position / p.chunk);
-  const int count = window_last - first + 1 + (min(p.keep_first, visible) > 0 ? 1 : 0);      // the kept keys' place comes last
-  const auto place_of = [&](int i) { return row * places + (first + i > window_last ? p.num_splits : first + i); };
-  pdl_wait();
-  const float2* ml = reinterpret_cast<const float2*>(p.partial_ml);
-  float best = -INFINITY;
-  for (int i = lane; i < count; i += 32) best = fmaxf(best, ml[place_of(i)].x);
-  best = warp_max(best);
-  float total = 0.0f, x[kOwn];
-#pragma unroll
-  for (int c = 0; c < kOwn; ++c) x[c] = 0.0f;
-#pragma unroll 4
-  for (int i = 0; i < count; ++i) {
-    const long long at = place_of(i);
-    const float2 part = ml[at];
-    const float w = part.x == -INFINITY ? 0.0f : exp2f(part.x - best);
-    const float* from = p.partial_out + at * D + lane * kOwn;
-    total += part.y * w;
-    if constexpr (kOwn == 4) {
-      const float4 v = *reinterpret_cast<const float4*>(from);
-      x[0] += v.x * w, x[1] += v.y * w, x[2] += v.z * w, x[3] += v.w * w;
-    } else {
-      const float2 v = *reinterpret_cast<const float2*>(from);
-      x[0] += v.x * w, x[1] += v.y * w;
-    }
-  }
-  if (p.sink) total += exp2f((p.sink_values ? p.sink_values[head] * kLog2e : 0.0f) - best);
-  const float* gate = p.gate ? p.gate + static_cast<size_t>(token) * p.gate_stride + (p.gate_per_head ? head : head * D + lane * kOwn) : nullptr;
-  uint32_t packed[kOwn / 2];
-#pragma unroll
-  for (int c = 0; c < kOwn; ++c) {
-    x[c] /= total;
-    if (gate) x[c] *= 1.0f / (1.0f + __expf(-gate[p.gate_per_head ? 0 : c]));
-  }
-#pragma unroll
-  for (int c = 0; c < kOwn; c += 2) packed[c / 2] = bits_of(__floats2bfloat162_rn(x[c], x[c + 1]));
-  uint32_t* to = reinterpret_cast<uint32_t*>(p.out + row * D + lane * kOwn);
-  if constexpr (kOwn == 4) *reinterpret_cast<uint2*>(to) = make_uint2(packed[0], packed[1]);
-  else to[0] = packed[0];
-}
-
 template <int D>
 int launch(const PortionParams& p, cudaStream_t s) {
   // heads of 64 ask for as much as those of 128: a block holds all of its SM's tensor memory, so nothing else that wants some should join it
@@ -772,8 +719,7 @@ VIPERA_API int vipera_attention_q4_portions(const PortionParams* given, const in
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int status = p.head_dim == 128 ? launch<128>(p, s) : launch<64>(p, s);
   if (status != VIPERA_OK || places == 1) return status;
-  const long long blocks = (static_cast<long long>(p.num_tokens) * p.num_heads + 7) / 8;
-  if (blocks > 0x7fffffffLL) return VIPERA_BAD_SHAPE;
-  return vipera_launch(p.head_dim == 128 ? attention_q4_portions_join_kernel<128> : attention_q4_portions_join_kernel<64>,
-                       dim3(static_cast<unsigned>(blocks)), 256, 0, s, p, positions);
+  const JoinParams join{p.partial_ml, p.partial_out, p.out, positions, p.entry_starts + p.num_entries, p.sink_values, p.gate, p.gate_stride,
+                        p.gate_per_head, p.sink, p.num_tokens, p.num_heads, p.window, p.keep_first, p.chunk, p.num_splits};
+  return p.head_dim == 128 ? launch_join<128, __nv_bfloat16>(join, s) : launch_join<64, __nv_bfloat16>(join, s);
 }
