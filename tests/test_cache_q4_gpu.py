@@ -715,3 +715,19 @@ def test_rows_behind_the_last_request_stay_as_they_are(ops, form, dtype):
     run(q[:32].contiguous(), alone)
     assert torch.equal(out[:32], alone)
     assert (out[32:] == 7.0).all()
+
+
+def test_a_key_that_is_not_finite_and_alone_in_its_cut(ops, form):
+    """A window whose first key is the last one of a cut of the keys: its row is NaN, and no other."""
+    heads, d, key = 2, 64, 127
+    step = Step([40], [110], 16)
+    raw = plain.make_pages(step.num_pages, 16, 1, d, 3, DEVICE)
+    pages = ops.Q4Pages(*raw)
+    q = torch.randn(40, heads * d, device=DEVICE).to(torch.bfloat16)
+    without = _portions(step, pages, q, ops, heads, 1, d, window=10)
+    raw[1][step.tables[0][key // 16], 0, key % 16, 0] = float("nan")
+    with_one = _portions(step, pages, q, ops, heads, 1, d, window=10)
+    sees = [key <= 110 + i < key + 10 for i in range(40)]
+    assert sees[26] and not sees[27]
+    assert with_one[sees].isnan().all()
+    assert torch.equal(with_one[[not s for s in sees]], without[[not s for s in sees]])

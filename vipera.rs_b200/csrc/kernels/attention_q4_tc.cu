@@ -29,10 +29,11 @@
 // What bounds it.  2,048 tokens of 28 heads of 128 on 4: 49 us, 57 from a cold cache, 617 and 525 TFLOP/s (of 1,661 measured; expanding and the
 // flash kernel take 69 and 73).  A block takes 5 us to its first scores and 2.5 to its ending, and 4,200 clocks for 128 keys of its 256
 // rows: the exponentials alone are 2,048 (16 a clock), the tensor cores are busy for 2,700 (products of 64 columns cost as much as of 128),
-// and both chains' softmax warps and the unpacking ones share the issue slots, of which they take 2,700.  Without the rows' loads 51 us, without the exponentials 55, without both 47.  Scores of 128 keys
-// at once, weights and products one behind the other, took 6,000 clocks, with the products of both tiles from one warp in turn 4,700; rows asked for
-// a whole tile ahead 4 % longer (registers), eight unpacking warps 7 % longer there and 10 % shorter where blocks have one tile.  A lone
-// block's 128 keys of 128 rows take 2 us: the unpacking warps' loads and work.
+// and both chains' softmax warps and the unpacking ones share the issue slots, of which they take 2,700.  Without the rows' loads 51 us (of
+// 55, an earlier form), without the exponentials 55, without both 47.  Scores of 128 keys at once, weights and products one behind the
+// other, took 6,000 clocks, with the products of both tiles from one warp in turn 4,700; rows asked for a whole tile ahead 4 % longer
+// (registers), eight unpacking warps 7 % longer there and 10 % shorter where blocks have one tile.  A lone block's 128 keys of 128 rows
+// take 2 us: the unpacking warps' loads and work.
 #include "attention_q4_join.cuh"
 #include "q4.cuh"
 #include "tcgen05.cuh"
@@ -471,7 +472,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_q4_portions_kernel(cons
         factor *= inverse;
         other_factor *= inverse;
       } else if (r < job.rows && tile == chain && !*abort_flag) {
-        *reinterpret_cast<float2*>(p.partial_ml + 2 * place) = make_float2(row_max, row_sum);
+        // (the joining kernel passes over -inf, which stands for no visible key and not for keys whose scores are all NaN)
+        *reinterpret_cast<float2*>(p.partial_ml + 2 * place) = make_float2(row_max == -INFINITY && row_sum != row_sum ? 0.0f : row_max, row_sum);
       }
       const float* gate = p.gate && !p.gate_per_head ? p.gate + static_cast<size_t>(token) * p.gate_stride + static_cast<size_t>(head) * D : nullptr;
       const uint32_t other_at = lanes + 256 + (chain ^ 1) * 128;
@@ -586,7 +588,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_q4_portions_kernel(cons
         any_large |= large_keys[i] | large_values[i];
       }
       if (j >= 2) wait(&sh->k_empty[stage], before, abort_flag, p.status);
-      // the notes of tile j - 4 have been read: its softmax came before the scores of tile j - 3, and their keys are gone
+      // the notes of tile j - 4 have been read: its softmax came before the scores of tile j - 2, and their keys are gone
       const uint32_t bad = __ballot_sync(0xffffffffu, any_bad);
       if (bad) {
 #pragma unroll
