@@ -1,0 +1,19 @@
+"""A cache in 4 bits at its edges, without a device: what launchers refuse before a launch, what plans and flags say."""
+import pytest
+
+
+@pytest.mark.parametrize("dtype, d, off", [("float32", 128, 4), ("float32", 128, 8), ("float32", 64, 4), ("bfloat16", 128, 2), ("bfloat16", 128, 4),
+                                           ("bfloat16", 64, 2)])
+def test_rows_are_not_stored_to_places_that_do_not_fit_their_pieces(dtype, d, off):
+    """The launcher of the kernel of any number of rows looks at `out` before it launches anything (every address here is made up)."""
+    import vipera_rs_b200  # noqa: F401
+    from vipera_rs_b200.kernels import ops
+
+    fn = ops._function("attention_q4", "vipera_attention_q4_rows", ops._ROWS_Q4_ARGS)
+    at = 1 << 20
+    block = ops._pack_rows_q4(at, at, at, at, at, at, at, at, 0, 0, 2, 16, 4, 1, 3, 4, 2, 0.125, 0, 0, 64, 1)
+    code = ops.F32 if dtype == "float32" else ops.BF16
+    call = lambda out, scratch: fn(block, out, code, d, at, 0, None, None, 0, 0, scratch, 1 << 20, None)
+    assert call(at + off, at) == -3
+    assert call(at, at + 4) == -3        # as a scratch that does not fit
+    assert fn(block, at, 7, d, at, 0, None, None, 0, 0, at, 1 << 20, None) == -1      # no such type

@@ -940,10 +940,14 @@ VIPERA_API int vipera_attention_q4_rows(const RowsParams* given, void* out, int 
       p.page_size % 16 || p.num_heads > 65535 || p.num_splits <= 0 || p.num_splits > 128 || p.chunk <= 0 || p.chunk % 64 ||
       (head_dim != 64 && head_dim != 128))
     return VIPERA_BAD_SHAPE;
+  if (dtype != VIPERA_F32 && dtype != VIPERA_BF16) return VIPERA_BAD_DTYPE;
   if (p.window <= 0) p.keep_first = 0;
   if (sink_values) sink = 1;
   const size_t rows = static_cast<size_t>(p.num_tokens) * p.num_heads * (p.num_splits + (p.keep_first > 0 ? 1 : 0));
   const size_t pairs = (2 * rows + 3) / 4 * 4;
+  // the joining kernel's lanes store a 32nd of a row at once
+  const uintptr_t piece = static_cast<uintptr_t>(head_dim / 32) * (dtype == VIPERA_F32 ? 4 : 2);
+  if (reinterpret_cast<uintptr_t>(out) & (piece - 1)) return VIPERA_BAD_ARGUMENT;
   if (!scratch || scratch_floats < pairs + rows * head_dim || !on_16_bytes(scratch) || !on_16_bytes(p.k_codes) ||
       !on_16_bytes(p.v_codes) || !on_16_bytes(p.k_scales) || !on_16_bytes(p.v_scales))
     return VIPERA_BAD_ARGUMENT;
