@@ -17,3 +17,24 @@ def test_rows_are_not_stored_to_places_that_do_not_fit_their_pieces(dtype, d, of
     assert call(at + off, at) == -3
     assert call(at, at + 4) == -3        # as a scratch that does not fit
     assert fn(block, at, 7, d, at, 0, None, None, 0, 0, at, 1 << 20, None) == -1      # no such type
+
+
+@pytest.mark.parametrize("kernel", ["tensor", "mma"])
+def test_the_flash_kernels_behind_an_expansion_refuse_rows_off_their_pieces(kernel):
+    """Pages that no kernel reads packed are expanded for the flash kernels, which move a row's 16 bytes at once."""
+    import vipera_rs_b200  # noqa: F401
+    from vipera_rs_b200.kernels import ops
+
+    kinds = [ops._c_void] * 7 + [ops._c_int] * 7 + [ops._c_float, ops._c_int]
+    at = 1 << 20
+
+    def call(q, out):
+        places, sizes = (q, out, at, at, at, at, at), (2, 24, 1, 3, 4, 2, 64, 0.125, 0)
+        if kernel == "tensor":
+            fn = ops._function("attention_tc", "vipera_attention_prefill_tc", kinds + [ops._c_int, ops._c_int, ops._c_void, ops._c_void])
+            return fn(*places, *sizes, 4, 0, at, None)
+        return ops._function("attention_mma", "vipera_attention_prefill", kinds + [ops._c_int, ops._c_void])(*places, *sizes, 0, None)
+
+    assert call(at + 2, at) == -3 and call(at + 8, at) == -3 and call(at, at + 2) == -3
+    if kernel == "tensor":
+        assert call(at, at + 8) == -3

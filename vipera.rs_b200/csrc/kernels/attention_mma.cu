@@ -811,6 +811,10 @@ static int run_prefill(const void* q, void* out, const void* k_pool, const void*
                        int skip_single, int keep_first, int sink, void* stream) {
   if (num_tokens <= 0 || num_entries <= 0) return VIPERA_OK;
   if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads || keep_first < 0) return VIPERA_BAD_SHAPE;
+  // rows come in pieces of 16 bytes and leave in pairs of values
+  if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_pool) | reinterpret_cast<uintptr_t>(v_pool)) & 15) ||
+      (reinterpret_cast<uintptr_t>(out) & 3))
+    return VIPERA_BAD_ARGUMENT;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (head_dim == 128)
     return launch_prefill<128>(q, out, k_pool, v_pool, entry_starts, entry_pos0, block_table, table_width, page_size,

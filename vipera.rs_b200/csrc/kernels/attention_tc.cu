@@ -916,7 +916,10 @@ VIPERA_API int vipera_attention_prefill_tc_gated(const void* q, void* out, const
   if (gate && !gate_per_head && ((reinterpret_cast<uintptr_t>(gate) & 15) || (gate_stride & 3))) return VIPERA_BAD_ARGUMENT;
   if ((head_dim != 64 && head_dim != 128) || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads || page_size <= 0 || num_pages <= 0)
     return VIPERA_BAD_SHAPE;
-  if (!status) return VIPERA_BAD_ARGUMENT;
+  // rows go in and out in pieces of 16 bytes
+  if (!status || ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(k_pool) |
+                   reinterpret_cast<uintptr_t>(v_pool)) & 15))
+    return VIPERA_BAD_ARGUMENT;
   Params p{};
   p.q = static_cast<const __nv_bfloat16*>(q);
   p.out = static_cast<__nv_bfloat16*>(out);
