@@ -38,3 +38,15 @@ def test_the_flash_kernels_behind_an_expansion_refuse_rows_off_their_pieces(kern
     assert call(at + 2, at) == -3 and call(at + 8, at) == -3 and call(at, at + 2) == -3
     if kernel == "tensor":
         assert call(at, at + 8) == -3
+
+
+def test_single_tokens_beside_portions_are_refused_without_their_word():
+    """A launch that may begin while the portions run needs the word that says what is complete."""
+    import vipera_rs_b200  # noqa: F401
+    from vipera_rs_b200.kernels import ops
+
+    fn = ops._function("attention_q4", "vipera_attention_q4_decode", ops._DECODE_Q4_ARGS)
+    at = 1 << 20
+    for settled, beside in ((2, 0), (3, at), (-1, at)):
+        block = ops._pack_decode_q4(at, at, at, at, at, at, at, at, at, 0, 0, 0, 0, 2, 16, 0, 4, 1, 4, 2, 64, 0.125, 0, 0, 0, 1, settled, beside, 0)
+        assert fn(block, None, 0, 0, None) == -3

@@ -36,3 +36,72 @@ def test_an_output_off_its_pieces_is_refused_by_steps_of_rows(ops, dtype, d):
         assert ops.launches == before
         # queries may begin anywhere: they are read value by value
         assert torch.equal(_attend(ops, step, pages, _off(q), 2, 1, d), _attend(ops, step, pages, q, 2, 1, d))
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_layers_that_share_their_buffers_beside_portions(ops, deal, monkeypatch, captured):
+    """Write, portions, single tokens, layer after layer as an engine runs them: queries, outputs and workspace are the same buffers in every
+    layer, pages are the layer's own.  Each layer's outputs are those of the same launches with a pause behind each."""
+    monkeypatch.setattr(ops, "Q4_ROWS_WORK", 0)
+    monkeypatch.setattr(ops, "q4_portion_plan", lambda *a: (128, 1 << 20, 1))
+    heads, kv_heads, d, layers = 8, 2, 128, 12
+    step = Step([1, 300, 1, 40, 1, 1], [900, 100, 700, 30, 1500, 3], 16)
+    tokens = sum(step.counts)
+    described, slots, room = step.device(), _int(step.slots), _workspace()
+    qkv = torch.randn(layers, tokens, (heads + 2 * kv_heads) * d, device=DEVICE)
+    start = [plain.make_pages(step.num_pages, 16, kv_heads, d, 3 + i, DEVICE) for i in range(layers)]
+    q, out, kept = (torch.zeros(*n, tokens, heads * d, dtype=torch.bfloat16, device=DEVICE) for n in ((), (), (layers,)))
+
+    def run(pages, pause):
+        for i in range(layers):
+            ops.rope_cache_q4(qkv[i], q, pages[i], num_heads=heads, num_kv_heads=kv_heads, head_dim=d, positions=described["positions"],
+                              cos=None, sin=None, style=ops.ROPE_NONE, slots=slots)
+            pause()
+            ops.attention_q4(q, out, pages[i], num_heads=heads, num_kv_heads=kv_heads, head_dim=d, scale=0.09, workspace=room, settled=True,
+                             **described)
+            pause()
+            kept[i].copy_(out)
+            pause()
+
+    fresh = lambda: [ops.Q4Pages(*[t.clone() for t in layer]) for layer in start]
+    run(fresh(), torch.cuda.synchronize)
+    expected = kept.clone()
+    pages = fresh()
+    torch.cuda.synchronize()
+    if captured:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            run(pages, lambda: None)
+        again = graph.replay
+    else:
+        again = lambda: run(pages, lambda: None)
+    for _ in range(5):
+        kept.zero_()
+        again()
+        torch.cuda.synchronize()
+        assert torch.equal(kept, expected)
+    assert int(room.get("attention.q4_beside", (1,), torch.int32)) == 0        # taken back
+
+
+@pytest.mark.parametrize("singles", [0, 1, 3])
+@pytest.mark.parametrize("portions", [0, 2])
+def test_steps_of_portions_alone_and_of_single_tokens_alone_said_to_hold_both(ops, deal, monkeypatch, singles, portions):
+    """Either kernel may find nothing to do: the other's rows are right, and the word between them is taken back."""
+    if not singles + portions:
+        return
+    monkeypatch.setattr(ops, "Q4_ROWS_WORK", 0)
+    monkeypatch.setattr(ops, "q4_portion_plan", lambda *a: (256, 1 << 20, 1))
+    step = Step([1] * singles + [70, 150][:portions], [500, 2, 90][:singles] + [0, 900][:portions], 16)
+    pages = ops.Q4Pages(*plain.make_pages(step.num_pages, 16, 2, 128, 3, DEVICE))
+    q = torch.randn(sum(step.counts), 8 * 128, device=DEVICE).to(torch.bfloat16)
+    room = _workspace()
+    both = _attend(ops, step, pages, q, 8, 2, 128, workspace=room, all_single=False, any_single=True)
+    assert int(room.get("attention.q4_beside", (1,), torch.int32)) == 0
+    if portions:
+        apart = _attend(ops, step, pages, q, 8, 2, 128, any_single=False)          # every row the portions' kernel's
+        assert torch.equal(both[singles:], apart[singles:])
+    if singles:
+        alone = Step([1] * singles, [500, 2, 90][:singles], 16)
+        alone.tables = step.tables[:singles]
+        expected = _attend(ops, alone, pages, q[:singles].contiguous(), 8, 2, 128)
+        assert torch.equal(both[:singles], expected)

@@ -52,9 +52,11 @@ struct DecodeParams {
   float scale;
   int window, keep_first, sink, shares;
   // 1: positions, tables and earlier steps' rows are complete before the kernel ahead of this one begins.  2: that kernel, of the same step's
-  // portions, lets this one begin once all that went before itself is complete, and shares nothing with it: this one waits for it at its end
-  // (portions of 512, 200 and 37 tokens beside 16 single ones behind 2,048: 57 us for 74).
+  // portions, lets this one begin once all that went before itself is complete, which `beside` says (attention_q4_join.cuh), and shares nothing
+  // with it: this one waits for it at its end (portions of 512, 200 and 37 tokens beside 16 single ones behind 2,048: 57 us for 74).
+  // What is read in front of a wait, and what another kernel has written behind it, is read from L2.
   int settled;
+  int* beside;
   uint32_t magic;                 // set by the launcher
 };
 
@@ -240,7 +242,7 @@ __device__ __forceinline__ void walk(const DecodeParams& p, const Shared<D, NT> 
     const int tile = warp_tile + (index >> 1) * 8 + (index & 1);
     if (tile >= tiles_end) return -1;
     const int key = seen.key_of(tile), place = p.page_shift >= 0 ? key >> p.page_shift : key / p.page_size;
-    const int page = place < p.table_width ? table[place] : -1;
+    const int page = place < p.table_width ? __ldcg(table + place) : -1;
     return page < p.num_pages ? page : -1;
   };
   int pages_now = page_of(lane), pages_next = steps > 16 ? page_of(32 + lane) : -1;
@@ -330,8 +332,11 @@ __device__ __forceinline__ void walk(const DecodeParams& p, const Shared<D, NT> 
 #pragma unroll
     for (int gr = 0; gr < G; ++gr) {
       q[gr][0] = q[gr][1] = q[gr][2] = q[gr][3] = 0;
-      if (h < group)
-        load_words<4>(q[gr], p.q + (static_cast<size_t>(token) * p.num_heads + kv_head * group + h) * D + 32 * gr + 8 * t);
+      if (h < group) {
+        const uint4 v = __ldcg(reinterpret_cast<const uint4*>(
+            p.q + (static_cast<size_t>(token) * p.num_heads + kv_head * group + h) * D + 32 * gr + 8 * t));
+        q[gr][0] = v.x, q[gr][1] = v.y, q[gr][2] = v.z, q[gr][3] = v.w;
+      }
     }
 #pragma unroll
     for (int gr = 0; gr < G; ++gr)
@@ -588,7 +593,7 @@ __device__ __forceinline__ void finish(const DecodeParams& p, int token, int hea
   if (p.gate) {
     const float* gate = p.gate + static_cast<size_t>(token) * p.gate_stride + (p.gate_per_head ? head : head * D + column);
 #pragma unroll
-    for (int c = 0; c < 4; ++c) out[c] *= 1.0f / (1.0f + expf(-gate[p.gate_per_head ? 0 : c]));
+    for (int c = 0; c < 4; ++c) out[c] *= 1.0f / (1.0f + expf(-__ldcg(gate + (p.gate_per_head ? 0 : c))));
   }
   store_four_as<__nv_bfloat16>(p.out + (static_cast<size_t>(token) * p.num_heads + head) * D + column, out[0], out[1], out[2], out[3]);
 }
@@ -607,6 +612,18 @@ struct Join {
   }
 };
 
+// The start and the end of a block beside the step's portions (DecodeParams::settled == 2).
+__device__ __forceinline__ void begin_beside(const DecodeParams& p) {
+  __shared__ int word;
+  if (threadIdx.x == 0) word = acquire_word(p.beside);
+  __syncthreads();
+  if (word != 1) pdl_wait();
+}
+__device__ __forceinline__ void end_beside(const DecodeParams& p, bool first_block) {
+  pdl_wait();
+  if (first_block && threadIdx.x == 0) release_word(p.beside, 0);
+}
+
 // Few (entry, KV head) pairs: the blocks of a cluster share the keys of one, each a part as large, and join their parts.
 // One entry of 2,048 keys, 12 heads of 128 on 2, sixteen blocks a pair: 7.8 us, the latency of a start (2), one walk and two cluster barriers.
 template <int D, int NT>
@@ -618,18 +635,21 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) attention_q4_clu
     pdl_wait();
     pdl_launch_dependents();
   }
+  if (p.settled == 2) begin_beside(p);
+  const bool first_block = (blockIdx.x | blockIdx.y | blockIdx.z) == 0;
   const int group = p.num_heads / p.num_kv_heads, head_tiles = (group + 8 * NT - 1) / (8 * NT);
   const int entry = blockIdx.x, share = blockIdx.z;
   const int kv_head = blockIdx.y / head_tiles, head0 = (blockIdx.y - kv_head * head_tiles) * 8 * NT;
   int token = entry;
   if (p.entry_starts) {
-    token = p.entry_starts[entry];
-    if (p.entry_starts[entry + 1] - token != 1) {   // the whole cluster's; a grid without an entry must not end before the kernels ahead
-      if (p.settled && entry == 0) pdl_wait();
+    token = __ldcg(p.entry_starts + entry);
+    if (__ldcg(p.entry_starts + entry + 1) - token != 1) {   // the whole cluster's; a grid without an entry must not end before the kernels ahead
+      if (p.settled == 2 && first_block) end_beside(p, true);
+      else if (p.settled && entry == 0) pdl_wait();
       return;
     }
   }
-  const Visible seen(p, p.positions[entry]);
+  const Visible seen(p, __ldcg(p.positions + entry));
   const int each = (seen.tiles + 8 * p.shares - 1) / (8 * p.shares) * 8;      // of a block: whole steps of its warps
   walk<D, NT>(p, shared, seen, entry, token, kv_head, head0, min(share * each, seen.tiles), min((share + 1) * each, seen.tiles), p.settled != 1);
   cluster_sync_all();
@@ -647,7 +667,7 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) attention_q4_clu
   }
   cluster_sync_all();   // nobody's shared memory goes while others read it
   if (p.settled == 2) {
-    pdl_wait();
+    end_beside(p, first_block);
     pdl_launch_dependents();
   }
 }
@@ -664,8 +684,8 @@ __device__ __forceinline__ int units_for(const DecodeParams& p, int position) {
   return tiles > 0 ? ((tiles + 7) >> 3) + kBegin : 0;
 }
 __device__ __forceinline__ int units_of(const DecodeParams& p, int entry) {
-  if (entry >= p.num_entries || (p.entry_starts && p.entry_starts[entry + 1] - p.entry_starts[entry] != 1)) return 0;
-  return units_for(p, p.positions[entry]);
+  if (entry >= p.num_entries || (p.entry_starts && __ldcg(p.entry_starts + entry + 1) - __ldcg(p.entry_starts + entry) != 1)) return 0;
+  return units_for(p, __ldcg(p.positions + entry));
 }
 constexpr int kRunEntries = 1024;   // entries whose lengths a block holds
 
@@ -679,6 +699,8 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) attention_q4_run
   if (p.settled != 2) {
     pdl_wait();
     pdl_launch_dependents();
+  } else {
+    begin_beside(p);
   }
   const bool last = p.settled == 2 && blockIdx.x == 0;      // a grid that found nothing to do must not end before the kernels ahead
   const int group = p.num_heads / p.num_kv_heads, head_tiles = (group + 8 * NT - 1) / (8 * NT), pairs = p.num_kv_heads * head_tiles;
@@ -687,7 +709,8 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) attention_q4_run
   for (int e0 = 0; e0 < p.num_entries; e0 += 32 * kWarps) {
     const int e = e0 + threadIdx.x;
     int position = -1;
-    if (e < p.num_entries && !(p.entry_starts && p.entry_starts[e + 1] - p.entry_starts[e] != 1)) position = p.positions[e];
+    if (e < p.num_entries && !(p.entry_starts && __ldcg(p.entry_starts + e + 1) - __ldcg(p.entry_starts + e) != 1))
+      position = __ldcg(p.positions + e);
     int upto = position >= 0 ? units_for(p, position) : 0;
 #pragma unroll
     for (int offset = 1; offset < 32; offset <<= 1) {
@@ -712,7 +735,7 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) attention_q4_run
   const long long all = static_cast<long long>(whole) * pairs;
   const long long runs = min(static_cast<long long>(gridDim.x), all);     // each with a unit at least
   if (blockIdx.x >= runs) {
-    if (last) pdl_wait();
+    if (last) end_beside(p, true);
     return;
   }
   long long at = all * blockIdx.x / runs;
@@ -726,13 +749,13 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) attention_q4_run
   const auto units_at = [&](int e) { return ends[e] - (e > 0 ? ends[e - 1] : 0); };
   int units = units_at(entry);
   if (units == 0) {
-    if (last) pdl_wait();
+    if (last) end_beside(p, true);
     return;
   }
   const int into = static_cast<int>(at - static_cast<long long>(ends[entry] - units) * pairs);
   int pair = into / units, unit = into - pair * units;
   while (at < stop && entry < p.num_entries) {
-    const int token = p.entry_starts ? p.entry_starts[entry] : entry;
+    const int token = p.entry_starts ? __ldcg(p.entry_starts + entry) : entry;
     const int kv_head = pair / head_tiles, head0 = (pair - kv_head * head_tiles) * 8 * NT;
     const int run = static_cast<int>(min(static_cast<long long>(units - unit), stop - at));
     // the run's own keys: units kBegin and behind
@@ -766,7 +789,7 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 3 : 2) attention_q4_run
     }
   }
   if (p.settled == 2) {
-    pdl_wait();
+    end_beside(p, blockIdx.x == 0);
     pdl_launch_dependents();
   }
 }
@@ -913,6 +936,7 @@ VIPERA_API int vipera_attention_q4_decode(const DecodeParams* given, float* part
   if (p.shares == 0 && (runs <= 0 || p.num_entries > kRunEntries || !parts || !on_16_bytes(parts) ||
                         parts_floats < vipera_attention_q4_parts(runs, p.num_heads, p.num_kv_heads, p.head_dim)))
     return VIPERA_BAD_ARGUMENT;
+  if (p.settled < 0 || p.settled > 2 || (p.settled == 2 && !p.beside)) return VIPERA_BAD_ARGUMENT;
   if (p.sink_values) p.sink = 1;
   if (!on_16_bytes(p.q) || !on_16_bytes(p.k_codes) || !on_16_bytes(p.v_codes) || !on_16_bytes(p.k_scales) || !on_16_bytes(p.v_scales) ||
       (reinterpret_cast<uintptr_t>(p.out) & 7))

@@ -1,5 +1,6 @@
-// The second kernel of attention over pages of 4 bits whose keys are cut: the parts of a row's cuts become its output.  Shared by the kernel
-// of any number of rows (attention_q4.cu) and the tensor cores' (attention_q4_tc.cu).
+// What the kernels of attention over pages of 4 bits share: the word between portions and single tokens that run beside them, and the second
+// kernel where keys are cut, behind the kernel of any number of rows (attention_q4.cu) and the tensor cores' (attention_q4_tc.cu): the parts of
+// a row's cuts become its output.
 //
 // Parts: [token][head][place]: maximum (in powers of two) and sum, and D outputs not yet divided; a place a cut and, with kept first keys,
 // one more for those.
@@ -8,6 +9,20 @@
 #include "attention_combine.cuh"
 
 namespace {
+
+// A step's portions and its single tokens share nothing but what went before both.  The portions' kernel waits for that and lets the single
+// tokens' one begin, which may not wait in its turn (its wait is for the portions' end).  What makes the writes before both visible to it is
+// therefore this word: 1 is released by the portions' kernel behind its wait and acquired by each block of the single tokens' kernel in front of
+// its first dependent read; a block that does not find it waits for the portions' end instead, which is always right.  The single tokens' kernel
+// takes the word back behind its own wait (a block of its that begins later finds the portions ended), so that 1 is this launch's and no other's.
+__device__ __forceinline__ void release_word(int* word, int value) {
+  asm volatile("st.release.gpu.global.s32 [%0], %1;" ::"l"(word), "r"(value) : "memory");
+}
+__device__ __forceinline__ int acquire_word(const int* word) {
+  int value;
+  asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(value) : "l"(word) : "memory");
+  return value;
+}
 
 struct JoinParams {
   const float* ml;
@@ -30,11 +45,11 @@ __global__ void __launch_bounds__(256) attention_q4_join_rows_kernel(const JoinP
   const long long row = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   const int token = static_cast<int>(min(row / p.num_heads, static_cast<long long>(p.num_tokens))), head = static_cast<int>(row % p.num_heads);
-  if (token >= min(p.num_tokens, *p.covered)) {
+  if (token >= min(p.num_tokens, __ldcg(p.covered))) {     // (in front of the wait: from L2, whatever this multiprocessor has read before)
     if (row == 0) pdl_wait();      // (a grid that finds nothing to do must not end before the kernels ahead)
     return;
   }
-  const int position = p.positions[token], visible = first_visible_key(position, p.window);
+  const int position = __ldcg(p.positions + token), visible = first_visible_key(position, p.window);
   const int places = p.num_splits + (p.keep_first > 0 ? 1 : 0);
   const int first = visible / p.chunk, window_last = min(p.num_splits - 1, position / p.chunk);
   const int count = window_last - first + 1 + (min(p.keep_first, visible) > 0 ? 1 : 0);      // the kept keys' place comes last

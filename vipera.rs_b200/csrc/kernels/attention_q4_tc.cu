@@ -56,6 +56,7 @@ struct PortionParams {
   float* partial_ml;              // null: the block's split is the only one
   float* partial_out;
   int* status;
+  int* beside;                    // for single tokens that run beside (attention_q4_join.cuh); null: none do
   int gate_per_head, sink;
   int table_width, page_size, num_pages, num_entries, num_tokens, num_heads, num_kv_heads, head_dim;
   float scale;
@@ -252,9 +253,9 @@ __device__ __forceinline__ Job find_job(const PortionParams& p, int index, int g
     const int e = base + lane;
     int start = 0, count = 0, pos0 = 0;
     if (e < p.num_entries) {
-      start = p.entry_starts[e];
-      count = max(p.entry_starts[e + 1] - start, 0);
-      pos0 = p.entry_pos0[e];
+      start = __ldcg(p.entry_starts + e);       // (in front of the wait: from L2, whatever this multiprocessor has read before)
+      count = max(__ldcg(p.entry_starts + e + 1) - start, 0);
+      pos0 = __ldcg(p.entry_pos0 + e);
     }
     if (p.skip_single && count == 1) count = 0;
     const int tiles = (count * group + p.block_rows - 1) / p.block_rows;
@@ -325,9 +326,13 @@ __global__ void __launch_bounds__(kThreads, 1) attention_q4_portions_kernel(cons
   const int begin = kept_split ? 0 : max(split * p.chunk, first_visible_key(low_position, p.window));
   const int end = kept_split ? min(p.keep_first, first_visible_key(high_position, p.window))
                              : min(p.num_splits > 1 ? (split + 1) * p.chunk : 0x7fffffff, high_position + 1);
+  const bool first_block = (blockIdx.x | blockIdx.y | blockIdx.z) == 0;
   if (job.entry < 0 || begin >= end) {  // no rows, or none of them sees a key here and none will be looked for
     // (a grid that found nothing to do must not end before the kernels ahead of it: one block stays for them)
-    if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0) pdl_wait();
+    if (first_block) {
+      pdl_wait();
+      if (p.beside && threadIdx.x == 0) release_word(p.beside, 1);
+    }
     if (warp == kIssueWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
     return;
   }
@@ -348,8 +353,13 @@ __global__ void __launch_bounds__(kThreads, 1) attention_q4_portions_kernel(cons
       pdl_wait();
       // The kernel behind may start from here on: not before every block has its tensor memory (one that took it would wait for this one's end),
       // and with what went before this kernel complete, so that the step's single tokens, which share nothing with the portions, need
-      // not wait for them (DecodeParams::settled in attention_q4.cu).
-      pdl_launch_dependents();
+      // not wait for them (DecodeParams::settled in attention_q4.cu).  One thread says so, in front of its block's leave to start.
+      if (!first_block || !p.beside) {
+        pdl_launch_dependents();
+      } else if (threadIdx.x == 0) {
+        release_word(p.beside, 1);
+        pdl_launch_dependents();
+      }
       // a warp's 32 rows, neighbouring lanes side by side in one row, all asked for before the first is stored
       const long long row_at = (static_cast<long long>(token) * p.num_heads + head) * D;
       const int warp_row = (warp & 3) * 32, piece_of = lane % kPieces, row_of = lane / kPieces;
@@ -541,11 +551,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_q4_portions_kernel(cons
     const int row = threadIdx.x - 32 * kUnpackWarp;
     const int* table = p.block_table + static_cast<size_t>(job.entry) * p.table_width;
     const int shift = (p.page_size & (p.page_size - 1)) == 0 ? 31 - __clz(p.page_size) : -1;
-    auto page_of = [&](int j) {
+    auto page_of = [&](int j, bool waited = true) {
       const int key = (first_tile + j) * kKeys + row;
       if (j >= num_tiles || key < begin || key >= end) return -1;
       const int index = shift >= 0 ? key >> shift : key / p.page_size;
-      const int page = index < p.table_width ? table[index] : -1;
+      const int page = index < p.table_width ? (waited ? table[index] : __ldcg(table + index)) : -1;
       return page < p.num_pages ? page : -1;
     };
     auto row_of = [&](int j, int page) {
@@ -566,7 +576,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_q4_portions_kernel(cons
     // a tile's keys are asked for when the last one's are unpacked, its values behind the last one's, its pages a tile before
     Row<D> keys, values;
     Scales<D> key_scales, value_scales, next_value_scales;
-    int page = page_of(0);
+    int page = page_of(0, false);
     pdl_wait();
     size_t at = page >= 0 ? row_of(0, page) : 0;
     codes(keys, p.k_codes, at, page >= 0);

@@ -1091,7 +1091,7 @@ class _DecodeQ4Params(ctypes.Structure):
                 ("sink_values", _c_void), ("gate", _c_void), ("gate_stride", ctypes.c_longlong), ("gate_per_head", _c_int),
                 ("table_width", _c_int), ("page_size", _c_int), ("page_shift", _c_int), ("num_pages", _c_int), ("num_entries", _c_int), ("num_heads", _c_int),
                 ("num_kv_heads", _c_int), ("head_dim", _c_int), ("scale", _c_float), ("window", _c_int), ("keep_first", _c_int),
-                ("sink", _c_int), ("shares", _c_int), ("settled", _c_int), ("magic", ctypes.c_uint)]
+                ("sink", _c_int), ("shares", _c_int), ("settled", _c_int), ("beside", _c_void), ("magic", ctypes.c_uint)]
 
 
 class _RowsQ4Params(ctypes.Structure):
@@ -1106,7 +1106,7 @@ class _PortionsQ4Params(ctypes.Structure):
     _fields_ = [("q", _c_void), ("out", _c_void), ("k_codes", _c_void), ("v_codes", _c_void), ("k_scales", _c_void), ("v_scales", _c_void),
                 ("entry_starts", _c_void), ("entry_pos0", _c_void), ("block_table", _c_void), ("sink_values", _c_void), ("gate", _c_void),
                 ("gate_stride", ctypes.c_longlong), ("partial_ml", _c_void), ("partial_out", _c_void), ("status", _c_void),
-                ("gate_per_head", _c_int), ("sink", _c_int), ("table_width", _c_int), ("page_size", _c_int), ("num_pages", _c_int),
+                ("beside", _c_void), ("gate_per_head", _c_int), ("sink", _c_int), ("table_width", _c_int), ("page_size", _c_int), ("num_pages", _c_int),
                 ("num_entries", _c_int), ("num_tokens", _c_int), ("num_heads", _c_int), ("num_kv_heads", _c_int), ("head_dim", _c_int),
                 ("scale", _c_float), ("window", _c_int), ("keep_first", _c_int), ("chunk", _c_int), ("num_splits", _c_int),
                 ("skip_single", _c_int), ("block_rows", _c_int)]
@@ -1314,7 +1314,7 @@ def q4_shares(pairs: int, seen: int, sm_count: int, runs: bool = True) -> int:
 
 
 def _attention_q4_decode(q, out, pages, positions, block_table, num_heads, num_kv_heads, head_dim, scale, max_keys, workspace, settled, entry_starts,
-                         window, keep_first, sink, sink_values, gate, gate_offset, gate_per_head) -> None:
+                         window, keep_first, sink, sink_values, gate, gate_offset, gate_per_head, beside=None) -> None:
     fn = _function("attention_q4", "vipera_attention_q4_decode", _DECODE_Q4_ARGS)
     _check_struct("attention_q4", "vipera_attention_q4_params_size", _DecodeQ4Params)
     entries = block_table.shape[0]
@@ -1334,7 +1334,8 @@ def _attention_q4_decode(q, out, pages, positions, block_table, num_heads, num_k
     p = _pack_decode_q4(*_places(what, torch.bfloat16, here, q, out), *_place_pages(what, pages, here),
                         *_places(what, int32, here, positions, block_table, entry_starts), sinks, gate_pointer, gate_stride,
                         1 if gate_per_head else 0, width, pages.k_codes.shape[2], 0, pages.k_codes.shape[0], entries,
-                        num_heads, num_kv_heads, head_dim, scale, window, keep_first, 1 if sink else 0, shares, int(settled), 0)
+                        num_heads, num_kv_heads, head_dim, scale, window, keep_first, 1 if sink else 0, shares, int(settled),
+                        0 if beside is None else beside.data_ptr(), 0)
     if shares:
         _check(fn(p, None, 0, 0, _stream_of(here)), "attention_decode")
     else:
@@ -1429,27 +1430,31 @@ def q4_portion_plan(tokens: int, num_heads: int, num_kv_heads: int, head_dim: in
 
 
 def _attention_q4_portions(q, out, pages, *, entry_starts, entry_pos0, positions, block_table, num_heads, num_kv_heads, head_dim, scale,
-                           max_keys, workspace, window, keep_first, sink, sink_values, gate, gate_offset, gate_per_head, skip_single) -> int:
-    """Launches what the plan says and returns how many kernels those were."""
+                           max_keys, workspace, window, keep_first, sink, sink_values, gate, gate_offset, gate_per_head, skip_single):
+    """Launches what the plan says.  With `skip_single`, and no joining kernel behind, the word by which the single tokens' kernel may run beside
+    this one is returned, else None."""
     fn = _function("attention_q4_tc", "vipera_attention_q4_portions", _PORTIONS_Q4_ARGS)
     _check_struct("attention_q4_tc", "vipera_attention_q4_portions_params_size", _PortionsQ4Params)
     here, int32, what = torch.cuda.current_device(), torch.int32, "attention_q4"
     count, entries = q.shape[0], entry_pos0.numel()
     rows, chunk, splits = q4_portion_plan(count, num_heads, num_kv_heads, head_dim, max_keys, window, _sm_count_of(here))
-    places, scratch = splits + (1 if keep_first else 0), None
+    places, scratch, beside = splits + (1 if keep_first else 0), None, None
     if places > 1:
         scratch = workspace.get("attention.partials", (attention_decode_scratch_floats(count, num_heads, head_dim, places),), torch.float32)
+    elif skip_single:
+        beside = workspace.get("attention.q4_beside", (1,), torch.int32)
     gate_pointer, gate_stride = (0, 0) if gate is None else _gate_pointer(
         gate, gate_offset, count, num_heads * (1 if gate_per_head else head_dim), what)
     sinks, = _places(what, torch.float32, here, sink_values)
     starts_at, pos0_at, table_at, positions_at = _places(what, int32, here, entry_starts, entry_pos0, block_table, positions)
     p = _pack_portions_q4(*_places(what, torch.bfloat16, here, q, out), *_place_pages(what, pages, here), starts_at, pos0_at, table_at, sinks,
-                          gate_pointer, gate_stride, 0, 0, kernel_status_word(q.device).data_ptr(), 1 if gate_per_head else 0,
+                          gate_pointer, gate_stride, 0, 0, kernel_status_word(q.device).data_ptr(),
+                          0 if beside is None else beside.data_ptr(), 1 if gate_per_head else 0,
                           1 if sink else 0, block_table.shape[1], pages.k_codes.shape[2], pages.k_codes.shape[0], entries, count, num_heads,
                           num_kv_heads, head_dim, scale, window, keep_first, chunk, splits, 1 if skip_single else 0, rows)
     _check(fn(p, positions_at, None if scratch is None else scratch.data_ptr(), 0 if scratch is None else scratch.numel(), _stream_of(here)),
            "attention", kernels=2 if places > 1 else 1)
-    return 2 if places > 1 else 1
+    return beside
 
 
 def attention_q4(q: torch.Tensor, out: torch.Tensor, pages: Q4Pages, *, entry_starts: torch.Tensor, entry_pos0: torch.Tensor,
@@ -1503,12 +1508,12 @@ def attention_q4(q: torch.Tensor, out: torch.Tensor, pages: Q4Pages, *, entry_st
         return
     if attention_q4_takes_portions(q.dtype, head_dim, page_size):
         apart = any_single      # single tokens beside portions are the other kernel's
-        kernels = _attention_q4_portions(q, out, pages, entry_starts=entry_starts, entry_pos0=entry_pos0, positions=positions,
-                                         block_table=block_table, max_keys=max_keys, workspace=workspace, skip_single=apart, **heads,
-                                         **endings)
+        beside = _attention_q4_portions(q, out, pages, entry_starts=entry_starts, entry_pos0=entry_pos0, positions=positions,
+                                        block_table=block_table, max_keys=max_keys, workspace=workspace, skip_single=apart, **heads,
+                                        **endings)
         if apart:       # right behind the portions' kernel they need not wait for it (behind a joining one, which writes their rows, they do)
             _attention_q4_decode(q, out, pages, positions=entry_pos0, block_table=block_table, max_keys=max_keys, workspace=workspace,
-                                 settled=2 if kernels == 1 else settled, entry_starts=entry_starts, **heads, **endings)
+                                 settled=settled if beside is None else 2, beside=beside, entry_starts=entry_starts, **heads, **endings)
         return
     # what the flash kernels know of endings decides whether portions are theirs (see parts/attention.py)
     extended = sink_values is not None or gate is not None
