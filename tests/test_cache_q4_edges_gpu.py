@@ -105,3 +105,27 @@ def test_steps_of_portions_alone_and_of_single_tokens_alone_said_to_hold_both(op
         alone.tables = step.tables[:singles]
         expected = _attend(ops, alone, pages, q[:singles].contiguous(), 8, 2, 128)
         assert torch.equal(both[:singles], expected)
+
+
+@pytest.mark.parametrize("heads", [6, 22])
+@pytest.mark.parametrize("d", [64, 128])
+def test_a_group_that_is_not_finite_shows_in_its_own_channels_of_single_tokens(ops, deal, d, heads):
+    """One group of one value, each in turn: the group's outputs of the heads that see it are NaN, all others those of the same step without,
+    bit for bit."""
+    kv_heads, key = 2, 141
+    step = Step([1, 1, 1], [700, 60, 150], 16)
+    raw = plain.make_pages(step.num_pages, 16, kv_heads, d, 3, DEVICE)
+    pages = ops.Q4Pages(*raw)
+    q = torch.randn(3, heads * d, device=DEVICE).to(torch.bfloat16)
+    without = _attend(ops, step, pages, q, heads, kv_heads, d).view(3, heads, d)
+    assert without.isfinite().all()
+    for group in range(d // 32):
+        usual = raw[3].clone()
+        for entry in (0, 2):
+            raw[3][step.tables[entry][key // 16], 1, key % 16, group] = float("nan")
+        with_one = _attend(ops, step, pages, q, heads, kv_heads, d).view(3, heads, d)
+        raw[3].copy_(usual)
+        bad = torch.zeros(3, heads, d, dtype=torch.bool, device=DEVICE)
+        bad[0::2, heads // 2:, 32 * group:32 * group + 32] = True
+        assert with_one[bad].isnan().all()
+        assert torch.equal(with_one[~bad], without[~bad])

@@ -377,7 +377,8 @@ __device__ __forceinline__ void walk(const DecodeParams& p, const Shared<D, NT> 
   __syncthreads();
   const uint32_t magic = p.magic;
   float o[NT][2 * G][4];      // channels 32 gr + 4 g + 2 h and the next (rows g, g + 8), heads 2 t and 2 t + 1, of codes + 136
-  float w_sum[NT][G / 2][4];  // sums of the scaled weights: rows below 8 of a pair's first group, rows above of its second
+  float w_sum[NT][G][4];      // sums of a group's scaled weights, alike in every row (a group's alone: ones in some rows and zeros in others would
+                              // carry a weight that is NaN into the other groups' sums)
   float most[NT][2], base[NT][2], sum[NT][2];   // base: most, or 0 where nothing has been seen
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
@@ -389,10 +390,10 @@ __device__ __forceinline__ void walk(const DecodeParams& p, const Shared<D, NT> 
 #pragma unroll
       for (int m = 0; m < 2 * G; ++m) o[nt][m][i] = 0.0f;
 #pragma unroll
-      for (int pair = 0; pair < G / 2; ++pair) w_sum[nt][pair][i] = 0.0f;
+      for (int gr = 0; gr < G; ++gr) w_sum[nt][gr][i] = 0.0f;
     }
   }
-  const uint32_t ones[2][4] = {{kOnes, 0, kOnes, 0}, {0, kOnes, 0, kOnes}};
+  const uint32_t ones[4] = {kOnes, kOnes, kOnes, kOnes};
   const int row_key = 4 * (g & 1) + (g >> 1);                       // the key of accumulator row g
   const uint32_t v_from = t * kRowBytes + (kChunks == 4 ? ((g >> 1) ^ (t & 2)) * 16 + (g & 1) * 8 : g * (2 * G));
 
@@ -488,9 +489,9 @@ __device__ __forceinline__ void walk(const DecodeParams& p, const Shared<D, NT> 
             o[nt][n][2 + c] *= shrink;
           }
 #pragma unroll
-          for (int pair = 0; pair < G / 2; ++pair) {
-            w_sum[nt][pair][c] *= shrink;
-            w_sum[nt][pair][2 + c] *= shrink;
+          for (int gr = 0; gr < G; ++gr) {
+            w_sum[nt][gr][c] *= shrink;
+            w_sum[nt][gr][2 + c] *= shrink;
           }
         }
     }
@@ -540,7 +541,7 @@ __device__ __forceinline__ void walk(const DecodeParams& p, const Shared<D, NT> 
           for (int nt = 0; nt < NT; ++nt) mma_bf16(o[nt][2 * gr + half], a, b[nt][0], b[nt][1]);
         }
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) mma_bf16(w_sum[nt][gr / 2], ones[gr & 1], b[nt][0], b[nt][1]);
+        for (int nt = 0; nt < NT; ++nt) mma_bf16(w_sum[nt][gr], ones, b[nt][0], b[nt][1]);
       }
     }
     __syncwarp();   // the stage is free
@@ -553,7 +554,7 @@ __device__ __forceinline__ void walk(const DecodeParams& p, const Shared<D, NT> 
 #pragma unroll
     for (int m = 0; m < 2 * G; ++m)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) o[nt][m][c] = fmaf(-kOffset, w_sum[nt][m / 4][(m & 2) + (c & 1)], o[nt][m][c]);
+      for (int c = 0; c < 4; ++c) o[nt][m][c] = fmaf(-kOffset, w_sum[nt][m / 2][c & 1], o[nt][m][c]);
 
   // each warp leaves its partial in shared memory
   float* mine = merge + warp * (8 * NT * kRow);
