@@ -129,3 +129,23 @@ def test_a_group_that_is_not_finite_shows_in_its_own_channels_of_single_tokens(o
         bad[0::2, heads // 2:, 32 * group:32 * group + 32] = True
         assert with_one[bad].isnan().all()
         assert torch.equal(with_one[~bad], without[~bad])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("page_size", [16, 24])
+@pytest.mark.parametrize("scale", [-0.3, 0.0])
+def test_scales_that_are_not_positive(ops, form, dtype, page_size, scale):
+    """A scale below 0 turns the order of the scores, one of 0 weighs all keys alike; hidden keys stay hidden."""
+    heads, kv_heads, d = 6, 2, 64
+    step = Step([50, 1, 70], [40, 300, 0], page_size)
+    raw = plain.make_pages(step.num_pages, page_size, kv_heads, d, 3, DEVICE)
+    k_rows, v_rows = plain.rows_of(raw[0], raw[1], True), plain.rows_of(raw[2], raw[3], False)
+    q = torch.randn(121, heads * d, device=DEVICE).to(dtype)
+    got = _attend(ops, step, ops.Q4Pages(*raw), q, heads, kv_heads, d, scale=scale).double().cpu().numpy().reshape(121, heads, d)
+    expected, parts = plain.attend(q.double().cpu().numpy(), k_rows, v_rows, counts=step.counts, history=step.history, tables=step.tables,
+                                   page_size=page_size, num_heads=heads, num_kv_heads=kv_heads, d=d, scale=scale,
+                                   k_steps=raw[1].double().cpu().numpy(), v_steps=raw[3].double().cpu().numpy())
+    for name in ("reach", "full"):      # sizes of scores' terms
+        parts[name] = np.abs(parts[name])
+    limit = plain.allowed(expected, parts, 301, d, dtype)
+    assert (np.abs(got - expected) <= limit).all()

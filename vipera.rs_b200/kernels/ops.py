@@ -1502,11 +1502,15 @@ def attention_q4(q: torch.Tensor, out: torch.Tensor, pages: Q4Pages, *, entry_st
     heads = dict(num_heads=num_heads, num_kv_heads=num_kv_heads, head_dim=head_dim, scale=scale, window=window)
     endings = dict(keep_first=keep_first, sink=sink, sink_values=sink_values, gate=gate, gate_offset=gate_offset,
                    gate_per_head=gate_per_head)
-    if attention_q4_takes_rows(q.dtype, head_dim, page_size, count * num_heads, max_keys, 1 if any_single else entries):
+    # The tensor cores' and the flash kernels find a row's largest score before they scale it: a scale that is not above 0, which turns or levels
+    # the scores' order, is for the kernels that scale first.
+    rising = scale > 0
+    if attention_q4_takes_rows(q.dtype, head_dim, page_size, count * num_heads if rising else 0, max_keys,
+                               1 if any_single or not rising else entries):
         _attention_q4_rows(q, out, pages, entry_starts=entry_starts, entry_pos0=entry_pos0, positions=positions, block_table=block_table,
                            max_keys=max_keys, workspace=workspace, **heads, **endings)
         return
-    if attention_q4_takes_portions(q.dtype, head_dim, page_size):
+    if rising and attention_q4_takes_portions(q.dtype, head_dim, page_size):
         apart = any_single      # single tokens beside portions are the other kernel's
         beside = _attention_q4_portions(q, out, pages, entry_starts=entry_starts, entry_pos0=entry_pos0, positions=positions,
                                         block_table=block_table, max_keys=max_keys, workspace=workspace, skip_single=apart, **heads,
@@ -1517,7 +1521,7 @@ def attention_q4(q: torch.Tensor, out: torch.Tensor, pages: Q4Pages, *, entry_st
         return
     # what the flash kernels know of endings decides whether portions are theirs (see parts/attention.py)
     extended = sink_values is not None or gate is not None
-    flash = (q.dtype == torch.bfloat16 and head_dim in MMA_HEAD_DIMS and
+    flash = (rising and q.dtype == torch.bfloat16 and head_dim in MMA_HEAD_DIMS and
              not (extended and (keep_first or head_dim not in TC_ATTENTION_HEAD_DIMS or os.environ.get("VIPERA_ATTENTION_TC", "1") == "0"
                                 or not attention_tc_takes_gate(gate, gate_offset, gate_per_head))))
     apart = flash and packed and any_single     # single tokens beside portions read the packed pages
