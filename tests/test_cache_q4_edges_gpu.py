@@ -149,3 +149,18 @@ def test_scales_that_are_not_positive(ops, form, dtype, page_size, scale):
         parts[name] = np.abs(parts[name])
     limit = plain.allowed(expected, parts, 301, d, dtype)
     assert (np.abs(got - expected) <= limit).all()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("queries, keys", [(126, -100), (124, -100), (100, -20), (-100, 60), (0, 117), (0, -90)])
+def test_single_tokens_with_numbers_near_the_ends_of_the_type(ops, deal, d, queries, keys):
+    """Queries and keys times powers of two, the scale divided by them: nothing on the way to a score leaves its type, so the outputs are the
+    same bits."""
+    step = Step([1, 1], [190, 17], 16)
+    raw = plain.make_pages(step.num_pages, 16, 1, d, 3, DEVICE)
+    q = torch.randn(2, 4 * d, device=DEVICE).clamp(-1.9, 1.9).to(torch.bfloat16)
+    usual = _attend(ops, step, ops.Q4Pages(*raw), q, 4, 1, d)
+    far = q.double() * 2.0 ** queries
+    assert torch.equal(far.to(torch.bfloat16).double(), far)
+    raw[1].mul_(2.0 ** keys)
+    assert torch.equal(_attend(ops, step, ops.Q4Pages(*raw), far.to(torch.bfloat16), 4, 1, d, scale=0.1 * 2.0 ** -(queries + keys)), usual)

@@ -352,9 +352,9 @@ __device__ __forceinline__ void walk(const DecodeParams& p, const Shared<D, NT> 
     }
     // the largest to 2^14 .. 2^15 (a number that is not finite: everything NaN)
     const int exponent = static_cast<int>(__float_as_uint(largest) >> 23) - 127;
-    const int up = min(max(14 - exponent, -110), 110);
+    const int up = min(max(14 - exponent, -113), 110);
     const float lift = fine ? __uint_as_float(static_cast<uint32_t>(127 + up) << 23) : __int_as_float(0x7fffffff);
-    const float factor = p.scale * kLog2e * __uint_as_float(static_cast<uint32_t>(127 - up) << 23) * 0x1p24f;   // a code is u 2^-24
+    const float factor = ldexpf(p.scale * kLog2e, 24 - up);   // a code is u 2^-24 (both powers at once: one alone may leave the type)
     q_factor[nt][0] = __shfl_sync(0xffffffffu, factor, 8 * t);
     q_factor[nt][1] = __shfl_sync(0xffffffffu, factor, 8 * t + 4);
 #pragma unroll
