@@ -50,3 +50,22 @@ def test_single_tokens_beside_portions_are_refused_without_their_word():
     for settled, beside in ((2, 0), (3, at), (-1, at)):
         block = ops._pack_decode_q4(at, at, at, at, at, at, at, at, at, 0, 0, 0, 0, 2, 16, 0, 4, 1, 4, 2, 64, 0.125, 0, 0, 0, 1, settled, beside, 0)
         assert fn(block, None, 0, 0, None) == -3
+
+
+def test_the_command_line_plans_no_other_cache_than_the_one_it_was_asked_for(tmp_path, capsys):
+    import json
+
+    import helpers
+    from vipera_rs_b200 import cli
+
+    (tmp_path / "config.json").write_text(json.dumps(helpers.CONFIGS["A"]))
+    command = ["plan", str(tmp_path), "--ctx", "64", "--json"]
+    assert cli.main(command) == 0
+    usual = capsys.readouterr().out
+    for name in ("bf16", "bfloat16", "f32", "float32"):       # names of the run's type, as for generate
+        assert cli.main([*command, "--kv-type", name]) == 0
+        assert capsys.readouterr().out == usual
+    for name in ("q5", "Q4", "q8_0", ""):
+        assert cli.main([*command, "--kv-type", name]) == 2
+        told = capsys.readouterr()
+        assert told.out == "" and "--kv-type" in told.err

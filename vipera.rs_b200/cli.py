@@ -137,6 +137,16 @@ def plan_memory(model_dir: str, ctx: int, batch: int, dtype: str, device_bytes: 
     return planner.plan_memory(arch.model_spec(config), ctx, batch, dtype, device_bytes, page_size, kv_type)
 
 
+def _kv_type(found: dict) -> Optional[str]:
+    """--kv-type as the engine and the plan take it: None for the run's type, by whichever name."""
+    kv_type = found.get("kv_type")
+    if kv_type in (None, "bf16", "bfloat16", "f32", "float32"):
+        return None
+    if kv_type != "q4":
+        raise InvalidArgumentError(f"--kv-type {kv_type!r}: the cache has the run's dtype, or 4 bits a value and scales (q4)")
+    return kv_type
+
+
 def plan(args: List[str]) -> int:
     found, places = _parse(args, "plan", {"--ctx": ("ctx", int), "--batch": ("batch", int),
                                           "--dtype": ("dtype", str), "--kv-type": ("kv_type", str),
@@ -146,7 +156,7 @@ def plan(args: List[str]) -> int:
         raise UsageError("plan needs a model path")
     report = plan_memory(places[0], found.get("ctx", 2048), found.get("batch", 1),
                          found.get("dtype", "bfloat16"), found.get("device_bytes"), found.get("page_size", 16),
-                         "q4" if found.get("kv_type") == "q4" else None)
+                         _kv_type(found))
     if found.get("json"):
         print(json.dumps(report, indent=2))
     else:
@@ -190,9 +200,7 @@ def generate(args: List[str]) -> int:
     if max_tokens < 1:
         raise InvalidArgumentError("--max-tokens must be at least 1")
     dtype = found.get("dtype", "bfloat16")
-    kv_type = found.get("kv_type")
-    if kv_type is not None and kv_type not in ("bf16", "bfloat16", "f32", "float32", "q4"):
-        raise InvalidArgumentError(f"--kv-type {kv_type!r}: the cache has the run's dtype, or 4 bits a value and scales (q4)")
+    kv_type = _kv_type(found)
 
     from .engine.engine import Engine
     from .sampling import SamplingParams
@@ -205,7 +213,7 @@ def generate(args: List[str]) -> int:
         frequency_penalty=found.get("frequency_penalty", 0.0), seed=found.get("seed", 0))
     engine = Engine(places[0], dtype=dtype, device=found.get("device", "cuda:0"),
                     page_size=found.get("page_size", 16), ctx=found.get("ctx"), max_num_seqs=1,
-                    kv_type="q4" if kv_type == "q4" else None)
+                    kv_type=kv_type)
     as_json = bool(found.get("json"))
     eos = set(engine.default_eos)
 
