@@ -69,3 +69,39 @@ def test_the_command_line_plans_no_other_cache_than_the_one_it_was_asked_for(tmp
         assert cli.main([*command, "--kv-type", name]) == 2
         told = capsys.readouterr()
         assert told.out == "" and "--kv-type" in told.err
+
+
+@pytest.mark.parametrize("heads, kv_heads, head_dim, window, keep_first", [(8, 8, 128, 0, 0), (12, 2, 128, 0, 0), (28, 4, 128, 0, 0), (14, 2, 64, 0, 0),
+                                                                         (28, 4, 128, 5000, 4)])
+@pytest.mark.parametrize("ctx", [256, 8192, 32000])
+def test_the_plan_counts_the_parts_that_a_step_asks_for(heads, kv_heads, head_dim, window, keep_first, ctx):
+    """Buffers of parts as the launches size them, for steps of any length up to the planned one, stay within the plan."""
+    import vipera_rs_b200  # noqa: F401
+    from vipera_rs_b200.engine import planner
+    from vipera_rs_b200.kernels import ops
+
+    kept = 1 if keep_first else 0
+    for batch in (1, 64):
+        planned = planner.part_bytes(heads, kv_heads, head_dim, window, keep_first, ctx, batch, 2, 16)
+        asked = [0]
+        for tokens in (64, 128, 512, 1024, 1536, 2048):
+            for keys in {ctx, ctx * 3 // 4, 2048}:
+                if tokens <= keys <= ctx:
+                    cuts = ops.q4_portion_plan(tokens, heads, kv_heads, head_dim, keys, window, 148)[2] + kept
+                    asked.append(ops.attention_decode_scratch_floats(tokens, heads, head_dim, cuts) if cuts > 1 else 0)
+                    splits = ops.q4_rows_splits(kv_heads * -(-tokens * (heads // kv_heads) // 16), keys, 148)[1] + kept
+                    asked.append(ops.attention_decode_scratch_floats(tokens, heads, head_dim, splits))
+        assert 4 * max(asked) <= planned + 16
+    if ctx == 8192 and not window:
+        assert planner.part_bytes(8, 8, 128, 0, 0, ctx, 1, 2, 16) >= 3 * 2048 * 8 * 130 * 4
+
+
+def test_the_plan_of_a_model_holds_its_layers_parts():
+    import helpers
+    from vipera_rs_b200.config import architecture_of
+    from vipera_rs_b200.engine import planner
+
+    raw = dict(helpers.CONFIGS["A"], hidden_size=1536, num_attention_heads=12, num_key_value_heads=2, max_position_embeddings=32768)
+    arch = architecture_of(raw)
+    spec = arch.model_spec(arch.config_from_dict(raw))
+    assert planner.room_bytes(spec, 8192, 1, 2) == planner.part_bytes(12, 2, 128, 0, 0, 8192, 1, 2, 16) >= 2 * 2048 * 12 * 130 * 4

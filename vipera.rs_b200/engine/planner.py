@@ -19,6 +19,7 @@ from ..weights.loader import FREE_EXTENT
 
 DEVICE_RESERVE_BYTES = 16 << 20  # kept free on the device (crates/vipera-core/src/planner.rs:23)
 PLANNED_STEP_TOKENS = 2048       # the step the workspace is sized for
+PLANNED_MULTIPROCESSORS = 148    # of the device it runs on
 PRODUCT_SCRATCH_BYTES = 32 << 20  # partial sums of split products (the buffer starts at this size)
 PRODUCT_PARTS_BYTES = 96 << 20    # the parts of a 32-bit product's left operand, at most (gemm_split.cuh: kMostParts)
 
@@ -85,6 +86,31 @@ def kv_bytes_per_token(spec: ModelSpec, element_bytes: int, kv_type: Optional[st
     return sum(group.bytes_per_token(element_bytes, kv_type) for group in groups)
 
 
+def part_bytes(heads: int, kv_heads: int, head_dim: int, window: int, keep_first: int, ctx: int, batch: int, element_bytes: int,
+               page_size: int) -> int:
+    """The parts of a layer's outputs where attention over pages of 4 bits cuts its keys: outputs, maximum and sum of every token and head of a
+    planned step, once, or as often as a bfloat16 step of any size up to that is cut (`ops.q4_portion_plan`), and once more for kept first keys; or
+    those of the even runs of a batch's single tokens.  (The kernel of any number of rows has 9,472 rows of parts at most, of four blocks of 16 rows
+    a multiprocessor, unless a row has one part: no more than the planned step's from five heads on.)"""
+    from ..kernels import ops
+
+    kept = 1 if window and keep_first else 0
+    places = PLANNED_STEP_TOKENS * (1 + kept)
+    most = 0
+    if element_bytes == 2 and head_dim in ops.TC_ATTENTION_HEAD_DIMS and page_size % 16 == 0:
+        lengths = [ctx] + [2 ** i for i in range(8, 31) if 2 ** i < ctx]
+        for tokens in range(64, PLANNED_STEP_TOKENS + 1, 64):
+            for keys in lengths:
+                cuts = ops.q4_portion_plan(tokens, heads, kv_heads, head_dim, keys, window, PLANNED_MULTIPROCESSORS)[2]
+                places = max(places, tokens * (cuts + kept))
+        wide = heads // kv_heads > 8
+        pairs = batch * kv_heads * -(-(heads // kv_heads) // (16 if wide else 8))
+        if not ops.q4_shares(pairs, min(ctx, window + keep_first) if window else ctx, PLANNED_MULTIPROCESSORS, batch <= ops.Q4_RUNS_ENTRIES):
+            runs = (2 if wide else ops.Q4_BLOCKS_PER_SM) * PLANNED_MULTIPROCESSORS
+            most = runs * 2 * (16 if wide else 8) * (head_dim + 4) * 4
+    return max(most, places * heads * (head_dim + 2) * 4)
+
+
 def room_bytes(spec: ModelSpec, ctx: int, batch: int, element_bytes: int, page_size: int = 16) -> int:
     """What attention over pages of 4 bits needs beside them: the parts of a step's outputs, and, where it does not read them packed (heads
     other than 64 and 128, pages not of a multiple of 16 tokens), a room to expand a layer's rows to: one cache slot's pages in the run's
@@ -92,8 +118,10 @@ def room_bytes(spec: ModelSpec, ctx: int, batch: int, element_bytes: int, page_s
     groups, _ = plan_groups(spec_cache_requests(spec))
     room = max([(batch * _group_tokens(group, ctx, page_size) + page_size) * group.bytes_per_token(element_bytes) // len(group.slots)
                 for group in groups if group.head_dim not in (64, 128) or page_size % 16] or [0])
-    parts = [part.params for layer in spec.layers for part in layer.parts.values()]
-    return room + PLANNED_STEP_TOKENS * 4 * max(int(p.get("num_heads", 0)) * (int(p.get("head_dim", 0)) + 2) for p in parts)
+    params = [part.params for layer in spec.layers for part in layer.parts.values()]
+    attends = {tuple(int(p.get(key) or 0) for key in ("num_heads", "num_kv_heads", "head_dim", "window", "keep_first"))
+               for p in params if p.get("num_heads") and p.get("num_kv_heads") and p.get("head_dim")}
+    return room + max([part_bytes(*sizes, ctx, batch, element_bytes, page_size) for sizes in attends] or [0])
 
 
 def workspace_bytes(spec: ModelSpec, batch: int, element_bytes: int, tokens: int = PLANNED_STEP_TOKENS) -> int:
