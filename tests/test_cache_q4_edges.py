@@ -105,3 +105,14 @@ def test_the_plan_of_a_model_holds_its_layers_parts():
     arch = architecture_of(raw)
     spec = arch.model_spec(arch.config_from_dict(raw))
     assert planner.room_bytes(spec, 8192, 1, 2) == planner.part_bytes(12, 2, 128, 0, 0, 8192, 1, 2, 16) >= 2 * 2048 * 12 * 130 * 4
+
+
+def test_what_a_step_builds_on_the_device_shares_no_line_with_what_it_builds_it_from():
+    import vipera_rs_b200  # noqa: F401
+    from vipera_rs_b200.engine.runner import step_offsets
+
+    for copied in ([3, 2, 1, 1, 1, 0, 2, 5], [32], [31, 1], [100, 4, 29]):
+        offsets, places = step_offsets(copied, [3, 3, 8, 0])
+        assert offsets == [sum(copied[:i]) for i in range(len(copied) + 1)]
+        assert places[0] % 32 == 0 and offsets[-1] <= places[0] < offsets[-1] + 32
+        assert [b - a for a, b in zip(places, places[1:])] == [3, 3, 8, 0]

@@ -39,6 +39,19 @@ class StepInput:
     logit_rows: np.ndarray      # int32 indices into tokens
 
 
+# 32-bit numbers that a multiprocessor fetches together, at most
+_LINE = 32
+
+
+def step_offsets(copied, built):
+    """Where a step's pieces lie in its buffer, with the end behind them: those that are copied to the device, then, from a line of their own on,
+    those that the device builds.  (Kernels read the latter in front of their wait, so no line of them may have been fetched by
+    the kernel that builds them from the former.)"""
+    offsets = np.concatenate([[0], np.cumsum(copied)]).astype(np.int64).tolist()
+    first = -(-offsets[-1] // _LINE) * _LINE
+    return offsets, (first + np.concatenate([[0], np.cumsum(built)])).astype(np.int64).tolist()
+
+
 def _round_up_pow2(value: int, least: int = 8) -> int:
     out = least
     while out < value:
@@ -219,25 +232,23 @@ class ModelRunner:
             widths.append(_round_up_pow2(max((max_len + page_size - 1) // page_size, int(np.diff(page_starts).max()))))
             pieces += [page_starts, pages]
         # what the device builds lies behind what is copied: positions, the tokens' entries, the tables
-        sizes = [p.shape[0] for p in pieces] + [total, total] + [entries * width for width in widths]
-        offsets = np.concatenate([[0], np.cumsum(sizes)]).astype(np.int64).tolist()
-        host, dev = self._staging(offsets[-1])
+        offsets, places = step_offsets([p.shape[0] for p in pieces], [total, total] + [entries * width for width in widths])
+        host, dev = self._staging(places[-1])
         if self._copy_pending:
             self._copy_done.synchronize()
         view = host.numpy()
         for piece, offset in zip(pieces, offsets):
             view[offset:offset + piece.shape[0]] = piece
-        copied = offsets[len(pieces)]
+        copied = offsets[-1]
         dev[:copied].copy_(host[:copied], non_blocking=True)
         self._copy_done.record()
         self._copy_pending = True
 
-        def part(index):
+        def part(index, offsets=offsets):
             return dev[offsets[index]:offsets[index + 1]]
 
-        behind = len(pieces)
-        positions, token_entry = part(behind), part(behind + 1)
-        block_tables = [part(behind + 2 + g).view(entries, width) for g, width in enumerate(widths)]
+        positions, token_entry = part(0, places), part(1, places)
+        block_tables = [part(2 + g, places).view(entries, width) for g, width in enumerate(widths)]
         if not block_tables:     # nothing is kept in pages
             ops.step_maps(part(1), part(2), page_size=1, block_table=dev[:0].view(entries, 0), positions=positions, token_entry=token_entry)
         for g, table in enumerate(block_tables):
