@@ -164,3 +164,17 @@ def test_single_tokens_with_numbers_near_the_ends_of_the_type(ops, deal, d, quer
     assert torch.equal(far.to(torch.bfloat16).double(), far)
     raw[1].mul_(2.0 ** keys)
     assert torch.equal(_attend(ops, step, ops.Q4Pages(*raw), far.to(torch.bfloat16), 4, 1, d, scale=0.1 * 2.0 ** -(queries + keys)), usual)
+
+
+def test_a_first_mixed_step_leaves_captured_steps_valid(ops, monkeypatch):
+    """A workspace that has seen a step of portions alone holds all that a mixed one asks for: nothing captured before goes stale."""
+    monkeypatch.setattr(ops, "Q4_ROWS_WORK", 0)
+    monkeypatch.setattr(ops, "q4_portion_plan", lambda *a: (256, 1 << 20, 1))
+    room, seen = _workspace(), []
+    for counts in ([70, 150], [70, 150, 1]):
+        step = Step(counts, [0, 900, 30][:len(counts)], 16)
+        pages = ops.Q4Pages(*plain.make_pages(step.num_pages, 16, 2, 128, 3, DEVICE))
+        q = torch.randn(sum(counts), 8 * 128, device=DEVICE).to(torch.bfloat16)
+        _attend(ops, step, pages, q, 8, 2, 128, workspace=room)
+        seen.append(room.generation)
+    assert seen[0] == seen[1]

@@ -1438,11 +1438,12 @@ def _attention_q4_portions(q, out, pages, *, entry_starts, entry_pos0, positions
     here, int32, what = torch.cuda.current_device(), torch.int32, "attention_q4"
     count, entries = q.shape[0], entry_pos0.numel()
     rows, chunk, splits = q4_portion_plan(count, num_heads, num_kv_heads, head_dim, max_keys, window, _sm_count_of(here))
-    places, scratch, beside = splits + (1 if keep_first else 0), None, None
+    places, scratch = splits + (1 if keep_first else 0), None
+    beside = workspace.get("attention.q4_beside", (1,), torch.int32)      # (asked for by every step: no later one makes captured steps stale with it)
     if places > 1:
         scratch = workspace.get("attention.partials", (attention_decode_scratch_floats(count, num_heads, head_dim, places),), torch.float32)
-    elif skip_single:
-        beside = workspace.get("attention.q4_beside", (1,), torch.int32)
+    if places > 1 or not skip_single:
+        beside = None
     gate_pointer, gate_stride = (0, 0) if gate is None else _gate_pointer(
         gate, gate_offset, count, num_heads * (1 if gate_per_head else head_dim), what)
     sinks, = _places(what, torch.float32, here, sink_values)
