@@ -116,3 +116,35 @@ def test_what_a_step_builds_on_the_device_shares_no_line_with_what_it_builds_it_
         assert offsets == [sum(copied[:i]) for i in range(len(copied) + 1)]
         assert places[0] % 32 == 0 and offsets[-1] <= places[0] < offsets[-1] + 32
         assert [b - a for a, b in zip(places, places[1:])] == [3, 3, 8, 0]
+
+
+def test_a_steps_pieces_are_written_one_behind_the_other_for_the_device():
+    import numpy as np
+
+    from vipera_rs_b200.build import runtime_module
+    from vipera_rs_b200.errors import InvalidArgumentError
+
+    manager = runtime_module().CacheManager([(16, 20, 0, 0), (8, 40, 32, 0)], 4, False)
+    for request, length in ((0, 40), (1, 5), (2, 80)):
+        manager.open(request)
+        manager.reserve(request, length)
+    manager.commit(2, 72)                    # the window's group gives pages back
+    requests, counts, pos0, fresh = [2, 0, 1], [8, 1, 5], [72, 39, 0], [0, 0, 1]
+    tokens, rows = np.arange(100, 114, dtype=np.int32), np.asarray([7, 13], dtype=np.int32)
+    lists = [manager.page_lists(requests, g) for g in (0, 1)]
+    expected = [tokens, [0, 8, 9, 14], pos0, [manager.state_slot(r) for r in requests], fresh, rows] + [p for pair in lists for p in pair]
+    buffer = np.full(300, 77, dtype=np.int32)
+    sizes, longest = manager.fill_step(requests, tokens, counts, pos0, fresh, rows, buffer.ctypes.data, buffer.size)
+    assert sizes == [len(piece) for piece in expected] and longest == [5, 10]
+    assert buffer[:sum(sizes)].tolist() == [int(x) for piece in expected for x in piece]
+    assert (buffer[sum(sizes):] == 77).all()
+    # a buffer that is too small stays as it was, and the sizes are told all the same
+    small = np.full(sum(sizes) - 1, 77, dtype=np.int32)
+    assert manager.fill_step(requests, tokens, counts, pos0, fresh, rows, small.ctypes.data, small.size) == (sizes, longest)
+    assert (small == 77).all()
+    for change in (dict(pos0=[72, 60, 0]), dict(pos0=[0, 39, 0], counts=[8, 1, 20])):      # no page for a last position
+        given = dict(dict(counts=counts, pos0=pos0), **change)
+        with pytest.raises(InvalidArgumentError):
+            manager.fill_step(requests, tokens, given["counts"], given["pos0"], fresh, rows, buffer.ctypes.data, buffer.size)
+    with pytest.raises(InvalidArgumentError):
+        manager.fill_step(requests, tokens, counts[:2], pos0, fresh, rows, buffer.ctypes.data, buffer.size)

@@ -18,12 +18,12 @@
 //            were 2^10: off by 2^-22 of that.
 //   values   codes become bfloat16 by a shift, a mask and an OR (0x4300 | u is 128 + u, 136 above the code); the weights take the
 //            scales in 32 bits, w[key, head, g] = p[key, head] scale[key, g], and are rounded to bfloat16 once; a product with
-//            ones sums them, and 136 times that sum goes off at the end.
+//            ones sums a group's, and 136 times that sum goes off at the end.
 // A score's accumulators have the keys on their rows, the second product wants them on its inner axis: movmatrix turns the
 // weights' 8 x 8 blocks in registers, so nothing passes through shared memory until the end.
 //
-// What bounds it.  48 requests of 8,192 keys, 40 heads of 128 on 8: 455 MB, read once, in 113 to 118 us with the joining kernel, 3.9 TB/s
-// (60 % of the measured copy).  It is bound by issuing: 16 keys of a head are 290 instructions of a warp (156 of them integer and logic, 20
+// What bounds it.  48 requests of 8,192 keys, 40 heads of 128 on 8: 455 MB, read once, in 116 to 121 us with the joining kernel, 3.8 TB/s
+// (58 % of the measured copy).  It is bound by issuing: 16 keys of a head are 290 instructions of a warp (156 of them integer and logic, 20
 // products), issue slots are 59 % busy and the integer pipe 56 %, and fetching, unpacking, scaling and weighing each shorten the time by
 // less than their share when taken out.  More blocks an SM (four of 128 registers), more or fewer stages and rows read
 // straight into registers change nothing; 8-bit operands (e4m3, where a nibble is a number as it stands) cost conversions on this

@@ -1,6 +1,6 @@
 // Attention of a step's tokens over pages of 4 bits, any number of tokens a request, split over the keys; part of attention_q4.cu.
 //
-// A block is (8 NT of the (token, query head) rows of one request and KV head, split of the keys); its four warps fold 32 keys at a
+// A block is (8 NT of the (token, query head) rows of one request and KV head, split of the keys); its four warps fold 16 keys at a
 // time each.  Rows lie on the side of 8 of both products, as in the kernel of single tokens, each with a range of visible keys of its
 // own.  What differs is exactness: codes become bfloat16 numbers exactly (128 + u less 136), and a 32-bit number (a query's channel, a
 // weight times the value's scale) is the exact sum of three bfloat16 ones, each a product of its own, so that 32-bit steps are as exact

@@ -5,8 +5,8 @@
 //   s = round5(-m / 8),   five significant bits, ties to even,
 // its codes are c = the nearest whole number to x / s (ties to even) within -8 .. 7, and the row stands for
 // c * s.  The signed scale puts m itself on code -8, the end of the range that has a code more, so a step is
-// an eighth of the magnitude and not a seventh.  Five bits of scale cost at most 1/64 of m at the far end
-// (a quarter of a code's half step) and make every c * s a bfloat16 exactly (|c| <= 7 has three bits, 8 is
+// an eighth of the magnitude and not a seventh.  Five bits of scale cost at most 1/33 of m at the far end
+// (a half of a code's half step, m / 16) and make every c * s a bfloat16 exactly (|c| <= 7 has three bits, 8 is
 // a power of two): a row can be expanded to bfloat16 without a second rounding.  Whether x lies nearer to one code or the next
 // is decided exactly: a border is (c + 1/2) s, nine significant bits at most, and a quotient in 32 bits
 // falls on a border's own quotient only if x does.

@@ -3,6 +3,7 @@
 #include <pybind11/pybind11.h>
 #include <pybind11/stl.h>
 
+#include <algorithm>
 #include <cstring>
 
 #include "cache_manager.hpp"
@@ -236,6 +237,65 @@ PYBIND11_MODULE(_vipera_runtime, m) {
                out_tables += b * width;
              }
              return n;
+           })
+      // What is copied to the device of a step that is launched kernel by kernel, one piece behind the other into a host buffer of
+      // `room` numbers that the caller owns: [tokens][entry starts n + 1][first positions n][state slots n][fresh n][wanted rows], then for each group
+      // where its requests' pages begin [n + 1] and those pages.  Returns (the pieces' sizes, the longest page list of each group); a buffer
+      // that is too small is left as it was.  The step has been checked but for its pages: every entry's last position must have one.
+      .def("fill_step",
+           [](const CacheManager& c, const std::vector<int64_t>& requests, py::array_t<int32_t, py::array::c_style | py::array::forcecast> tokens,
+              py::array_t<int32_t, py::array::c_style | py::array::forcecast> counts, py::array_t<int32_t, py::array::c_style | py::array::forcecast> pos0,
+              py::array_t<int32_t, py::array::c_style | py::array::forcecast> fresh, py::array_t<int32_t, py::array::c_style | py::array::forcecast> rows,
+              uintptr_t host, int64_t room) {
+             const size_t n = requests.size();
+             if (counts.size() != static_cast<py::ssize_t>(n) || pos0.size() != counts.size() || fresh.size() != counts.size())
+               throw InvalidArgument("requests, counts and first positions must have one item per entry");
+             std::vector<int64_t> sizes{tokens.size(), static_cast<int64_t>(n) + 1, static_cast<int64_t>(n), static_cast<int64_t>(n),
+                                        static_cast<int64_t>(n), rows.size()};
+             std::vector<int64_t> longest;
+             int64_t total = 0;
+             for (int g = 0; g < c.num_groups(); ++g) {
+               const int page_size = c.group(g).page_size;
+               int64_t pages = 0, most = 0;
+               for (size_t i = 0; i < n; ++i) {
+                 const std::vector<int32_t>& table = c.table(requests[i], g);
+                 const int64_t last = (static_cast<int64_t>(pos0.data()[i]) + counts.data()[i] - 1) / page_size;
+                 if (last < 0 || last >= static_cast<int64_t>(table.size()) || table[last] < 0)
+                   throw InvalidArgument("a request of the step has no page reserved for its last position");
+                 pages += static_cast<int64_t>(table.size());
+                 most = std::max(most, static_cast<int64_t>(table.size()));
+               }
+               sizes.push_back(static_cast<int64_t>(n) + 1);
+               sizes.push_back(pages);
+               longest.push_back(most);
+             }
+             for (int64_t size : sizes) total += size;
+             if (total <= room) {
+               int32_t* out = reinterpret_cast<int32_t*>(host);
+               out = std::copy_n(tokens.data(), tokens.size(), out);
+               int32_t start = 0;
+               for (size_t i = 0; i < n; ++i) {
+                 *out++ = start;
+                 start += counts.data()[i];
+               }
+               *out++ = start;
+               out = std::copy_n(pos0.data(), n, out);
+               for (size_t i = 0; i < n; ++i) *out++ = c.state_slot(requests[i]);
+               out = std::copy_n(fresh.data(), n, out);
+               out = std::copy_n(rows.data(), rows.size(), out);
+               for (int g = 0; g < c.num_groups(); ++g) {
+                 int32_t *starts = out, *pages = out + n + 1, at = 0;
+                 for (size_t i = 0; i < n; ++i) {
+                   const std::vector<int32_t>& table = c.table(requests[i], g);
+                   *starts++ = at;
+                   pages = std::copy(table.begin(), table.end(), pages);
+                   at += static_cast<int32_t>(table.size());
+                 }
+                 *starts = at;
+                 out = pages;
+               }
+             }
+             return py::make_tuple(sizes, longest);
            })
       // The pages of several requests one behind the other: (where each request's begin, one item more than requests; the
       // pages, -1 where a window has given one back).

@@ -13,6 +13,7 @@ vocabulary, positions inside the model's reach, block tables that cover every po
 from __future__ import annotations
 
 from dataclasses import dataclass
+from itertools import accumulate
 from typing import Dict, List, Optional, Sequence
 
 import gc
@@ -47,9 +48,8 @@ def step_offsets(copied, built):
     """Where a step's pieces lie in its buffer, with the end behind them: those that are copied to the device, then, from a line of their own on,
     those that the device builds.  (Kernels read the latter in front of their wait, so no line of them may have been fetched by
     the kernel that builds them from the former.)"""
-    offsets = np.concatenate([[0], np.cumsum(copied)]).astype(np.int64).tolist()
-    first = -(-offsets[-1] // _LINE) * _LINE
-    return offsets, (first + np.concatenate([[0], np.cumsum(built)])).astype(np.int64).tolist()
+    offsets = list(accumulate(copied, initial=0))
+    return offsets, list(accumulate(built, initial=-(-offsets[-1] // _LINE) * _LINE))
 
 
 def _round_up_pow2(value: int, least: int = 8) -> int:
@@ -213,55 +213,42 @@ class ModelRunner:
         from ..kernels import ops
 
         self.validate(step)
-        counts = np.asarray(step.counts, dtype=np.int32)
-        pos0 = np.asarray(step.pos0, dtype=np.int32)
-        entries, total = counts.shape[0], int(counts.sum())
-        starts = np.zeros(entries + 1, dtype=np.int32)
-        np.cumsum(counts, out=starts[1:])
+        entries, total, requests = len(step.counts), int(step.tokens.shape[0]), list(step.requests)
+        host_counts, host_pos0 = [int(c) for c in step.counts], [int(p) for p in step.pos0]
+        max_len = max(first + count for first, count in zip(host_pos0, host_counts))
         rows = np.asarray(step.logit_rows, dtype=np.int32)
-        slots = np.asarray([self.manager.state_slot(r) for r in step.requests], dtype=np.int32)
-        max_len = int((pos0 + counts).max())
-        pieces = [step.tokens.astype(np.int32, copy=False), starts, pos0, slots, np.asarray(step.fresh, dtype=np.int32), rows]
-        widths = []
-        for g, page_size in enumerate(self._page_sizes):
-            page_starts, pages = self.manager.page_lists(list(step.requests), g)
-            # Every position of the step must have its page.
-            last = page_starts[:-1] + (pos0 + counts - 1) // page_size
-            if (last >= page_starts[1:]).any() or (pages[last] < 0).any():
-                raise InvalidArgumentError("a request of the step has no page reserved for its last position")
-            widths.append(_round_up_pow2(max((max_len + page_size - 1) // page_size, int(np.diff(page_starts).max()))))
-            pieces += [page_starts, pages]
-        # what the device builds lies behind what is copied: positions, the tokens' entries, the tables
-        offsets, places = step_offsets([p.shape[0] for p in pieces], [total, total] + [entries * width for width in widths])
-        host, dev = self._staging(places[-1])
+        host, dev = self._staging(1)
         if self._copy_pending:
             self._copy_done.synchronize()
-        view = host.numpy()
-        for piece, offset in zip(pieces, offsets):
-            view[offset:offset + piece.shape[0]] = piece
+        while True:
+            sizes, longest = self.manager.fill_step(requests, step.tokens, host_counts, host_pos0, step.fresh, rows, host.data_ptr(), host.numel())
+            widths = [_round_up_pow2(max(-(-max_len // page_size), held)) for page_size, held in zip(self._page_sizes, longest)]
+            # what the device builds lies behind what is copied: positions, the tokens' entries, the tables
+            built = [total, total] + [entries * width for width in widths]
+            offsets, places = step_offsets(sizes, built)
+            if places[-1] <= host.numel():
+                break
+            host, dev = self._staging(places[-1])
         copied = offsets[-1]
         dev[:copied].copy_(host[:copied], non_blocking=True)
         self._copy_done.record()
         self._copy_pending = True
-
-        def part(index, offsets=offsets):
-            return dev[offsets[index]:offsets[index + 1]]
-
-        positions, token_entry = part(0, places), part(1, places)
-        block_tables = [part(2 + g, places).view(entries, width) for g, width in enumerate(widths)]
+        parts = dev[:places[-1]].split_with_sizes([*sizes, places[0] - copied, *built])
+        positions, token_entry, *tables = parts[len(sizes) + 1:]
+        block_tables = [table.view(entries, width) for table, width in zip(tables, widths)]
         if not block_tables:     # nothing is kept in pages
-            ops.step_maps(part(1), part(2), page_size=1, block_table=dev[:0].view(entries, 0), positions=positions, token_entry=token_entry)
+            ops.step_maps(parts[1], parts[2], page_size=1, block_table=dev[:0].view(entries, 0), positions=positions, token_entry=token_entry)
         for g, table in enumerate(block_tables):
             per_token = {} if g else dict(positions=positions, token_entry=token_entry)
-            ops.step_maps(part(1), part(2), page_size=self._page_sizes[g], block_table=table, page_starts=part(6 + 2 * g),
-                          pages=part(7 + 2 * g), **per_token)
+            ops.step_maps(parts[1], parts[2], page_size=self._page_sizes[g], block_table=table, page_starts=parts[6 + 2 * g],
+                          pages=parts[7 + 2 * g], **per_token)
         return StepContext(
-            num_tokens=total, num_entries=entries, tokens=part(0), positions=positions, token_entry=token_entry,
-            entry_starts=part(1), entry_pos0=part(2), state_slots=part(3), fresh=part(4),
-            block_tables=block_tables, logit_rows=part(5) if rows.size else None, num_logit_rows=int(rows.size),
-            host_counts=[int(c) for c in counts], host_pos0=[int(p) for p in pos0],
-            max_count=int(counts.max()), max_kv_len=max_len, all_single=bool((counts == 1).all()),
-            any_single=bool((counts == 1).any()), dtype=self.model.dtype, workspace=self.workspace,
+            num_tokens=total, num_entries=entries, tokens=parts[0], positions=positions, token_entry=token_entry,
+            entry_starts=parts[1], entry_pos0=parts[2], state_slots=parts[3], fresh=parts[4],
+            block_tables=block_tables, logit_rows=parts[5] if rows.size else None, num_logit_rows=int(rows.size),
+            host_counts=host_counts, host_pos0=host_pos0,
+            max_count=max(host_counts), max_kv_len=max_len, all_single=max(host_counts) == 1,
+            any_single=1 in host_counts, dtype=self.model.dtype, workspace=self.workspace,
             logits_all_rows=bool(rows.size == total and np.array_equal(rows, np.arange(total))))
 
     def forward(self, ctx: StepContext) -> Optional[torch.Tensor]:

@@ -1221,8 +1221,8 @@ def rope_cache_q4(qkv: torch.Tensor, q_out: torch.Tensor, pages: Q4Pages, *, num
                   slots: Optional[torch.Tensor], rot_dims: Optional[int] = None) -> None:
     """As rope_cache, into pages of 4 bits: rotate q and k of a float32 product whose rows begin with (heads + 2 kv_heads) * d
     values (what follows is not read), write q to q_out [tokens, heads * d] and k and v, quantised, to their ``slots`` (int32, page *
-    page_size + place, from step_maps; a slot that is negative or outside the pool is not written).  Two tokens of a step do not
-    share a slot.  ``slots=None`` writes q alone.  Positions lie inside the tables.  Every product and sum of the rotation is
+    page_size + place, from step_maps; a slot that is negative or outside the pool is not written).  Two tokens of a step
+    share a slot only where they bring the same keys and values (as copies that pad a step do).  ``slots=None`` writes q alone.  Positions lie inside the tables.  Every product and sum of the rotation is
     rounded by itself in 32 bits."""
     fn = _function("cache_q4", "vipera_rope_cache_q4", _STORE_Q4_ARGS)
     _check_struct("cache_q4", "vipera_rope_cache_q4_params_size", _StoreQ4Params)
@@ -1346,7 +1346,8 @@ Q4_ROWS = {(torch.float32, 128): 8, (torch.float32, 64): 16, (torch.bfloat16, 12
 
 
 # bfloat16 portions of little work (rows times keys) and few requests are shared by the blocks of the kernel of any number of rows; the
-# tensor cores' kernel has a longer start and more behind it.  12 heads of 128, one request: 64 tokens behind 500 take 20 and 24
+# tensor cores' kernel has a longer start and more behind it.  A step with single tokens among them counts as one request's portions, however
+# many there are: the host does not know how many.  12 heads of 128, one request: 64 tokens behind 500 take 20 and 24
 # microseconds, 128 tokens 27 and 27, 16 behind 4,000 22 and 22, 64 41 and 33; eight requests of 4 behind 500 18 and 18, of 64 51 and 25.
 Q4_ROWS_WORK, Q4_ROWS_HALF, Q4_ROWS_PORTIONS = 1e6, 1.4, 2
 
@@ -1465,17 +1466,20 @@ def attention_q4(q: torch.Tensor, out: torch.Tensor, pages: Q4Pages, *, entry_st
                  gate: Optional[torch.Tensor] = None, gate_offset: int = 0, gate_per_head: bool = False, longest: int = 0,
                  settled: bool = False) -> None:
     """Causal grouped-query attention of every token of a step over its request's pages of 4 bits; q and out [tokens, heads * d],
-    bfloat16 or float32, the step described as for the other attentions.  ``max_keys``: no request sees more; ``all_single``: every
+    bfloat16 or float32, the step described as for the other attentions; every key that a token sees lies in a page that the block
+    table names.  ``max_keys``: no request sees more; ``all_single``: every
     entry brings one token; ``any_single``: some entry may.  ``window``, ``keep_first``, ``sink``, ``sink_values`` and the gate as
     for ``attention``, ``longest`` too.  ``settled``: positions, tables and the rows of earlier steps were complete before the kernel ahead of
-    this call was launched (as in a step whose description the host copied), so that they may be read while that kernel still runs.
+    this call was launched (as in a step whose description the host copied), so that they may be read while that kernel still runs;
+    lengths and tables always are, or that kernel is step_maps, which lets nothing begin before its end.
     ``workspace.get(name, shape, dtype)`` gives rooms that the call may use until it is
     done on its stream.
 
     With heads of 64 or 128 values and pages of a multiple of 16 tokens every kernel reads the packed pages: the single tokens' one, that of
     any number of rows (32-bit steps, short portions), the tensor cores' (other portions).  Elsewhere, and with VIPERA_ATTENTION_TC=0, the
     rows that the step sees are expanded to the run's type first (a room as large as one layer's pages in that type) and the kernels for
-    such pages attend."""
+    such pages attend.  Rows of q behind the last entry's tokens leave their rows of out as they were, but where the general kernel attends
+    (32-bit steps and other head sizes over expanded rows): it takes every row for a token of the entry that ``token_entry`` names."""
     page_size = _check_q4_pages("attention_q4", pages, num_kv_heads, head_dim)
     count, entries = q.shape[0], entry_pos0.numel()
     if num_kv_heads <= 0 or num_heads % num_kv_heads or q.shape != (count, num_heads * head_dim) or out.shape != q.shape \
