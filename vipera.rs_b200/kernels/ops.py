@@ -1221,9 +1221,9 @@ def rope_cache_q4(qkv: torch.Tensor, q_out: torch.Tensor, pages: Q4Pages, *, num
                   slots: Optional[torch.Tensor], rot_dims: Optional[int] = None) -> None:
     """As rope_cache, into pages of 4 bits: rotate q and k of a float32 product whose rows begin with (heads + 2 kv_heads) * d
     values (what follows is not read), write q to q_out [tokens, heads * d] and k and v, quantised, to their ``slots`` (int32, page *
-    page_size + place, from step_maps; a slot that is negative or outside the pool is not written).  Two tokens of a step
-    share a slot only where they bring the same keys and values (as copies that pad a step do).  ``slots=None`` writes q alone.  Positions lie inside the tables.  Every product and sum of the rotation is
-    rounded by itself in 32 bits."""
+    page_size + place, from step_maps; a slot that is negative or outside the pool is not written).  A slot that several
+    tokens of a step share holds pieces of any of them (copies that pad a step bring the same ones).  ``slots=None`` writes q alone.
+    Positions lie inside the tables.  Every product and sum of the rotation is rounded by itself in 32 bits."""
     fn = _function("cache_q4", "vipera_rope_cache_q4", _STORE_Q4_ARGS)
     _check_struct("cache_q4", "vipera_rope_cache_q4_params_size", _StoreQ4Params)
     page_size = _check_q4_pages("rope_cache_q4", pages, num_kv_heads, head_dim)
