@@ -148,3 +148,11 @@ def test_a_steps_pieces_are_written_one_behind_the_other_for_the_device():
             manager.fill_step(requests, tokens, given["counts"], given["pos0"], fresh, rows, buffer.ctypes.data, buffer.size)
     with pytest.raises(InvalidArgumentError):
         manager.fill_step(requests, tokens, counts[:2], pos0, fresh, rows, buffer.ctypes.data, buffer.size)
+
+
+def test_a_mixer_finds_the_view_of_packed_pages_beside_the_other_one():
+    import vipera_rs_b200  # noqa: F401
+    from vipera_rs_b200 import parts
+
+    for name in ("PagedKV", "PagedKVView", "PagedQ4View"):
+        assert name in parts.__all__ and hasattr(parts, name)

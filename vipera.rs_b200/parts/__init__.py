@@ -9,6 +9,7 @@ from .base import (
     Norm,
     PagedKV,
     PagedKVView,
+    PagedQ4View,
     Part,
     PositionEncoding,
     StateView,
@@ -20,6 +21,6 @@ from .linear import Linear, NormedInput, interleave_gate_up
 from .model import DecoderModel, model_schema
 
 __all__ = [
-    "CacheBundle", "FeedForward", "FixedState", "Mixer", "Norm", "PagedKV", "PagedKVView", "Part", "PositionEncoding",
+    "CacheBundle", "FeedForward", "FixedState", "Mixer", "Norm", "PagedKV", "PagedKVView", "PagedQ4View", "Part", "PositionEncoding",
     "StateView", "StepContext", "Workspace", "Block", "Linear", "NormedInput", "interleave_gate_up", "DecoderModel", "model_schema",
 ]
