@@ -178,3 +178,14 @@ def test_a_first_mixed_step_leaves_captured_steps_valid(ops, monkeypatch):
         _attend(ops, step, pages, q, 8, 2, 128, workspace=room)
         seen.append(room.generation)
     assert seen[0] == seen[1]
+
+
+@pytest.mark.parametrize("page_size", [16, 24])
+@pytest.mark.parametrize("per_head", [False, True])
+def test_a_sink_of_score_0_beside_a_gate(ops, form, page_size, per_head):
+    """No flash kernel has both endings: over expanded rows such a step is the general kernel's, and is not refused."""
+    from test_cache_q4_gpu import _attend as attend_and_compare
+
+    heads, d = 4, 64
+    gate = np.random.default_rng(9).standard_normal((60, heads * (1 if per_head else d))).astype(np.float32)
+    attend_and_compare(ops, Step([19, 1, 40], [33, 64, 0], page_size), torch.bfloat16, heads, 2, d, sink=True, gate=gate, gate_per_head=per_head)

@@ -1524,10 +1524,10 @@ def attention_q4(q: torch.Tensor, out: torch.Tensor, pages: Q4Pages, *, entry_st
             _attention_q4_decode(q, out, pages, positions=entry_pos0, block_table=block_table, max_keys=max_keys, workspace=workspace,
                                  settled=settled if beside is None else 2, beside=beside, entry_starts=entry_starts, **heads, **endings)
         return
-    # what the flash kernels know of endings decides whether portions are theirs (see parts/attention.py)
+    # what the flash kernels know of endings decides whether portions are theirs (a sink of score 0 and a gate are not one kernel's)
     extended = sink_values is not None or gate is not None
     flash = (rising and q.dtype == torch.bfloat16 and head_dim in MMA_HEAD_DIMS and
-             not (extended and (keep_first or head_dim not in TC_ATTENTION_HEAD_DIMS or os.environ.get("VIPERA_ATTENTION_TC", "1") == "0"
+             not (extended and (keep_first or (sink and sink_values is None) or head_dim not in TC_ATTENTION_HEAD_DIMS or os.environ.get("VIPERA_ATTENTION_TC", "1") == "0"
                                 or not attention_tc_takes_gate(gate, gate_offset, gate_per_head))))
     apart = flash and packed and any_single     # single tokens beside portions read the packed pages
     shape = (pages.k_codes.shape[0], page_size, num_kv_heads, head_dim)
